@@ -186,7 +186,7 @@ def prepare(case, seed):
             st["op"] = mla.MlaDecode(mla.MlaCache(st["pool"], rank), heads, nope, v, max_rows=len(lens) * new)
     else:
         nq, nk = _spans(case)
-        st = dict(cu_q=_offsets(nq), cu_k=_offsets(nk), max_q=max(nq))
+        st = dict(cu_q=_offsets(nq), cu_k=_offsets(nk))
         st["q"] = normal(sum(nq), heads, nope + rope, scale=2.0)
         st["kv"] = normal(sum(nk), heads, nope + v)
         st["rows"] = normal(sum(nk), rank + rope)  # the latent and the rotated key of each token, as appended
@@ -262,7 +262,7 @@ def _prefill(st):
     if own:
         from vib3_amd import mla
         return mla.mla_prefill(st["q"][..., :nope], st["q"][..., nope:], st["kv"], k_rope, st["cu_q"], st["cu_k"],
-                               max_q=st["max_q"], scale=st["scale"], out=st["out"])
+                               scale=st["scale"], out=st["out"])
     q0 = k0 = 0
     for nq, nk in zip(*_spans(case)):
         hidden = torch.arange(nk, device=DEV) > torch.arange(nq, device=DEV)[:, None] + (nk - nq)
