@@ -475,6 +475,124 @@ size_t vib3_moe_mxfp4_workspace_bytes(const vib3_moe_mxfp4_batch *batch);
 int vib3_launch_moe_mxfp4_batched(const vib3_moe_mxfp4_batch *batch, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Latent attention (MLA), the sublayer in front of the MoE block (additive launchers). A cached
+ * token is one row: the latent c[rank], which every head's key and value are expanded from, then
+ * the rotated key part kr[rope] that all heads share. The cache is a pool of pages of page_size
+ * rows; a sequence's token j is row j % page_size of page block_table[seq][j / page_size].
+ *
+ * For all three launchers: dtype is VIB3_DT_F16 or VIB3_DT_BF16; (rank, rope) are 256 or 512 and
+ * 32 or 64; strides are in elements and multiples of 8, tensor addresses are 16-byte aligned
+ * (VIB3_ERR_BAD_POINTER otherwise), and the innermost dimension of every tensor is contiguous.
+ * Index tensors are int32 on the device and read while the kernels run: an index that is out of
+ * its range is never followed (each launcher says what happens instead). Launches are safe inside
+ * HIP graph capture and keep no state between calls.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct vib3_mla_cache {
+    void *pool;                 /* [num_pages][page_size][rank + rope] */
+    int dtype;
+    int num_pages, page_size;   /* page_size 1..65536 */
+    int rank, rope;
+    int64_t page_stride, row_stride;
+    const int32_t *block_table; /* [num_seqs][max_pages] page numbers, contiguous; an entry
+                                   outside [0, num_pages) is a page that is not resident */
+    int num_seqs, max_pages;
+} vib3_mla_cache;
+
+/* New tokens into the cache. Token t is token positions[t] of sequence seqs[t]. With
+ * row = kv[t] (rank + rope values: the latent and the shared key as projected):
+ *   c  = row[:rank] * norm_weight / sqrt(mean(row[:rank]^2) + norm_eps)   (norm_weight NULL: as is)
+ *   kr = rot(row[rank:], positions[t]),
+ * stored as [c | kr] in the cache and, if kv_out is given, in kv_out[t]; if q_rope is given,
+ * q_out[t][h] = rot(q_rope[t][h]) (q_out may be q_rope itself). rot(x, p) turns the pair
+ * i (elements 2i and 2i + 1 if interleaved, else i and i + rope/2) by the angle
+ * p * inv_freq[i] (64-bit) and multiplies by rope_scale. Sums in f32, one rounding at the end.
+ * A token with seqs[t] outside [0, num_seqs) or a negative position is padding: nothing of it is
+ * written. A token whose page is not resident, or lies past max_pages, is not cached; its kv_out
+ * and q_out rows are written. The (sequence, position) pairs of a call must differ (of equal ones
+ * the cached row may be a mixture). */
+typedef struct vib3_mla_append {
+    vib3_mla_cache cache;
+    int tokens;
+    const int32_t *seqs, *positions;   /* [tokens] */
+    const void *kv;                    /* [tokens][rank + rope], kv_dtype f32, f16 or bf16 */
+    int kv_dtype;
+    int64_t kv_stride;
+    const void *norm_weight;           /* [rank] f16, or NULL */
+    float norm_eps;
+    const float *inv_freq;             /* [rope / 2] */
+    float rope_scale;
+    int interleaved;
+    const void *q_rope;                /* [tokens][heads][rope] in the cache's dtype, or NULL */
+    int heads;
+    int64_t q_token_stride, q_head_stride;
+    void *q_out;                       /* [tokens][heads][rope] in the cache's dtype */
+    int64_t q_out_token_stride, q_out_head_stride;
+    void *kv_out;                      /* [tokens][rank + rope] in the cache's dtype, or NULL */
+    int64_t kv_out_stride;
+} vib3_mla_append;
+
+int vib3_launch_mla_append(const vib3_mla_append *args, void *stream);
+
+/* Attention over the cache, absorbed form: row r is one query token of sequence seqs[r] and sees
+ * the first lens[r] cached tokens (several tokens of a sequence are several rows). With
+ * W_uk = kv_b[h][:nope], W_uv = kv_b[h][nope:]:
+ *   ql = q_nope[r][h] . W_uk;   s_j = scale * (ql . c_j + q_rope[r][h] . kr_j),   j < lens[r]
+ *   out[r][h] = W_uv . (sum_j softmax(s)_j c_j)
+ * kv_b NULL: q_nope holds ql ([rows][heads][rank]) and out receives the weighted latent
+ * ([rows][heads][rank]). Tokens on pages that are not resident are not seen; a row that sees no
+ * token (lens[r] <= 0, a sequence outside [0, num_seqs)) is zero; lens[r] beyond the block table
+ * counts as its capacity. Softmax statistics and sums in f32; ql, the probabilities and the
+ * weighted latent are rounded to the cache's dtype for the matrix cores. */
+typedef struct vib3_mla_decode {
+    vib3_mla_cache cache;
+    int rows, heads;                   /* rows <= 65536, heads 1..128 */
+    const int32_t *seqs;               /* [rows], or NULL: row r reads sequence r */
+    const int32_t *lens;               /* [rows] */
+    const void *q_nope;                /* [rows][heads][nope] (or [rank] without kv_b) */
+    int64_t q_nope_row_stride, q_nope_head_stride;
+    const void *q_rope;                /* [rows][heads][rope] */
+    int64_t q_rope_row_stride, q_rope_head_stride;
+    const void *kv_b;                  /* [heads][nope + v_dim][rank], contiguous, or NULL */
+    int nope, v_dim;                   /* multiples of 32, 32..256 (ignored without kv_b) */
+    float scale;
+    void *out;                         /* [rows][heads][v_dim] */
+    int64_t out_row_stride, out_head_stride;
+    void *workspace;                   /* vib3_mla_decode_workspace_bytes() bytes, 256-byte
+                                          aligned; calls that may overlap need one each */
+    size_t workspace_bytes;
+} vib3_mla_decode;
+
+size_t vib3_mla_decode_workspace_bytes(const vib3_mla_decode *args);
+int vib3_launch_mla_decode(const vib3_mla_decode *args, void *stream);
+
+/* Causal attention of whole prompts, expanded form. Sequence s has the queries
+ * [cu_q[s], cu_q[s+1]) and the keys [cu_k[s], cu_k[s+1]); with nq and nk of them, query i sees the
+ * keys j <= i + nk - nq (the queries are the newest tokens). A head's key is its nope part of kv
+ * and the shared k_rope, its value the rest of kv:
+ *   out[i][h] = sum_j softmax_j(scale * (q_nope . kv[j][h][:nope] + q_rope . k_rope[j])) kv[j][h][nope:]
+ * A query that sees no key is zero. Queries behind cu_q[num_seqs] are left as they were; offsets
+ * are cut to [0, q_tokens] and [0, k_tokens]. Probabilities are rounded to dtype for the matrix
+ * cores, statistics and sums are f32. */
+typedef struct vib3_mla_prefill {
+    int dtype, heads, nope, rope, v_dim; /* nope and v_dim 64 or 128 */
+    int num_seqs, q_tokens, k_tokens;
+    const int32_t *cu_q, *cu_k;        /* [num_seqs + 1] */
+    const void *q_nope;                /* [q_tokens][heads][nope] */
+    int64_t q_nope_token_stride, q_nope_head_stride;
+    const void *q_rope;                /* [q_tokens][heads][rope] */
+    int64_t q_rope_token_stride, q_rope_head_stride;
+    const void *kv;                    /* [k_tokens][heads][nope + v_dim] */
+    int64_t kv_token_stride, kv_head_stride;
+    const void *k_rope;                /* [k_tokens][rope] */
+    int64_t k_rope_stride;
+    float scale;
+    void *out;                         /* [q_tokens][heads][v_dim] */
+    int64_t out_token_stride, out_head_stride;
+} vib3_mla_prefill;
+
+int vib3_launch_mla_prefill(const vib3_mla_prefill *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * The .vib3 model file (host side; format.rs). The file is memory-mapped read-only; page data
  * is returned as host pointers into the mapping, for the caller to upload where its page pool
  * lives. vib3_build_page_table then writes the fused layer's page table from the catalog.

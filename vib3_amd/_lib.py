@@ -72,6 +72,61 @@ class MoeMxfp4Batch(C.Structure):
     ]
 
 
+class MlaCacheDesc(C.Structure):
+    """vib3_mla_cache (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("pool", C.c_void_p), ("dtype", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int),
+        ("rank", C.c_int), ("rope", C.c_int), ("page_stride", C.c_int64),
+        ("row_stride", C.c_int64), ("block_table", C.c_void_p), ("num_seqs", C.c_int),
+        ("max_pages", C.c_int),
+    ]
+
+
+class MlaAppendDesc(C.Structure):
+    """vib3_mla_append (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("cache", MlaCacheDesc), ("tokens", C.c_int), ("seqs", C.c_void_p),
+        ("positions", C.c_void_p), ("kv", C.c_void_p), ("kv_dtype", C.c_int),
+        ("kv_stride", C.c_int64), ("norm_weight", C.c_void_p), ("norm_eps", C.c_float),
+        ("inv_freq", C.c_void_p), ("rope_scale", C.c_float), ("interleaved", C.c_int),
+        ("q_rope", C.c_void_p), ("heads", C.c_int), ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("q_out", C.c_void_p), ("q_out_token_stride", C.c_int64),
+        ("q_out_head_stride", C.c_int64), ("kv_out", C.c_void_p), ("kv_out_stride", C.c_int64),
+    ]
+
+
+class MlaDecodeDesc(C.Structure):
+    """vib3_mla_decode (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("cache", MlaCacheDesc), ("rows", C.c_int), ("heads", C.c_int), ("seqs", C.c_void_p),
+        ("lens", C.c_void_p), ("q_nope", C.c_void_p), ("q_nope_row_stride", C.c_int64),
+        ("q_nope_head_stride", C.c_int64), ("q_rope", C.c_void_p),
+        ("q_rope_row_stride", C.c_int64), ("q_rope_head_stride", C.c_int64),
+        ("kv_b", C.c_void_p), ("nope", C.c_int), ("v_dim", C.c_int), ("scale", C.c_float),
+        ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class MlaPrefillDesc(C.Structure):
+    """vib3_mla_prefill (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("dtype", C.c_int), ("heads", C.c_int), ("nope", C.c_int), ("rope", C.c_int),
+        ("v_dim", C.c_int), ("num_seqs", C.c_int), ("q_tokens", C.c_int), ("k_tokens", C.c_int),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_nope", C.c_void_p),
+        ("q_nope_token_stride", C.c_int64), ("q_nope_head_stride", C.c_int64),
+        ("q_rope", C.c_void_p), ("q_rope_token_stride", C.c_int64),
+        ("q_rope_head_stride", C.c_int64), ("kv", C.c_void_p), ("kv_token_stride", C.c_int64),
+        ("kv_head_stride", C.c_int64), ("k_rope", C.c_void_p), ("k_rope_stride", C.c_int64),
+        ("scale", C.c_float), ("out", C.c_void_p), ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/vib3_hip.h
 P, I, F, S, U64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
 SIGNATURES = {
@@ -102,6 +157,10 @@ SIGNATURES = {
     "vib3_launch_moe_int4_layer_stage": (I, [C.POINTER(MoeInt4Layer), I, P]),
     "vib3_moe_mxfp4_workspace_bytes": (S, [C.POINTER(MoeMxfp4Batch)]),
     "vib3_launch_moe_mxfp4_batched": (I, [C.POINTER(MoeMxfp4Batch), P]),
+    "vib3_launch_mla_append": (I, [C.POINTER(MlaAppendDesc), P]),
+    "vib3_mla_decode_workspace_bytes": (S, [C.POINTER(MlaDecodeDesc)]),
+    "vib3_launch_mla_decode": (I, [C.POINTER(MlaDecodeDesc), P]),
+    "vib3_launch_mla_prefill": (I, [C.POINTER(MlaPrefillDesc), P]),
     "vib3_hip_zero": (I, [P, S, P]),
     "vib3_synth_bytes": (I, [P, S, U64, U64, S, P]),
     "vib3_synth_normal": (I, [P, I, S, U64, U64, S, F, P]),

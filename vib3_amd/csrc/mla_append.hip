@@ -1,0 +1,139 @@
+// mla_append.hip — new tokens into the paged latent cache: RMSNorm of the latent, rotation of the
+// shared key and of the queries' rotary part, in one launch.
+//
+// Bound: bytes for prompts (every value read and written once), the launch for single tokens.
+// A wave takes one kv row: lane l holds rank / 64 neighbouring latent elements, the sum of squares
+// is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the
+// rest takes (part of) the heads of one token: its first rope / 2 threads form the cosines and sines
+// once (the angle and its reduction in 64 bits: positions reach 10^6 radians, where f32 angles are
+// off by 0.03), and each thread turns eight pairs, 32 bytes, of one head at a time.
+#include "mla.h"
+
+namespace vib3 {
+
+struct AppendGrid {
+  int kv_blocks;    // workgroups of four kv rows
+  int splits;       // workgroups over one token's heads
+  int heads_each;   // heads of each of them
+};
+
+// Cosine and sine of p * inv_freq, times g.
+__device__ __forceinline__ float2 turn_of(int p, float inv_freq, float g) {
+  double t = (double)p * (double)inv_freq * 0.15915494309189535;  // turns
+  t -= __builtin_rint(t);
+  float s, c;
+  sincospif(2.0f * (float)t, &s, &c);
+  return make_float2(g * c, g * s);
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGrid grid) {
+  const int tid = (int)threadIdx.x;
+  const int rank = a.cache.rank, rope = a.cache.rope, half = rope / 2;
+  if ((int)blockIdx.x < grid.kv_blocks) {
+    const int t = (int)blockIdx.x * 4 + (tid >> 6), lane = tid & 63;
+    if (t >= a.tokens) return;
+    const int s = a.seqs[t], p = a.positions[t];
+    if ((unsigned)s >= (unsigned)a.cache.num_seqs || p < 0) return;
+    const size_t at = (size_t)t * a.kv_stride;
+    uint16_t* row = (uint16_t*)cache_row(a.cache, s, p);
+    uint16_t* copy = a.kv_out ? (uint16_t*)a.kv_out + (size_t)t * a.kv_out_stride : nullptr;
+    // the rotary pair of this lane (lanes past rope / 2 have none)
+    const int i0 = a.interleaved ? 2 * lane : lane, i1 = a.interleaved ? 2 * lane + 1 : lane + half;
+    float x0 = 0.0f, x1 = 0.0f;
+    if (lane < half) {
+      x0 = load_act(a.kv, a.kv_dtype, at + rank + i0);
+      x1 = load_act(a.kv, a.kv_dtype, at + rank + i1);
+    }
+    // latent: 8 (rank 512) or 4 elements a lane
+    const int n = rank >> 6;
+    float c[8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      c[i] = i < n ? load_act(a.kv, a.kv_dtype, at + (size_t)lane * n + i) : 0.0f;
+      ss = __builtin_fmaf(c[i], c[i], ss);
+    }
+    if (a.norm_weight) {
+      ss = wave_sum(ss);
+      const float inv = 1.0f / sqrtf(ss / (float)rank + a.norm_eps);
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < n) c[i] = c[i] * inv * f16_to_f32(((const uint16_t*)a.norm_weight)[lane * n + i]);
+    }
+    float2 cs = make_float2(0.0f, 0.0f);
+    if (lane < half) cs = turn_of(p, a.inv_freq[lane], a.rope_scale);
+    const uint16_t y0 = from_f32<DT>(x0 * cs.x - x1 * cs.y), y1 = from_f32<DT>(x0 * cs.y + x1 * cs.x);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      uint16_t* dst = k ? copy : row;
+      if (!dst) continue;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < n) dst[lane * n + i] = from_f32<DT>(c[i]);
+      if (lane < half) {
+        dst[rank + i0] = y0;
+        dst[rank + i1] = y1;
+      }
+    }
+    return;
+  }
+  // the queries' rotary part
+  const int b = (int)blockIdx.x - grid.kv_blocks;
+  const int t = b / grid.splits, h0 = (b - t * grid.splits) * grid.heads_each;
+  const int p = a.positions[t];
+  if ((unsigned)a.seqs[t] >= (unsigned)a.cache.num_seqs || p < 0) return;
+  __shared__ float2 cs[32];
+  if (tid < half) cs[tid] = turn_of(p, a.inv_freq[tid], a.rope_scale);
+  __syncthreads();
+  const int units = half / 8;  // threads on one head
+  const int h1 = min(a.heads, h0 + grid.heads_each);
+  const uint16_t* q = (const uint16_t*)a.q_rope + (int64_t)t * a.q_token_stride;
+  uint16_t* o = (uint16_t*)a.q_out + (int64_t)t * a.q_out_token_stride;
+  for (int u = tid; u < (h1 - h0) * units; u += 256) {
+    const int h = h0 + u / units, j = u % units;  // pairs 8j .. 8j + 7 of head h
+    const int e0 = a.interleaved ? 16 * j : 8 * j, e1 = a.interleaved ? 16 * j + 8 : 8 * j + half;
+    float x[16], y[16];
+    unpack8<DT>(*(const uint4*)(q + (int64_t)h * a.q_head_stride + e0), x);
+    unpack8<DT>(*(const uint4*)(q + (int64_t)h * a.q_head_stride + e1), x + 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float2 w = cs[8 * j + i];
+      const int k0 = a.interleaved ? 2 * i : i, k1 = a.interleaved ? 2 * i + 1 : i + 8;
+      y[k0] = x[k0] * w.x - x[k1] * w.y;
+      y[k1] = x[k0] * w.y + x[k1] * w.x;
+    }
+    *(uint4*)(o + (int64_t)h * a.q_out_head_stride + e0) = pack8<DT>(y);
+    *(uint4*)(o + (int64_t)h * a.q_out_head_stride + e1) = pack8<DT>(y + 8);
+  }
+}
+
+}  // namespace vib3
+
+using namespace vib3;
+
+extern "C" int vib3_launch_mla_append(const vib3_mla_append* args, void* stream) {
+  if (!args) return VIB3_ERR_BAD_POINTER;
+  const vib3_mla_append& a = *args;
+  if (const int rc = check_cache(a.cache)) return rc;
+  if (a.kv_dtype != VIB3_DT_F32 && !mla_dtype(a.kv_dtype)) return VIB3_ERR_UNSUPPORTED;
+  if (a.tokens < 0 || (a.q_rope && a.heads < 1)) return VIB3_ERR_BAD_COUNT;
+  if (a.tokens == 0) return 0;
+  if (!a.seqs || !a.positions || !a.inv_freq || !mla_aligned(a.kv) || !mla_stride(a.kv_stride))
+    return VIB3_ERR_BAD_POINTER;
+  if (a.norm_weight && !mla_aligned(a.norm_weight)) return VIB3_ERR_BAD_POINTER;
+  if (a.kv_out && (!mla_aligned(a.kv_out) || !mla_stride(a.kv_out_stride))) return VIB3_ERR_BAD_POINTER;
+  AppendGrid g{(a.tokens + 3) / 4, 1, 0};
+  int64_t blocks = g.kv_blocks;
+  if (a.q_rope) {
+    if (!mla_aligned(a.q_rope) || !mla_aligned(a.q_out) || !mla_stride(a.q_token_stride) || !mla_stride(a.q_head_stride) ||
+        !mla_stride(a.q_out_token_stride) || !mla_stride(a.q_out_head_stride))
+      return VIB3_ERR_BAD_POINTER;
+    g.heads_each = a.heads;
+    blocks += (int64_t)a.tokens * g.splits;
+  }
+  if (blocks > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
+  auto kernel = a.cache.dtype == VIB3_DT_F16 ? k_mla_append<VIB3_DT_F16> : k_mla_append<VIB3_DT_BF16>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, g);
+  VIB3_RETURN_LAUNCH();
+}
