@@ -60,9 +60,10 @@ __device__ __forceinline__ const uint16_t* cache_row(const vib3_mla_cache& c, in
   return (const uint16_t*)c.pool + (int64_t)id * c.page_stride + (int64_t)(j - page * c.page_size) * c.row_stride;
 }
 
-// Cached tokens that a row of lens[r] = n sees at most: the block table's capacity bounds n.
+// Cached tokens that a row of lens[r] = n sees at most: the block table's capacity bounds n (and 2^31 - 128, so
+// that a token's number plus a tile's width stays an int).
 __device__ __forceinline__ int clamp_len(const vib3_mla_cache& c, int n) {
-  const int64_t cap = (int64_t)c.max_pages * c.page_size;
+  const int64_t cap = min((int64_t)c.max_pages * c.page_size, (int64_t)0x7fffff80);
   return n <= 0 ? 0 : n > cap ? (int)cap : n;
 }
 
@@ -81,6 +82,68 @@ inline int check_cache(const vib3_mla_cache& c) {
   if (!mla_stride(c.page_stride) || !mla_stride(c.row_stride)) return VIB3_ERR_BAD_POINTER;
   if (c.row_stride < c.rank + c.rope || c.page_stride < 0) return VIB3_ERR_BAD_COUNT;
   return 0;
+}
+
+}  // namespace vib3
+
+namespace vib3 {
+
+// ------------------------------------------------------------------------- matrix cores
+//
+// Operand layouts of the 16x16 products: lane l holds row (A) or column (B) l % 16 at
+// k = 8 (l / 16) + 0..7 (k = 4 (l / 16) + 0..3 for the 16-deep one); of the result, column l % 16 of rows
+// 4 (l / 16) + 0..3.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma32(s16x8 a, s16x8 b, f32x4 c) {
+  if (DT == VIB3_DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma16(s16x4 a, s16x4 b, f32x4 c) {
+  if (DT == VIB3_DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+}
+
+// Two f32 rounded to a pair of 16-bit elements (nearest even).
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (DT == VIB3_DT_F16) return __builtin_bit_cast(uint32_t, h2{(half_t)a, (half_t)b});
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// 16 bytes a lane from global memory to LDS at base + 16 * lane (base wave-uniform), without passing
+// through registers; counted by vmcnt.
+__device__ __forceinline__ void load_to_lds16(const void* g, lds_u8* base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+__device__ __forceinline__ s16x8 lds_read16(const lds_u8* p) {
+  return *(const __attribute__((address_space(3))) s16x8*)p;
+}
+
+// Transposing read: 16 lanes address 4 rows of 16 elements (lane i: row i / 4, elements 4 (i % 4) + 0..3)
+// and lane i receives column i of the 4 rows.
+__device__ __forceinline__ s16x4 lds_read_tr(lds_u8* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
+__device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 }  // namespace vib3

@@ -1,89 +1,479 @@
 // mla_decode.hip — attention of single query tokens over the paged latent cache, absorbed form.
+//
+// Per row and head: ql = q_nope . W_uk, scores of every visible cached row against [ql | q_rope], softmax, the
+// weighted sum of the latents, out = W_uv . that. All heads share the cached rows, so a row of 1152 bytes
+// serves 64 heads x 2176 flops: at 64 heads the cache read and the matrix cores are of one order, and the read bounds.
+// Three launches:
+//   k_mla_absorb   ql for all rows, on the matrix cores; one more workgroup plans the next launch
+//   k_mla_attend   the attention in the latent space, over equal shares of all rows' cached tokens
+//   k_mla_finish   rows that several workgroups shared are joined, and W_uv applied
+//
+// The plan: tokens are taken 64 at a time (a unit). All units of all rows in order are cut into kShares
+// equal runs, one workgroup each, whatever the rows' lengths: a long row is shared by many workgroups, a run
+// covers many short rows. Nothing on the host depends on the lengths, so a captured launch follows them.
 #include "mla.h"
 
 namespace vib3 {
 
 constexpr int kMlaMaxRows = 65536;
+constexpr int kUnit = 64;      // cached tokens of one step
+constexpr int kShares = 256;   // workgroups of the attention launch, one per CU (its LDS tiles fill one)
+constexpr int kMinUnits = 1;   // units of a share at least
 
-// One workgroup per (row, head). The query goes into the latent space (thread c holds column c),
-// each wave then takes every fourth cached token with a softmax of its own (running maximum and
-// sum; lane l holds eight latent elements), the four waves are joined, and the weighted latent
-// goes through W_uv, a wave per output element.
+// Device workspace. Slot 2w holds the part of the row that share w starts in the middle of, or that it covers the
+// middle of; slot 2w + 1 the part of the row it ends in (if it starts that row).
+struct DecodeWs {
+  int64_t* head;      // [2]: units per share, all units
+  int64_t* prefix;    // [rows + 1] units before each row
+  int32_t* first;     // [kShares] row in which a share starts
+  uint16_t* ql;       // [rows][heads][rank]
+  uint16_t* ol;       // [rows][heads][rank] weighted latent of rows that one share covers
+  float* part;        // [2 kShares][heads][rank] unnormalised sums
+  float2* stat;       // [2 kShares][heads] running maximum (of scores in log2 units) and sum
+};
+
+inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return (uint8_t*)base + p;
+  };
+  const size_t row = (size_t)a.heads * a.cache.rank;
+  DecodeWs r;
+  r.head = (int64_t*)take(16);
+  r.prefix = (int64_t*)take(8 * ((size_t)a.rows + 1));
+  r.first = (int32_t*)take(4 * kShares);
+  r.ql = (uint16_t*)take(a.kv_b ? 2 * row * a.rows : 0);
+  r.ol = (uint16_t*)take(2 * row * a.rows);
+  r.part = (float*)take(4 * row * 2 * kShares);
+  r.stat = (float2*)take(8 * (size_t)a.heads * 2 * kShares);
+  if (w) *w = r;
+  return at;
+}
+
+struct DecodeArgs {
+  vib3_mla_decode a;
+  DecodeWs w;
+};
+
+// Visible cached tokens of row r and its sequence.
+__device__ __forceinline__ int row_len(const vib3_mla_decode& a, int r, int* seq) {
+  const int s = a.seqs ? a.seqs[r] : r;
+  *seq = s;
+  return (unsigned)s < (unsigned)a.cache.num_seqs ? clamp_len(a.cache, a.lens[r]) : 0;
+}
+
+// ------------------------------------------------------------------------- the plan
+
+// One workgroup of 256: running sums of the rows' units, the share size, and the row each share starts in.
+__device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
+  __shared__ int64_t wave_total[4];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  int64_t before = 0;
+  for (int r0 = 0; r0 < a.rows; r0 += 256) {
+    const int r = r0 + tid;
+    int seq;
+    const int64_t n = r < a.rows ? ((int64_t)row_len(a, r, &seq) + kUnit - 1) / kUnit : 0;
+    int64_t sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 63) wave_total[tid >> 6] = sum;
+    __syncthreads();
+    int64_t base = before;
+    for (int i = 0; i < 4; i++) {
+      if (i < (tid >> 6)) base += wave_total[i];
+      before += wave_total[i];
+    }
+    if (r < a.rows) w.prefix[r] = base + sum - n;
+    __syncthreads();
+  }
+  const int64_t per = max((int64_t)kMinUnits, (before + kShares - 1) / kShares);
+  if (tid == 0) {
+    w.prefix[a.rows] = before;
+    w.head[0] = per;
+    w.head[1] = before;
+  }
+  __syncthreads();
+  for (int r = tid; r < a.rows; r += 256) {
+    const int64_t lo = w.prefix[r], hi = w.prefix[r + 1];
+    for (int64_t s = (lo + per - 1) / per; s * per < hi; s++) w.first[s] = r;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_mla_plan(DecodeArgs d) { make_plan(d.a, d.w); }
+
+// ------------------------------------------------------------------------- ql = q_nope . W_uk
+
+constexpr int kAbsorbCols = 128;
+
+// A workgroup takes 128 latent columns of one head: that part of W_uk goes to LDS once, and 16 rows at a
+// time are multiplied by it as (W_uk^T) . (q^T), each wave 32 columns. W_uk lies with the latent columns contiguous, so
+// its operand is read transposed. LDS rows are 256 bytes; 16-byte chunk c of row n lies at c ^ swizzle(n), which
+// spreads a transposing read over the banks.
+__device__ __forceinline__ int absorb_swizzle(int n) { return ((n & 3) << 2) ^ (((n >> 3) & 1) << 1); }
+
 template <int DT>
-__global__ __launch_bounds__(256) void k_mla_decode(vib3_mla_decode a) {
-  const int r = (int)blockIdx.x, h = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int rank = a.cache.rank, rope = a.cache.rope;
-  __shared__ float q[512 + 64];
-  __shared__ float acc[4][512];
-  __shared__ float stat[4][2];
-  const uint16_t* qn = (const uint16_t*)a.q_nope + (int64_t)r * a.q_nope_row_stride + (int64_t)h * a.q_nope_head_stride;
-  const uint16_t* qr = (const uint16_t*)a.q_rope + (int64_t)r * a.q_rope_row_stride + (int64_t)h * a.q_rope_head_stride;
-  const uint16_t* w = (const uint16_t*)a.kv_b + (size_t)h * (a.nope + a.v_dim) * rank;
-  for (int c = tid; c < rank; c += 256) {
-    float s = 0.0f;
-    if (a.kv_b) {
-      for (int n = 0; n < a.nope; n++) s = __builtin_fmaf(to_f32<DT>(qn[n]), to_f32<DT>(w[(size_t)n * rank + c]), s);
-    } else {
-      s = to_f32<DT>(qn[c]);
-    }
-    q[c] = s;
-  }
-  if (tid < rope) q[rank + tid] = to_f32<DT>(qr[tid]);
-  __syncthreads();
-  const int seq = a.seqs ? a.seqs[r] : r;
-  const int len = (unsigned)seq < (unsigned)a.cache.num_seqs ? clamp_len(a.cache, a.lens[r]) : 0;
-  const bool mine = lane * 8 < rank;
-  float m = -__builtin_huge_valf(), l = 0.0f, o[8] = {};
-  for (int j = wave; j < len; j += 4) {
-    const uint16_t* row = cache_row(a.cache, seq, j);
-    if (!row) continue;
-    float c[8], s = 0.0f;
-    if (mine) {
-      unpack8<DT>(*(const uint4*)(row + lane * 8), c);
-      for (int i = 0; i < 8; i++) s = __builtin_fmaf(c[i], q[lane * 8 + i], s);
-    }
-    if (lane < rope) s = __builtin_fmaf(to_f32<DT>(row[rank + lane]), q[rank + lane], s);
-    s = wave_sum(s) * a.scale;
-    const float mn = fmaxf(m, s), base = mn == -__builtin_huge_valf() ? 0.0f : mn;
-    const float f = expf(m - base), p = expf(s - base);
-    l = l * f + p;
-    if (mine)
-      for (int i = 0; i < 8; i++) o[i] = o[i] * f + p * c[i];
-    m = mn;
-  }
-  if (mine)
-    for (int i = 0; i < 8; i++) acc[wave][lane * 8 + i] = o[i];
-  if (lane == 0) {
-    stat[wave][0] = m;
-    stat[wave][1] = l;
-  }
-  __syncthreads();
-  float mm = fmaxf(fmaxf(stat[0][0], stat[1][0]), fmaxf(stat[2][0], stat[3][0]));
-  if (mm == -__builtin_huge_valf()) mm = 0.0f;
-  float f[4], sum = 0.0f;
-  for (int i = 0; i < 4; i++) {
-    f[i] = expf(stat[i][0] - mm);
-    sum += f[i] * stat[i][1];
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int c = tid; c < rank; c += 256)
-    q[c] = (f[0] * acc[0][c] + f[1] * acc[1][c] + f[2] * acc[2][c] + f[3] * acc[3][c]) * inv;
-  __syncthreads();
-  uint16_t* out = (uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride;
-  if (!a.kv_b) {
-    for (int c = tid; c < rank; c += 256) out[c] = from_f32<DT>(q[c]);
+__global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks) {
+  const vib3_mla_decode& a = d.a;
+  __shared__ __align__(16) uint8_t tile[256 * kAbsorbCols * 2];
+  if ((int)blockIdx.x == a.heads * col_blocks) {
+    if (blockIdx.y == 0) make_plan(a, d.w);
     return;
   }
-  for (int v = wave; v < a.v_dim; v += 4) {
-    float s = 0.0f;
-    if (mine) {
-      float x[8];
-      unpack8<DT>(*(const uint4*)(w + (size_t)(a.nope + v) * rank + lane * 8), x);
-      for (int i = 0; i < 8; i++) s = __builtin_fmaf(x[i], q[lane * 8 + i], s);
-    }
-    s = wave_sum(s);
-    if (lane == 0) out[v] = from_f32<DT>(s);
+  const int h = (int)blockIdx.x / col_blocks, c0 = ((int)blockIdx.x % col_blocks) * kAbsorbCols;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rank = a.cache.rank;
+  const uint16_t* w = (const uint16_t*)a.kv_b + (size_t)h * (a.nope + a.v_dim) * rank + c0;
+  for (int i = wave; i < a.nope / 4; i += 4) {  // four rows of W_uk at a time
+    const int n = 4 * i + (lane >> 4), c = (lane & 15) ^ absorb_swizzle(n);
+    load_to_lds16(w + (size_t)n * rank + 8 * c, (lds_u8*)tile + i * 1024);
   }
+  const int row = lane & 15, g = lane >> 4;
+  // this lane's element of a transposing read: row 8 g + row / 4 (+ 4), columns 16 blk + 4 (row % 4)
+  const int n0 = 8 * g + (row >> 2);
+  const int part = 8 * (row & 1);
+  const int r_end = min(a.rows, ((int)blockIdx.y + 1) * 64);
+  __syncthreads();
+  for (int r0 = (int)blockIdx.y * 64; r0 < r_end; r0 += 16) {
+    const int r = min(r0 + row, a.rows - 1);
+    const uint16_t* q = (const uint16_t*)a.q_nope + (int64_t)r * a.q_nope_row_stride + (int64_t)h * a.q_nope_head_stride;
+    f32x4 acc[2] = {};
+    for (int k = 0; k < a.nope; k += 32) {
+      const s16x8 b = *(const s16x8*)(q + k + 8 * g);
+#pragma unroll
+      for (int blk = 0; blk < 2; blk++) {
+        const int c = (wave * 2 + blk) * 2 + ((row & 3) >> 1);
+        const int na = k + n0, nb = na + 4;
+        const s16x4 lo = lds_read_tr((lds_u8*)tile + na * 256 + (c ^ absorb_swizzle(na)) * 16 + part);
+        const s16x4 hi = lds_read_tr((lds_u8*)tile + nb * 256 + (c ^ absorb_swizzle(nb)) * 16 + part);
+        acc[blk] = mma32<DT>(join(lo, hi), b, acc[blk]);
+      }
+    }
+    if (r0 + row < a.rows) {
+      uint16_t* o = d.w.ql + ((size_t)(r0 + row) * a.heads + h) * rank + c0 + wave * 32 + 4 * g;
+#pragma unroll
+      for (int blk = 0; blk < 2; blk++)  // rounded for the matrix cores: relative error half a step
+        *(uint2*)(o + 16 * blk) = make_uint2(pack2<DT>(acc[blk][0], acc[blk][1]), pack2<DT>(acc[blk][2], acc[blk][3]));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------- attention in the latent space
+
+// What masked tokens read instead of the cache: their probability is 0, and 0 times whatever lies there must be 0.
+__device__ const uint4 zero_row[(512 + 64) / 8] = {};
+
+// Shapes of a workgroup for HB blocks of 16 heads. A wave owns 16 heads and the whole latent width of their sums; where
+// heads are few, the waves split a unit's tokens instead (TS groups, each with a softmax of its own, joined at the end).
+template <int HB>
+struct AttendShape {
+  static constexpr int kWaves = HB == 1 ? 4 : 8;
+  static constexpr int kTS = kWaves / HB;         // 4, 4, 2, 1
+  static constexpr int kTok = kUnit / kTS;        // tokens of a wave's share of a unit: 16, 16, 32, 64
+};
+
+// Scores are formed transposed, S^T = K . Q^T, so that a lane holds one head's scores of 4 tokens per 16: as the
+// matrix cores' B operand of the second product, O^T = C^T . P^T, that is already the layout needed (the tokens' order along k
+// is free as long as C^T is read in the same one), and the running maximum, the sum and the rescaling are per lane.
+// C^T is read from the same LDS rows by transposing reads.
+//
+// A unit's rows go from the pages straight to LDS (16 bytes a lane), double-buffered: while one unit is
+// worked on, the next is in flight (74 KB a CU, 19 MB over the chip). A row's 16-byte chunk c lies at c ^ f(row)
+// (f = (row / 2) % 8, rows 32 banks apart; for widths of 4 chunks modulo 8 (row / 4) % 4, rows 16 banks apart), which
+// spreads the row-wise and the transposing reads over all 64 banks.
+template <int DT, int R, int P, int HB>
+__global__ __launch_bounds__(AttendShape<HB>::kWaves * 64) void k_mla_attend(DecodeArgs d) {
+  using Sh = AttendShape<HB>;
+  constexpr int kWaves = Sh::kWaves, kTS = Sh::kTS, kTok = Sh::kTok;
+  constexpr int W = R + P, CH = W / 8, kRowBytes = W * 2;
+  constexpr int kMask = CH % 8 == 0 ? 7 : 3, kShift = CH % 8 == 0 ? 1 : 2;
+  constexpr int kTpw = kUnit / kWaves;                 // rows a wave loads
+  constexpr int kLoads = (kTpw * CH + 63) / 64;
+  constexpr int kTile = kUnit * kRowBytes;
+  constexpr int NB = kTok / 16;                        // token blocks of a wave's scores
+  constexpr int CB = R / 16;                           // column blocks of a wave's sums
+  __shared__ __align__(1024) uint8_t tile[2 * kTile];
+  __shared__ __align__(16) float seen[2][kUnit];       // 1: the token is seen
+  __shared__ float2 stats[kWaves][64];
+
+  const vib3_mla_decode& a = d.a;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = lane >> 4, col = lane & 15;
+  const int hb = wave % HB, ts = wave / HB;
+  const int head = hb * 16 + col;
+  const float to_log2 = a.scale * 1.44269504088896341f;
+
+  const int64_t per = d.w.head[0], all = d.w.head[1];
+  const int64_t begin = (int64_t)blockIdx.x * per, end = min(begin + per, all);
+  if (begin >= end) return;
+  int r = d.w.first[blockIdx.x];
+
+  // LDS offsets of this lane within a tile: rows 16 b + col of this wave's tokens for the scores, rows 16 b + 4 g + col / 4 for
+  // the transposing reads (16 rows further the swizzle is the same)
+  const int krow = ts * kTok + col, vrow = ts * kTok + 4 * g + (col >> 2);
+  const int kf = (krow >> kShift) & kMask, vf = (vrow >> kShift) & kMask;
+
+  for (int64_t u0 = begin; u0 < end; r++) {
+    const int64_t row_begin = d.w.prefix[r], row_end = d.w.prefix[r + 1];
+    const int64_t u1 = min(end, row_end);
+    if (u1 <= u0) continue;
+    int seq;
+    const int len = row_len(a, r, &seq);
+    const int32_t* table = a.cache.block_table + (size_t)seq * a.cache.max_pages;
+    const int first_unit = (int)(u0 - row_begin), units = (int)(u1 - u0);
+
+    // token of unit n whose row this lane finds the address of (lanes < kTpw), and its page's number
+    auto page_of = [&](int n) {
+      const int j = (first_unit + n) * kUnit + wave * kTpw + lane;
+      return lane < kTpw && n < units && j < len ? table[j / a.cache.page_size] : -1;
+    };
+    auto issue = [&](int n, int id) {
+      const int j = (first_unit + n) * kUnit + wave * kTpw + lane;
+      const bool ok = (unsigned)id < (unsigned)a.cache.num_pages;
+      const uint16_t* p = (const uint16_t*)zero_row;
+      if (ok)
+        p = (const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
+            (int64_t)(j % a.cache.page_size) * a.cache.row_stride;
+      if (lane < kTpw) seen[n & 1][wave * kTpw + lane] = ok ? 1.0f : 0.0f;
+      const int lo = (int)(uint32_t)(uintptr_t)p, hi = (int)(uint32_t)((uintptr_t)p >> 32);
+      lds_u8* base = (lds_u8*)tile + (n & 1) * kTile + wave * kTpw * kRowBytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int slot = i * 64 + lane, t = slot / CH;
+        const int c = (slot - t * CH) ^ (((wave * kTpw + t) >> kShift) & kMask);
+        const uint64_t at = (uint32_t)__shfl(lo, t) | ((uint64_t)(uint32_t)__shfl(hi, t) << 32);
+        if (kTpw * CH % 64 == 0 || slot < kTpw * CH) load_to_lds16((const uint8_t*)(uintptr_t)at + c * 16, base + i * 1024);
+      }
+    };
+
+    // queries: the B operand, this lane's head at k = 32 s + 8 g
+    s16x8 q[W / 32];
+    {
+      const int64_t hh = min(head, a.heads - 1);
+      const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + hh) * R
+                                  : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + hh * a.q_nope_head_stride;
+      const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + hh * a.q_rope_head_stride;
+#pragma unroll
+      for (int s = 0; s < W / 32; s++) q[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
+    }
+    f32x4 o[CB] = {};
+    float m = -__builtin_huge_valf(), l = 0.0f;
+
+    int id = page_of(0);
+    __syncthreads();  // the last row's tiles are done with
+    issue(0, id);
+    id = page_of(1);
+    for (int n = 0; n < units; n++) {
+      __syncthreads();  // unit n is in LDS; everyone is past unit n - 1
+      if (n + 1 < units) {
+        issue(n + 1, id);
+        id = page_of(n + 2);
+      }
+      lds_u8* t = (lds_u8*)tile + (n & 1) * kTile;
+      f32x4 s[NB] = {};
+#pragma unroll
+      for (int k = 0; k < W / 32; k++) {
+        const int c = ((4 * k + g) & ~kMask) | (((4 * k + g) & kMask) ^ kf);
+#pragma unroll
+        for (int b = 0; b < NB; b++) s[b] = mma32<DT>(lds_read16(t + (krow + 16 * b) * kRowBytes + c * 16), q[k], s[b]);
+      }
+      float top = -__builtin_huge_valf();
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const float4 v = *(const float4*)&seen[n & 1][ts * kTok + 16 * b + 4 * g];
+        const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          s[b][i] = vv[i] != 0.0f ? s[b][i] * to_log2 : -__builtin_huge_valf();
+          top = fmaxf(top, s[b][i]);
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top), base = mn == -__builtin_huge_valf() ? 0.0f : mn;
+      if (__any(mn != m)) {
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < CB; c++) o[c] *= f;
+        m = mn;
+      }
+      uint2 p[NB];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          e[i] = __builtin_amdgcn_exp2f(s[b][i] - base);
+          l += e[i];
+        }
+        // rounded for the matrix cores; the sum l takes them unrounded
+        p[b] = make_uint2(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
+      }
+#pragma unroll
+      for (int c = 0; c < CB; c++) {
+        const int ch = 2 * c + ((col & 3) >> 1);
+        lds_u8* v = t + vrow * kRowBytes + ((ch & ~kMask) | ((ch & kMask) ^ vf)) * 16 + 8 * (col & 1);
+        if (NB == 1) {
+          o[c] = mma16<DT>(lds_read_tr(v), __builtin_bit_cast(s16x4, p[0]), o[c]);
+        } else {
+#pragma unroll
+          for (int b = 0; b + 1 < NB; b += 2)
+            o[c] = mma32<DT>(join(lds_read_tr(v + 16 * b * kRowBytes), lds_read_tr(v + 16 * (b + 1) * kRowBytes)),
+                             join(__builtin_bit_cast(s16x4, p[b]), __builtin_bit_cast(s16x4, p[b + 1])), o[c]);
+        }
+      }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // join the token groups, halving: the upper half hands its sums over through LDS
+#pragma unroll
+    for (int half = kTS / 2; half >= 1; half /= 2) {
+      __syncthreads();
+      float4* box = (float4*)tile + (size_t)(((ts - half) * HB + hb) * CB) * 64 + lane;
+      if (ts >= half && ts < 2 * half) {
+        stats[wave][lane] = make_float2(m, l);
+#pragma unroll
+        for (int c = 0; c < CB; c++) box[c * 64] = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
+      }
+      __syncthreads();
+      if (ts < half) {
+        box += half * HB * CB * 64;
+        const float2 x = stats[wave + half * HB][lane];
+        const float mn = fmaxf(m, x.x), base = mn == -__builtin_huge_valf() ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(x.x - base);
+        l = l * f0 + x.y * f1;
+#pragma unroll
+        for (int c = 0; c < CB; c++) {
+          const float4 y = box[c * 64];
+          o[c] = o[c] * f0 + f32x4{y.x, y.y, y.z, y.w} * f1;
+        }
+        m = mn;
+      }
+    }
+    if (ts == 0 && head < a.heads) {
+      if (u0 == row_begin && u1 == row_end) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* out = d.w.ol + ((size_t)r * a.heads + head) * R + 4 * g;
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+          *(uint2*)(out + 16 * c) = make_uint2(pack2<DT>(o[c][0] * inv, o[c][1] * inv), pack2<DT>(o[c][2] * inv, o[c][3] * inv));
+      } else {
+        const size_t slot = 2 * (size_t)blockIdx.x + (u0 == begin ? 0 : 1);
+        float* out = d.w.part + (slot * a.heads + head) * R + 4 * g;
+#pragma unroll
+        for (int c = 0; c < CB; c++) *(float4*)(out + 16 * c) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
+        if (g == 0) d.w.stat[slot * a.heads + head] = make_float2(m, l);
+      }
+    }
+    u0 = u1;
+  }
+}
+
+// ------------------------------------------------------------------------- joined rows and W_uv
+
+// A workgroup takes 16 rows of one head: their weighted latents (joined from the shares' parts where a row
+// has several) go to LDS in 16 bits, and each wave multiplies them by 16 rows of W_uv at a time. Without W_uv
+// the weighted latents are the result.
+template <int DT, int R>
+__global__ __launch_bounds__(256) void k_mla_finish(DecodeArgs d) {
+  const vib3_mla_decode& a = d.a;
+  constexpr int kStride = R + 8;  // 16 bytes more: rows start in different banks
+  __shared__ __align__(16) uint16_t lat[16 * kStride];
+  const int h = (int)blockIdx.x, r0 = (int)blockIdx.y * 16;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t per = d.w.head[0];
+  constexpr int kCols = R / 64;  // columns of a lane: one wave joins a row
+  for (int i = wave; i < 16; i += 4) {
+    const int r = r0 + i;
+    uint16_t* dst = lat + i * kStride + lane * kCols;
+    float o[kCols] = {};
+    const int64_t lo = r < a.rows ? d.w.prefix[r] : 0, hi = r < a.rows ? d.w.prefix[r + 1] : 0;
+    if (hi > lo) {
+      const int64_t w0 = lo / per, w1 = (hi - 1) / per;
+      if (w0 == w1) {
+        const uint16_t* p = d.w.ol + ((size_t)r * a.heads + h) * R + lane * kCols;
+#pragma unroll
+        for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
+      } else {
+        float m = -__builtin_huge_valf(), l = 0.0f;
+        for (int64_t w = w0; w <= w1; w++) {
+          const size_t at = (2 * (size_t)w + (w == w0 && lo != w * per ? 1 : 0)) * a.heads + h;
+          const float2 s = d.w.stat[at];
+          const float* p = d.w.part + at * R + lane * kCols;
+          const float mn = fmaxf(m, s.x), base = mn == -__builtin_huge_valf() ? 0.0f : mn;
+          const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(s.x - base);
+          l = l * f0 + s.y * f1;
+#pragma unroll
+          for (int c = 0; c < kCols; c++) o[c] = o[c] * f0 + p[c] * f1;
+          m = mn;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int c = 0; c < kCols; c++) o[c] *= inv;
+      }
+    }
+    if (a.kv_b) {
+#pragma unroll
+      for (int c = 0; c < kCols; c++) dst[c] = from_f32<DT>(o[c]);
+    } else if (r < a.rows) {
+      uint16_t* out = (uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + lane * kCols;
+#pragma unroll
+      for (int c = 0; c < kCols; c++) out[c] = from_f32<DT>(o[c]);
+    }
+  }
+  if (!a.kv_b) return;
+  __syncthreads();
+  const int g = lane >> 4, n = lane & 15;
+  for (int v0 = wave * 16; v0 < a.v_dim; v0 += 64) {
+    const uint16_t* w = (const uint16_t*)a.kv_b + ((size_t)h * (a.nope + a.v_dim) + a.nope + v0 + n) * R;
+    f32x4 acc = {};
+#pragma unroll
+    for (int k = 0; k < R; k += 32)  // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
+      acc = mma32<DT>(*(const s16x8*)(w + k + 8 * g), *(const s16x8*)(lat + n * kStride + k + 8 * g), acc);
+    const int r = r0 + n;
+    if (r < a.rows)
+      *(uint2*)((uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + v0 + 4 * g) =
+          make_uint2(pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3]));
+  }
+}
+
+template <int DT, int R, int P>
+int launch_decode(const DecodeArgs& d, hipStream_t st) {
+  const vib3_mla_decode& a = d.a;
+  if (a.kv_b) {
+    const int col_blocks = R / kAbsorbCols;
+    hipLaunchKernelGGL(k_mla_absorb<DT>, dim3((unsigned)(a.heads * col_blocks + 1), (unsigned)((a.rows + 63) / 64)), dim3(256), 0, st,
+                       d, col_blocks);
+  } else {
+    hipLaunchKernelGGL(k_mla_plan, dim3(1), dim3(256), 0, st, d);
+  }
+  if (a.heads <= 16)
+    hipLaunchKernelGGL((k_mla_attend<DT, R, P, 1>), dim3(kShares), dim3(256), 0, st, d);
+  else if (a.heads <= 32)
+    hipLaunchKernelGGL((k_mla_attend<DT, R, P, 2>), dim3(kShares), dim3(512), 0, st, d);
+  else if (a.heads <= 64)
+    hipLaunchKernelGGL((k_mla_attend<DT, R, P, 4>), dim3(kShares), dim3(512), 0, st, d);
+  else
+    hipLaunchKernelGGL((k_mla_attend<DT, R, P, 8>), dim3(kShares), dim3(512), 0, st, d);
+  hipLaunchKernelGGL((k_mla_finish<DT, R>), dim3((unsigned)a.heads, (unsigned)((a.rows + 15) / 16)), dim3(256), 0, st, d);
+  VIB3_RETURN_LAUNCH();
+}
+
+template <int DT>
+int launch_decode_dt(const DecodeArgs& d, hipStream_t st) {
+  if (d.a.cache.rank == 512)
+    return d.a.cache.rope == 64 ? launch_decode<DT, 512, 64>(d, st) : launch_decode<DT, 512, 32>(d, st);
+  return d.a.cache.rope == 64 ? launch_decode<DT, 256, 64>(d, st) : launch_decode<DT, 256, 32>(d, st);
+}
+
+bool decode_counts(const vib3_mla_decode& a) {
+  return a.rows >= 0 && a.rows <= kMlaMaxRows && a.heads >= 1 && a.heads <= 128;
 }
 
 }  // namespace vib3
@@ -91,15 +481,17 @@ __global__ __launch_bounds__(256) void k_mla_decode(vib3_mla_decode a) {
 using namespace vib3;
 
 extern "C" size_t vib3_mla_decode_workspace_bytes(const vib3_mla_decode* args) {
-  if (!args || args->rows < 0 || args->rows > kMlaMaxRows || args->heads < 1 || args->heads > 128) return 0;
-  return 256;
+  if (!args || !decode_counts(*args) || (args->cache.rank != 256 && args->cache.rank != 512)) return 0;
+  vib3_mla_decode a = *args;
+  a.kv_b = &a;  // the larger of the two forms
+  return decode_ws(a, nullptr, nullptr);
 }
 
 extern "C" int vib3_launch_mla_decode(const vib3_mla_decode* args, void* stream) {
   if (!args) return VIB3_ERR_BAD_POINTER;
   const vib3_mla_decode& a = *args;
   if (const int rc = check_cache(a.cache)) return rc;
-  if (a.rows < 0 || a.rows > kMlaMaxRows || a.heads < 1 || a.heads > 128) return VIB3_ERR_BAD_COUNT;
+  if (!decode_counts(a)) return VIB3_ERR_BAD_COUNT;
   if (a.kv_b && (a.nope < 32 || a.nope > 256 || a.nope % 32 || a.v_dim < 32 || a.v_dim > 256 || a.v_dim % 32))
     return VIB3_ERR_UNSUPPORTED;
   if (a.rows == 0) return 0;
@@ -109,7 +501,9 @@ extern "C" int vib3_launch_mla_decode(const vib3_mla_decode* args, void* stream)
       !mla_stride(a.out_head_stride) || !a.workspace || ((uintptr_t)a.workspace & 255))
     return VIB3_ERR_BAD_POINTER;
   if (a.workspace_bytes < vib3_mla_decode_workspace_bytes(args)) return VIB3_ERR_WORKSPACE;
-  auto kernel = a.cache.dtype == VIB3_DT_F16 ? k_mla_decode<VIB3_DT_F16> : k_mla_decode<VIB3_DT_BF16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows, (unsigned)a.heads), dim3(256), 0, (hipStream_t)stream, a);
-  VIB3_RETURN_LAUNCH();
+  DecodeArgs d;
+  d.a = a;
+  decode_ws(a, &d.w, a.workspace);
+  return a.cache.dtype == VIB3_DT_F16 ? launch_decode_dt<VIB3_DT_F16>(d, (hipStream_t)stream)
+                                      : launch_decode_dt<VIB3_DT_BF16>(d, (hipStream_t)stream);
 }
