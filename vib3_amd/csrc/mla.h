@@ -126,14 +126,26 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 // 16 bytes a lane from global memory to LDS at base + 16 * lane (base wave-uniform), without passing
-// through registers; counted by vmcnt.
+// through registers. Written as an instruction because the compiler lets every LDS read wait for every such load in
+// flight, also those into another buffer; it has no result register, and it is counted by vmcnt, which the caller waits
+// for (wait_lds_loads) before the barrier that publishes the tile. Waits that the compiler places for its own loads only come out
+// stricter by it.
 __device__ __forceinline__ void load_to_lds16(const void* g, lds_u8* base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(g) : "memory", "m0");
+}
+
+__device__ __forceinline__ void wait_lds_loads() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 __device__ __forceinline__ s16x8 lds_read16(const lds_u8* p) {
   return *(const __attribute__((address_space(3))) s16x8*)p;
+}
+
+__device__ __forceinline__ void lds_write8(lds_u8* p, uint32_t a, uint32_t b) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  *(__attribute__((address_space(3))) u32x2*)p = u32x2{a, b};
 }
 
 // Transposing read: 16 lanes address 4 rows of 16 elements (lane i: row i / 4, elements 4 (i % 4) + 0..3)
