@@ -23,10 +23,21 @@ constexpr int kMinUnits = 1;   // units of a share at least
 
 // Device workspace. Slot 2w holds the part of the item that share w starts in the middle of, or that it covers the
 // middle of; slot 2w + 1 the part of the item it ends in (if it starts that item).
+struct Item {
+  int64_t begin;      // units before the item
+  int32_t len, seq;   // visible tokens of its row, and their sequence
+};
+
+struct Share {        // what a workgroup starts with
+  int64_t total;      // its units
+  int32_t item, seq, len, unit, left;  // the first item, its units before the share and in it
+  int32_t pad;
+};
+
 struct DecodeWs {
   int64_t* head;      // [2]: units per share, all units
-  int64_t* prefix;    // [items + 1] units before each item
-  int32_t* first;     // [kShares] item in which a share starts
+  Item* items;        // [items + 1]
+  Share* shares;      // [kShares]
   uint16_t* ql;       // [rows][heads][rank]
   uint16_t* ol;       // [rows][heads][rank] weighted latent of items that one share covers
   float* part;        // [2 kShares][heads of a group][rank] unnormalised sums
@@ -46,8 +57,8 @@ inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   const size_t row = (size_t)a.heads * a.cache.rank;
   DecodeWs r;
   r.head = (int64_t*)take(16);
-  r.prefix = (int64_t*)take(8 * ((size_t)a.rows * head_groups(a.heads) + 1));
-  r.first = (int32_t*)take(4 * kShares);
+  r.items = (Item*)take(sizeof(Item) * ((size_t)a.rows * head_groups(a.heads) + 1));
+  r.shares = (Share*)take(sizeof(Share) * kShares);
   r.ql = (uint16_t*)take(a.kv_b ? 2 * row * a.rows : 0);
   r.ol = (uint16_t*)take(2 * row * a.rows);
   r.part = (float*)take(4 * (size_t)group_heads(a.heads) * a.cache.rank * 2 * kShares);
@@ -78,8 +89,9 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
   int64_t before = 0;
   for (int x0 = 0; x0 < items; x0 += 256) {
     const int x = x0 + tid;
-    int seq;
-    const int64_t n = x < items ? ((int64_t)row_len(a, x / groups, &seq) + kUnit - 1) / kUnit : 0;
+    int seq = 0;
+    const int len = x < items ? row_len(a, x / groups, &seq) : 0;
+    const int64_t n = ((int64_t)len + kUnit - 1) / kUnit;
     int64_t sum = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -93,20 +105,31 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
       if (i < (tid >> 6)) base += wave_total[i];
       before += wave_total[i];
     }
-    if (x < items) w.prefix[x] = base + sum - n;
+    if (x < items) w.items[x] = Item{base + sum - n, len, seq};
     __syncthreads();
   }
   const int64_t per = max((int64_t)kMinUnits, (before + kShares - 1) / kShares);
   if (tid == 0) {
-    w.prefix[items] = before;
+    w.items[items] = Item{before, 0, 0};
     w.head[0] = per;
     w.head[1] = before;
   }
   __syncthreads();
-  for (int x = tid; x < items; x += 256) {
-    const int64_t lo = w.prefix[x], hi = w.prefix[x + 1];
-    for (int64_t s = (lo + per - 1) / per; s * per < hi; s++) w.first[s] = x;
+  static_assert(kShares == 256, "a thread per share");
+  const int64_t from = tid * per, to = min(from + per, before);
+  if (from >= before) {
+    w.shares[tid].total = 0;
+    return;
   }
+  int lo = 0, hi = items;  // the last item that begins at or before the share's first unit: the one that holds it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (w.items[mid].begin <= from) lo = mid;
+    else hi = mid;
+  }
+  const Item it = w.items[lo];
+  w.shares[tid] = Share{to - from, lo, it.seq, it.len, (int32_t)(from - it.begin),
+                        (int32_t)(min(to, w.items[lo + 1].begin) - from), 0};
 }
 
 __global__ __launch_bounds__(256) void k_mla_plan(DecodeArgs d) { make_plan(d.a, d.w); }
@@ -114,11 +137,12 @@ __global__ __launch_bounds__(256) void k_mla_plan(DecodeArgs d) { make_plan(d.a,
 // ------------------------------------------------------------------------- ql = q_nope . W_uk
 
 constexpr int kAbsorbCols = 128;
+constexpr int kAbsorbRows = 64;
 
-// A workgroup takes 128 latent columns of one head: that part of W_uk goes to LDS once, and 16 rows at a
-// time are multiplied by it as (W_uk^T) . (q^T), each wave 32 columns. W_uk lies with the latent columns contiguous, so
-// its operand is read transposed. LDS rows are 256 bytes; 16-byte chunk c of row n lies at c ^ swizzle(n), which
-// spreads a transposing read over the banks.
+// A workgroup takes 128 latent columns of one head for 64 rows, 16 rows a wave: that part of W_uk goes to LDS while each wave loads
+// its queries, and is multiplied as (W_uk^T) . (q^T). W_uk lies with the latent columns contiguous, so its operand is read
+// transposed. LDS rows are 256 bytes; 16-byte chunk c of row n lies at c ^ swizzle(n), which spreads a transposing read over the
+// banks. Bound by the read of W_uk (8.4 MB for 64 heads of 128 x 512), and below some 16 rows by its latency.
 __device__ __forceinline__ int absorb_swizzle(int n) { return ((n & 3) << 2) ^ (((n >> 3) & 1) << 1); }
 
 template <int DT>
@@ -130,7 +154,7 @@ __global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks
     return;
   }
   const int h = (int)blockIdx.x / col_blocks, c0 = ((int)blockIdx.x % col_blocks) * kAbsorbCols;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = a.cache.rank;
   const uint16_t* w = (const uint16_t*)a.kv_b + (size_t)h * (a.nope + a.v_dim) * rank + c0;
   for (int i = wave; i < a.nope / 4; i += 4) {  // four rows of W_uk at a time
@@ -138,33 +162,34 @@ __global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks
     load_to_lds16(w + (size_t)n * rank + 8 * c, (lds_u8*)tile + i * 1024);
   }
   const int row = lane & 15, g = lane >> 4;
+  const int r = (int)blockIdx.y * kAbsorbRows + wave * 16 + row;
+  const uint16_t* q = (const uint16_t*)a.q_nope + (int64_t)min(r, a.rows - 1) * a.q_nope_row_stride + (int64_t)h * a.q_nope_head_stride + 8 * g;
+  s16x8 b[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) b[k] = k * 32 < a.nope ? *(const s16x8*)(q + k * 32) : s16x8{};
   // this lane's element of a transposing read: row 8 g + row / 4 (+ 4), columns 16 blk + 4 (row % 4)
   const int n0 = 8 * g + (row >> 2);
-  const int part = 8 * (row & 1);
-  const int r_end = min(a.rows, ((int)blockIdx.y + 1) * 64);
   wait_lds_loads();
   __syncthreads();
-  for (int r0 = (int)blockIdx.y * 64; r0 < r_end; r0 += 16) {
-    const int r = min(r0 + row, a.rows - 1);
-    const uint16_t* q = (const uint16_t*)a.q_nope + (int64_t)r * a.q_nope_row_stride + (int64_t)h * a.q_nope_head_stride;
-    f32x4 acc[2] = {};
-    for (int k = 0; k < a.nope; k += 32) {
-      const s16x8 b = *(const s16x8*)(q + k + 8 * g);
+  if ((int)blockIdx.y * kAbsorbRows + wave * 16 >= a.rows) return;
+  f32x4 acc[8] = {};
 #pragma unroll
-      for (int blk = 0; blk < 2; blk++) {
-        const int c = (wave * 2 + blk) * 2 + ((row & 3) >> 1);
-        const int na = k + n0, nb = na + 4;
-        const s16x4 lo = lds_read_tr((lds_u8*)tile + na * 256 + (c ^ absorb_swizzle(na)) * 16 + part);
-        const s16x4 hi = lds_read_tr((lds_u8*)tile + nb * 256 + (c ^ absorb_swizzle(nb)) * 16 + part);
-        acc[blk] = mma32<DT>(join(lo, hi), b, acc[blk]);
-      }
-    }
-    if (r0 + row < a.rows) {
-      uint16_t* o = d.w.ql + ((size_t)(r0 + row) * a.heads + h) * rank + c0 + wave * 32 + 4 * g;
+  for (int k = 0; k < 8; k++) {
+    if (k * 32 >= a.nope) break;
+    const int na = k * 32 + n0, nb = na + 4;
+    lds_u8* t = (lds_u8*)tile + na * 256 + 8 * (row & 1);
 #pragma unroll
-      for (int blk = 0; blk < 2; blk++)  // rounded for the matrix cores: relative error half a step
-        *(uint2*)(o + 16 * blk) = make_uint2(pack2<DT>(acc[blk][0], acc[blk][1]), pack2<DT>(acc[blk][2], acc[blk][3]));
+    for (int blk = 0; blk < 8; blk++) {
+      const int c = blk * 2 + ((row & 3) >> 1);
+      acc[blk] = mma32<DT>(join(lds_read_tr(t + (c ^ absorb_swizzle(na)) * 16), lds_read_tr(t + 1024 + (c ^ absorb_swizzle(nb)) * 16)),
+                           b[k], acc[blk]);
     }
+  }
+  if (r < a.rows) {
+    uint16_t* o = d.w.ql + ((size_t)r * a.heads + h) * rank + c0 + 4 * g;
+#pragma unroll
+    for (int blk = 0; blk < 8; blk++)  // rounded for the matrix cores: relative error half a step
+      *(uint2*)(o + 16 * blk) = make_uint2(pack2<DT>(acc[blk][0], acc[blk][1]), pack2<DT>(acc[blk][2], acc[blk][3]));
   }
 }
 
@@ -181,30 +206,57 @@ __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 // wave's sums at 64 registers (heads x 64 columns), so that next to the 72 of its queries enough remain for LDS reads in
 // flight, and every cached row is read from LDS once for all heads' sums.
 //
-// A unit's rows go from the pages straight to LDS (16 bytes a lane), double-buffered: while one unit is
-// worked on, the next is in flight (74 KB a CU, 19 MB over the chip). A row's 16-byte chunk c lies at c ^ f(row)
-// (f = (row / 2) % 8, rows 32 banks apart; for widths of 4 chunks modulo 8 (row / 4) % 4, rows 16 banks apart), which
-// spreads the row-wise and the transposing reads over all 64 banks.
+// Rows go from the pages straight to LDS (16 bytes a lane), double-buffered: while a unit is worked on, the next, of
+// this item or the share's next one, is in flight (74 KB a CU, 19 MB over the chip). The latent parts of the rows and the rotary parts lie apart, so
+// that one load instruction covers whole rows. Chunk c (16 bytes) of a latent part lies at c ^ row_swizzle(row): the
+// rows' stride is a multiple of all 64 banks, and so the 16 rows of a score operand, and the 8 rows of half a transposing
+// read, fall into different banks; a rotary part has 128 bytes whatever its width, chunk c at c ^ (row / 2) % 8.
+__device__ __forceinline__ int row_swizzle(int row) { return ((row & 3) << 1) | (((row >> 3) & 1) << 3) | ((row >> 2) & 1); }
+
+// v as a value that the compiler does not know to be the same each time: what is formed from it is formed where it is used,
+// not held in registers over the loop.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T ld_const(const T* p) {  // wave-uniform address: a scalar load
+  return *(const __attribute__((address_space(4))) T*)p;
+}
+
+__device__ __forceinline__ const uint8_t* lane_ptr(uint64_t p, int lane) {  // a lane's pointer, wave-uniform
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)p, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(p >> 32), lane);
+  return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Maximum over the four lanes that share lane % 16.
+__device__ __forceinline__ float max_over_rows(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <int DT, int R, int P, int HB>
 __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
   constexpr int kWaves = 8;
-  constexpr int W = R + P, CH = W / 8, kRowBytes = W * 2;
-  constexpr int kMask = CH % 8 == 0 ? 7 : 3, kShift = CH % 8 == 0 ? 1 : 2;
-  constexpr int kTpw = kUnit / kWaves;                 // rows a wave loads
-  constexpr int kLoads = (kTpw * CH + 63) / 64;
-  constexpr int kTile = kUnit * kRowBytes;
+  constexpr int kTpw = kUnit / kWaves;                 // rows a wave loads: 8, eight lanes for each
+  constexpr int RC = R / 8, PC = P / 8;                // 16-byte chunks of the two parts of a row
+  constexpr int kPer = 64 / RC;                        // latent parts of one load instruction: 1 or 2
   constexpr int NB = HB == 4 ? 2 : 1;                  // 16-token blocks of a wave's scores (HB = 1: four waves have none)
   constexpr int CB = R / 16 / kWaves;                  // 16-column blocks of a wave's sums
-  __shared__ __align__(1024) uint8_t tile[2 * kTile];
+  __shared__ __align__(1024) uint8_t lat[2][kUnit * R * 2];
+  __shared__ __align__(1024) uint8_t rot[2][kUnit * 128];
   __shared__ __align__(16) uint8_t prob[HB * 16 * kUnit * 2];  // [head][token], chunk c of a row at c ^ (head / 2) % 8
   __shared__ float tops[4][HB * 16];                   // maximum of 16 tokens' scores per head; at the end their sums
   __shared__ float fade[HB * 16];                      // factor of a head's earlier sums
-  __shared__ float2 stats[HB * 16];                    // at the end: maximum and sum
+  __shared__ float last_top[HB * 16];                  // at the end: the heads' maxima
   __shared__ __align__(16) float seen[2][kUnit];       // 1: the token is seen
-  __shared__ uint64_t row_at[kUnit];                   // addresses of the next unit's rows, each wave its own
 
   const vib3_mla_decode& a = d.a;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
   // this wave's scores: head block hb, token blocks tb .. tb + NB - 1
   const int hb = HB == 4 ? wave >> 1 : HB == 2 ? wave >> 2 : 0;
@@ -213,101 +265,133 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
   const int groups = head_groups(a.heads);
   const float to_log2 = a.scale * 1.44269504088896341f;
 
-  const int64_t per = d.w.head[0], all = d.w.head[1];
-  const int64_t begin = (int64_t)blockIdx.x * per, end = min(begin + per, all);
-  if (begin >= end) return;
-  int x = d.w.first[blockIdx.x];
+  const Share* sh = d.w.shares + blockIdx.x;
+  int64_t to_load = ld_const(&sh->total);  // units of the share not yet on their way to LDS
+  if (to_load == 0) return;
 
-  // this lane's places within a tile: row tb * 16 + col for the scores, row 8 g + col / 4 (and 4 further) for the transposing
-  // reads, at 16 * wave * CB columns; 16 rows further the swizzle is the same
-  const int krow = tb * 16 + col, kf = (krow >> kShift) & kMask;
-  const int vrow = 8 * g + (col >> 2), vf0 = (vrow >> kShift) & kMask, vf1 = ((vrow + 4) >> kShift) & kMask;
-  lds_u8* const pw = (lds_u8*)prob + (hb * 16 + col) * (kUnit * 2);  // where this lane's probabilities go
+  // The stream of units into LDS. Lane holds the token, page and place in the page of row wave * 8 + lane / 8 of the next unit to
+  // look up, and the page's number and place of the next unit to load (-1: not seen).
+  const int page_size = a.cache.page_size, page_step = kUnit / page_size, off_step = kUnit % page_size;
+  int s_item = ld_const(&sh->item), s_left = ld_const(&sh->left), s_len = ld_const(&sh->len);  // of the unit to look up
+  int64_t s_ahead = to_load;                                                                   // units not yet looked up
+  const int32_t* s_table = a.cache.block_table + (size_t)ld_const(&sh->seq) * a.cache.max_pages;
+  int s_token = ld_const(&sh->unit) * kUnit + wave * kTpw + (lane >> 3);
+  int s_page = s_token / page_size, s_off = s_token - s_page * page_size;
+  int id = -1, id_off = 0;
+  auto look_up = [&] {
+    if (s_left == 0 && s_ahead > 0) {
+      int units;
+      do {
+        s_item++;
+        s_len = ld_const(&d.w.items[s_item].len);
+        units = (s_len + kUnit - 1) / kUnit;
+      } while (units == 0);
+      s_left = (int)min((int64_t)units, s_ahead);
+      s_table = a.cache.block_table + (size_t)ld_const(&d.w.items[s_item].seq) * a.cache.max_pages;
+      s_token = wave * kTpw + (lane >> 3);
+      s_page = s_token / page_size;
+      s_off = s_token - s_page * page_size;
+    }
+    id = -1;
+    if (s_left > 0 && s_token < s_len) id = s_table[s_page];
+    id_off = s_off;
+    s_left--;
+    s_ahead--;
+    s_token += kUnit;
+    s_off += off_step;
+    s_page += page_step;
+    if (s_off >= page_size) {
+      s_off -= page_size;
+      s_page++;
+    }
+  };
+  auto issue = [&](int slot) {
+    const bool ok = (unsigned)id < (unsigned)a.cache.num_pages;
+    const uint64_t row = ok ? (uint64_t)(uintptr_t)((const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
+                                                    (int64_t)id_off * a.cache.row_stride)
+                            : (uint64_t)(uintptr_t)zero_row;
+    const int ln = fresh(lane);
+    if ((ln & 7) == 0) seen[slot][wave * kTpw + (ln >> 3)] = ok ? 1.0f : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTpw / kPer; i++) {
+      const int t = i * kPer + (kPer == 2 ? ln >> 5 : 0);
+      const uint8_t* p = lane_ptr(row, 8 * i * kPer);
+      if (kPer == 2) {
+        const uint8_t* p1 = lane_ptr(row, 8 * i * kPer + 8);
+        p = ln >= 32 ? p1 : p;
+      }
+      load_to_lds16(p + ((ln & (RC - 1)) ^ row_swizzle(wave * kTpw + t)) * 16, (lds_u8*)lat[slot] + (wave * kTpw + i * kPer) * R * 2);
+    }
+    const int c = (ln & 7) ^ ((ln >> 4) & 3) ^ (wave & 1) * 4;  // (row / 2) % 8 of row wave * 8 + lane / 8
+    if (PC == 8 || c < PC) load_to_lds16((const uint8_t*)(uintptr_t)row + R * 2 + c * 16, (lds_u8*)rot[slot] + wave * kTpw * 128);
+  };
+
+  // queries: the B operand, this lane's head at k = 32 s + 8 g
+  s16x8 q[(R + P) / 32];
+  auto load_q = [&](int x) {
+    const int r = x / groups, h0 = (x - r * groups) * 64;
+    const int64_t hh = min(h0 + hb * 16 + col, a.heads - 1);
+    const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + hh) * R
+                                : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + hh * a.q_nope_head_stride;
+    const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + hh * a.q_rope_head_stride;
+#pragma unroll
+    for (int s = 0; s < (R + P) / 32; s++)
+      q[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
+  };
+
+  // this lane's places within a unit: row tb * 16 + col for the scores, rows 8 g + col / 4 (and 4 further) for the
+  // transposing reads; 16 rows further the swizzles are the same
+  const int krow = tb * 16 + col, kf = row_swizzle(krow), rf = (col >> 1) & 7;
+  const int vrow = 8 * g + (col >> 2), vf = row_swizzle(vrow);  // row_swizzle(vrow + 4) = vf | 1
   const int pf = (col >> 1) & 7;
 
-  for (int64_t u0 = begin; u0 < end; x++) {
-    const int64_t row_begin = d.w.prefix[x], row_end = d.w.prefix[x + 1];
-    const int64_t u1 = min(end, row_end);
-    if (u1 <= u0) continue;
-    const int r = x / groups, h0 = (x - r * groups) * 64;
-    int seq;
-    const int len = row_len(a, r, &seq);
-    const int32_t* table = a.cache.block_table + (size_t)seq * a.cache.max_pages;
-    const int first_unit = (int)(u0 - row_begin), units = (int)(u1 - u0);
-
-    // token of unit n whose row this lane finds the address of (lanes < kTpw), and its page's number
-    auto page_of = [&](int n) {
-      const int j = (first_unit + n) * kUnit + wave * kTpw + lane;
-      return lane < kTpw && n < units && j < len ? table[j / a.cache.page_size] : -1;
-    };
-    auto issue = [&](int n, int id) {
-      const int j = (first_unit + n) * kUnit + wave * kTpw + lane;
-      const bool ok = (unsigned)id < (unsigned)a.cache.num_pages;
-      const uint16_t* p = (const uint16_t*)zero_row;
-      if (ok)
-        p = (const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
-            (int64_t)(j % a.cache.page_size) * a.cache.row_stride;
-      if (lane < kTpw) {
-        seen[n & 1][wave * kTpw + lane] = ok ? 1.0f : 0.0f;
-        row_at[wave * kTpw + lane] = (uint64_t)(uintptr_t)p;
-      }
-      lds_u8* base = (lds_u8*)tile + (n & 1) * kTile + wave * kTpw * kRowBytes;
-      int ln = lane;
-      asm volatile("" : "+v"(ln));  // the loads' places are formed anew for each unit, not held in registers
-#pragma unroll
-      for (int i = 0; i < kLoads; i++) {
-        const int slot = i * 64 + ln, t = slot / CH;
-        const int c = (slot - t * CH) ^ (((wave * kTpw + t) >> kShift) & kMask);
-        if (kTpw * CH % 64 == 0 || slot < kTpw * CH)
-          load_to_lds16((const uint8_t*)(uintptr_t)row_at[wave * kTpw + t] + c * 16, base + i * 1024);
-      }
-    };
-
-    // queries: the B operand, this lane's head at k = 32 s + 8 g
-    s16x8 q[W / 32];
-    {
-      const int64_t hh = min(h0 + hb * 16 + col, a.heads - 1);
-      const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + hh) * R
-                                  : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + hh * a.q_nope_head_stride;
-      const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + hh * a.q_rope_head_stride;
-#pragma unroll
-      for (int s = 0; s < W / 32; s++) q[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
-    }
+  look_up();
+  int x = ld_const(&sh->item), unit = ld_const(&sh->unit), units = ld_const(&sh->left), len = ld_const(&sh->len);
+  int64_t left = to_load;
+  issue(0);
+  look_up();
+  to_load--;
+  load_q(x);
+  VIB3_WAIT_VM(0);
+  int n = 0;  // unit of the share
+  for (;;) {
     f32x4 o[HB][CB] = {};
     float m = -__builtin_huge_valf(), l = 0.0f;  // of this lane's head; l over this lane's own tokens
-
-    int id = page_of(0);
-    __syncthreads();  // the last item's tiles and statistics are done with
-    issue(0, id);
-    id = page_of(1);
-    for (int n = 0; n < units; n++) {
+    const int first_of_share = n;
+    left -= units;
+    int next = x;
+    for (int i = 1;; i++, n++) {
       wait_lds_loads();
-      __syncthreads();  // unit n is in LDS; everyone is past unit n - 1
-      if (n + 1 < units) {
-        issue(n + 1, id);
-        id = page_of(n + 2);
+      __syncthreads();  // unit n is in LDS; everyone is done with unit n - 1
+      if (to_load > 0) {
+        issue((n + 1) & 1);
+        look_up();
+        to_load--;
       }
-      lds_u8* t = (lds_u8*)tile + (n & 1) * kTile;
-      f32x4 s[NB] = {};
+      f32x4 s[NB];
       if (scores) {
+        const lds_u8* t = (lds_u8*)lat[n & 1] + krow * R * 2;
+        const lds_u8* u = (lds_u8*)rot[n & 1] + krow * 128;
+        const int k0 = fresh((g ^ kf) * 16);
+        f32x4 s0[NB] = {}, s1[NB] = {};
 #pragma unroll
-        for (int k = 0; k < W / 32; k++) {
-          const int c = ((4 * k + g) & ~kMask) | (((4 * k + g) & kMask) ^ kf);
+        for (int k = 0; k < R / 32; k += 2)  // chunk (4 k + g) ^ kf, a constant and two bits away from g ^ kf
 #pragma unroll
-          for (int b = 0; b < NB; b++) s[b] = mma32<DT>(lds_read16(t + (krow + 16 * b) * kRowBytes + c * 16), q[k], s[b]);
-        }
+          for (int b = 0; b < NB; b++) {
+            s0[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ k % 4 * 64) + k / 4 * 256), q[k], s0[b]);
+            s1[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ (k + 1) % 4 * 64) + k / 4 * 256), q[k + 1], s1[b]);
+          }
+#pragma unroll
+        for (int k = 0; k < P / 32; k++)
+#pragma unroll
+          for (int b = 0; b < NB; b++) s0[b] = mma32<DT>(lds_read16(u + b * 16 * 128 + ((4 * k + g) ^ rf) * 16), q[R / 32 + k], s0[b]);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           const float4 v = *(const float4*)&seen[n & 1][(tb + b) * 16 + 4 * g];
           const float vv[4] = {v.x, v.y, v.z, v.w};
-          float top = -__builtin_huge_valf();
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            s[b][i] = vv[i] != 0.0f ? s[b][i] * to_log2 : -__builtin_huge_valf();
-            top = fmaxf(top, s[b][i]);
-          }
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
+          for (int i = 0; i < 4; i++) s[b][i] = vv[i] != 0.0f ? (s0[b][i] + s1[b][i]) * to_log2 : -__builtin_huge_valf();
+          const float top = max_over_rows(fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
           if (g == 0) tops[tb + b][hb * 16 + col] = top;
         }
       }
@@ -320,60 +404,75 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
         m = mn;
         l *= f;
         if (g == 0 && tb == 0) fade[at] = f;
+        lds_u8* const pw = (lds_u8*)prob + at * (kUnit * 2) + 8 * (g & 1);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           float e[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            e[i] = __builtin_amdgcn_exp2f(s[b][i] - base);
-            l += e[i];
-          }
+          for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(s[b][i] - base);
+          l += (e[0] + e[1]) + (e[2] + e[3]);
           // rounded for the matrix cores; the sum l takes them unrounded
-          lds_write8(pw + ((2 * (tb + b) + (g >> 1)) ^ pf) * 16 + 8 * (g & 1), pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
+          lds_write8(pw + ((2 * (tb + b) + (g >> 1)) ^ pf) * 16, pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
         }
       }
       __syncthreads();
+      {
+        // chunk ch ^ vf of column block c, ch = 2 (wave CB + c) + (col % 4) / 2
+        lds_u8* t = (lds_u8*)lat[n & 1] + vrow * R * 2 + 8 * (col & 1) + wave * 2 * CB / 16 * 256;
+        const int v0 = fresh(((wave * 2 * CB % 16 + ((col & 3) >> 1)) ^ vf) * 16);
+        float f[HB];
+        bool changed = false;
 #pragma unroll
-      for (int h = 0; h < HB; h++) {
-        const float f = fade[h * 16 + col];
-        if (__any(f != 1.0f)) {
+        for (int h = 0; h < HB; h++) {
+          f[h] = fade[h * 16 + col];
+          changed |= f[h] != 1.0f;
+        }
+        if (__any(changed)) {
 #pragma unroll
-          for (int c = 0; c < CB; c++) o[h][c] *= f;
+          for (int h = 0; h < HB; h++)
+#pragma unroll
+            for (int c = 0; c < CB; c++) o[h][c] *= f[h];
+        }
+#pragma unroll
+        for (int k = 0; k < kUnit / 32; k++) {
+          s16x8 pb[HB];
+#pragma unroll
+          for (int h = 0; h < HB; h++) pb[h] = lds_read16((lds_u8*)prob + (h * 16 + col) * (kUnit * 2) + ((4 * k + g) ^ pf) * 16);
+#pragma unroll
+          for (int c = 0; c < CB; c++) {
+            const s16x8 av = join(lds_read_tr(t + k * 64 * R + (v0 ^ 32 * c)), lds_read_tr(t + k * 64 * R + 8 * R + (v0 ^ 32 * c ^ 16)));
+#pragma unroll
+            for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av, pb[h], o[h][c]);
+          }
         }
       }
-#pragma unroll
-      for (int k = 0; k < kUnit / 32; k++) {
-        s16x8 pb[HB];
-#pragma unroll
-        for (int h = 0; h < HB; h++)
-          pb[h] = lds_read16((lds_u8*)prob + (h * 16 + col) * (kUnit * 2) + ((4 * k + g) ^ pf) * 16);
-#pragma unroll
-        for (int c = 0; c < CB; c++) {
-          const int ch = 2 * (wave * CB + c) + ((col & 3) >> 1);
-          lds_u8* v = t + (32 * k + vrow) * kRowBytes + 8 * (col & 1);
-          const s16x8 av = join(lds_read_tr(v + ((ch & ~kMask) | ((ch & kMask) ^ vf0)) * 16),
-                                lds_read_tr(v + 4 * kRowBytes + ((ch & ~kMask) | ((ch & kMask) ^ vf1)) * 16));
-#pragma unroll
-          for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av, pb[h], o[h][c]);
-        }
-      }
+      if (i == units) break;
     }
+    n++;
+    if (left > 0) {
+      do next++;
+      while (ld_const(&d.w.items[next].len) == 0);
+      load_q(next);
+    }
+
     // the heads' sums of probabilities, over a wave's lanes and the waves of a head block
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    __syncthreads();
     if (scores && g == 0) {
       tops[HB == 4 ? tb >> 1 : tb][hb * 16 + col] = l;
-      if (tb == 0) stats[hb * 16 + col].x = m;
+      if (tb == 0) last_top[hb * 16 + col] = m;
     }
+    VIB3_WAIT_VM(0);  // the next queries, before the stores below: those are not waited for
     __syncthreads();
-    const bool whole = u0 == row_begin && u1 == row_end;
+    const bool whole = unit == 0 && units == (len + kUnit - 1) / kUnit;
+    const int r = x / groups, h0 = (x - r * groups) * 64;
+    const int fcol = fresh(col), fg = fresh(g);
 #pragma unroll
     for (int h = 0; h < HB; h++) {
-      const int at = h * 16 + col, head = h0 + at;
+      const int at = h * 16 + fcol, head = h0 + at;
       const float sum = HB == 4 ? tops[0][at] + tops[1][at] : (tops[0][at] + tops[1][at]) + (tops[2][at] + tops[3][at]);
       if (head >= a.heads) continue;
-      const int c0 = wave * CB * 16 + 4 * g;
+      const int c0 = wave * CB * 16 + 4 * fg;
       if (whole) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         uint16_t* out = d.w.ol + ((size_t)r * a.heads + head) * R + c0;
@@ -382,84 +481,122 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
           *(uint2*)(out + 16 * c) =
               make_uint2(pack2<DT>(o[h][c][0] * inv, o[h][c][1] * inv), pack2<DT>(o[h][c][2] * inv, o[h][c][3] * inv));
       } else {
-        const size_t slot = (2 * (size_t)blockIdx.x + (u0 == begin ? 0 : 1)) * group_heads(a.heads) + at;
+        const size_t slot = (2 * (size_t)blockIdx.x + (first_of_share == 0 ? 0 : 1)) * group_heads(a.heads) + at;
         float* out = d.w.part + slot * R + c0;
 #pragma unroll
         for (int c = 0; c < CB; c++) *(float4*)(out + 16 * c) = make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
-        if (g == 0 && wave == 0) d.w.stat[slot] = make_float2(stats[at].x, sum);
+        if (fg == 0 && wave == 0) d.w.stat[slot] = make_float2(last_top[at], sum);
       }
     }
-    u0 = u1;
+    if (left == 0) break;
+    x = next;
+    unit = 0;
+    len = ld_const(&d.w.items[x].len);
+    units = (int)min((int64_t)((len + kUnit - 1) / kUnit), left);
   }
 }
 
 // ------------------------------------------------------------------------- joined rows and W_uv
 
-// A workgroup takes 16 rows of one head: their weighted latents (joined from the shares' parts where a row
-// has several) go to LDS in 16 bits, and each wave multiplies them by 16 rows of W_uv at a time. Without W_uv
-// the weighted latents are the result.
+// A workgroup takes up to 16 rows of one head. Its 16 waves are dealt over the rows: a wave, or where there are fewer rows
+// several, joins a row's parts (the weights of all parts first, then the parts' sums, several loads in flight). The rows' weighted latents
+// go to LDS in 16 bits, and v_dim / 16 waves multiply them by 16 rows of W_uv each, which they have loaded before the join. Without W_uv the weighted latents are the result.
 template <int DT, int R>
-__global__ __launch_bounds__(256) void k_mla_finish(DecodeArgs d) {
+__global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
   const vib3_mla_decode& a = d.a;
   constexpr int kStride = R + 8;  // 16 bytes more: rows start in different banks
+  constexpr int kCols = R / 64;   // columns of a lane
   __shared__ __align__(16) uint16_t lat[16 * kStride];
+  __shared__ __align__(16) float sums[16][R];
   const int h = (int)blockIdx.x, r0 = (int)blockIdx.y * 16;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t per = d.w.head[0];
-  constexpr int kCols = R / 64;  // columns of a lane: one wave joins a row
-  for (int i = wave; i < 16; i += 4) {
-    const int r = r0 + i;
-    uint16_t* dst = lat + i * kStride + lane * kCols;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  const int rows = min(16, a.rows - r0);
+  const uint16_t* wv = (const uint16_t*)a.kv_b + ((size_t)h * (a.nope + a.v_dim) + a.nope + col) * R + 8 * g;
+  s16x8 first[R / 32];
+  const bool product = a.kv_b && wave * 16 < a.v_dim;
+  if (product) {
+#pragma unroll
+    for (int k = 0; k < R / 32; k++) first[k] = *(const s16x8*)(wv + (size_t)wave * 16 * R + k * 32);
+  }
+  const int teams = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;  // rows joined at a time
+  const int per_row = 16 / teams, i = wave / per_row, mate = wave % per_row;
+  {
+    const int r = r0 + i, x = r * head_groups(a.heads) + h / 64;
     float o[kCols] = {};
-    const int x = r * head_groups(a.heads) + h / 64;
-    const int64_t lo = r < a.rows ? d.w.prefix[x] : 0, hi = r < a.rows ? d.w.prefix[x + 1] : 0;
+    const int64_t per = d.w.head[0];
+    const int64_t lo = i < rows ? d.w.items[x].begin : 0, hi = i < rows ? d.w.items[x + 1].begin : 0;
     if (hi > lo) {
-      const int64_t w0 = lo / per, w1 = (hi - 1) / per;
-      if (w0 == w1) {
-        const uint16_t* p = d.w.ol + ((size_t)r * a.heads + h) * R + lane * kCols;
+      const int w0 = (int)(lo / per), parts = (int)((hi - 1) / per) - w0 + 1;
+      if (parts == 1) {
+        if (mate == 0) {
+          const uint16_t* p = d.w.ol + ((size_t)r * a.heads + h) * R + lane * kCols;
 #pragma unroll
-        for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
-      } else {
-        float m = -__builtin_huge_valf(), l = 0.0f;
-        for (int64_t w = w0; w <= w1; w++) {
-          const size_t at = (2 * (size_t)w + (w == w0 && lo != w * per ? 1 : 0)) * group_heads(a.heads) + h % 64;
-          const float2 s = d.w.stat[at];
-          const float* p = d.w.part + at * R + lane * kCols;
-          const float mn = fmaxf(m, s.x), base = mn == -__builtin_huge_valf() ? 0.0f : mn;
-          const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(s.x - base);
-          l = l * f0 + s.y * f1;
-#pragma unroll
-          for (int c = 0; c < kCols; c++) o[c] = o[c] * f0 + p[c] * f1;
-          m = mn;
+          for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
         }
+      } else {
+        // part j: slot 2 (w0 + j), but the first one 2 w0 + 1 where its share began with another item
+        const bool late = lo != w0 * per;
+        const int hg = group_heads(a.heads), hh = h % 64;
+        auto place = [&](int j) { return ((size_t)2 * (w0 + j) + (j == 0 && late ? 1 : 0)) * hg + hh; };
+        float2 st[kShares / 64];  // lane l: parts l, l + 64, ...
+        float m = -__builtin_huge_valf();
+#pragma unroll
+        for (int k = 0; k < kShares / 64; k++) {
+          st[k] = lane + 64 * k < parts ? d.w.stat[place(lane + 64 * k)] : make_float2(-__builtin_huge_valf(), 0.0f);
+          m = fmaxf(m, st[k].x);
+        }
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
+        const float base = m == -__builtin_huge_valf() ? 0.0f : m;
+        float l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kShares / 64; k++) {
+          st[k].x = __builtin_amdgcn_exp2f(st[k].x - base);
+          l += st[k].x * st[k].y;
+        }
+        l = wave_sum(l);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int c = 0; c < kCols; c++) o[c] *= inv;
+        for (int k = 0; k < kShares / 64; k++) {
+#pragma unroll 4
+          for (int j = 64 * k + mate; j < min(parts, 64 * k + 64); j += per_row) {
+            const float f = __shfl(st[k].x, j - 64 * k) * inv;
+            const float* p = d.w.part + place(j) * R + lane * kCols;
+#pragma unroll
+            for (int c = 0; c < kCols; c += 4) {
+              const float4 v = *(const float4*)(p + c);
+              o[c] += f * v.x;
+              o[c + 1] += f * v.y;
+              o[c + 2] += f * v.z;
+              o[c + 3] += f * v.w;
+            }
+          }
+        }
       }
     }
-    if (a.kv_b) {
 #pragma unroll
-      for (int c = 0; c < kCols; c++) dst[c] = from_f32<DT>(o[c]);
-    } else if (r < a.rows) {
-      uint16_t* out = (uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + lane * kCols;
-#pragma unroll
-      for (int c = 0; c < kCols; c++) out[c] = from_f32<DT>(o[c]);
-    }
+    for (int c = 0; c < kCols; c += 4) *(float4*)&sums[wave][lane * kCols + c] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+  }
+  __syncthreads();
+  for (int at = tid; at < rows * R; at += 1024) {
+    const int k = at / R, c = at % R;
+    float v = 0.0f;
+    for (int s = 0; s < per_row; s++) v += sums[k * per_row + s][c];
+    if (a.kv_b) lat[k * kStride + c] = from_f32<DT>(v);
+    else ((uint16_t*)a.out)[(int64_t)(r0 + k) * a.out_row_stride + (int64_t)h * a.out_head_stride + c] = from_f32<DT>(v);
   }
   if (!a.kv_b) return;
   __syncthreads();
-  const int g = lane >> 4, n = lane & 15;
-  for (int v0 = wave * 16; v0 < a.v_dim; v0 += 64) {
-    const uint16_t* w = (const uint16_t*)a.kv_b + ((size_t)h * (a.nope + a.v_dim) + a.nope + v0 + n) * R;
-    f32x4 acc = {};
+  if (!product) return;
+  const int row = min(col, rows - 1);
+  f32x4 acc = {};
 #pragma unroll
-    for (int k = 0; k < R; k += 32)  // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
-      acc = mma32<DT>(*(const s16x8*)(w + k + 8 * g), *(const s16x8*)(lat + n * kStride + k + 8 * g), acc);
-    const int r = r0 + n;
-    if (r < a.rows)
-      *(uint2*)((uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + v0 + 4 * g) =
-          make_uint2(pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3]));
-  }
+  for (int k = 0; k < R / 32; k++)  // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
+    acc = mma32<DT>(first[k], *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
+  if (col < rows)
+    *(uint2*)((uint16_t*)a.out + (int64_t)(r0 + col) * a.out_row_stride + (int64_t)h * a.out_head_stride + wave * 16 + 4 * g) =
+        make_uint2(pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3]));
 }
 
 template <int DT, int R, int P>
@@ -467,7 +604,7 @@ int launch_decode(const DecodeArgs& d, hipStream_t st) {
   const vib3_mla_decode& a = d.a;
   if (a.kv_b) {
     const int col_blocks = R / kAbsorbCols;
-    hipLaunchKernelGGL(k_mla_absorb<DT>, dim3((unsigned)(a.heads * col_blocks + 1), (unsigned)((a.rows + 63) / 64)), dim3(256), 0, st,
+    hipLaunchKernelGGL(k_mla_absorb<DT>, dim3((unsigned)(a.heads * col_blocks + 1), (unsigned)((a.rows + kAbsorbRows - 1) / kAbsorbRows)), dim3(256), 0, st,
                        d, col_blocks);
   } else {
     hipLaunchKernelGGL(k_mla_plan, dim3(1), dim3(256), 0, st, d);
@@ -478,7 +615,7 @@ int launch_decode(const DecodeArgs& d, hipStream_t st) {
     hipLaunchKernelGGL((k_mla_attend<DT, R, P, 2>), dim3(kShares), dim3(512), 0, st, d);
   else
     hipLaunchKernelGGL((k_mla_attend<DT, R, P, 4>), dim3(kShares), dim3(512), 0, st, d);
-  hipLaunchKernelGGL((k_mla_finish<DT, R>), dim3((unsigned)a.heads, (unsigned)((a.rows + 15) / 16)), dim3(256), 0, st, d);
+  hipLaunchKernelGGL((k_mla_finish<DT, R>), dim3((unsigned)a.heads, (unsigned)((a.rows + 15) / 16)), dim3(1024), 0, st, d);
   VIB3_RETURN_LAUNCH();
 }
 
