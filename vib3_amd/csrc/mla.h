@@ -158,4 +158,11 @@ __device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// v as a value that the compiler does not know to be the same each time: what is formed from it is formed where it is used,
+// not held in registers over the loop.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 }  // namespace vib3

@@ -213,13 +213,6 @@ __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 // read, fall into different banks; a rotary part has 128 bytes whatever its width, chunk c at c ^ (row / 2) % 8.
 __device__ __forceinline__ int row_swizzle(int row) { return ((row & 3) << 1) | (((row >> 3) & 1) << 3) | ((row >> 2) & 1); }
 
-// v as a value that the compiler does not know to be the same each time: what is formed from it is formed where it is used,
-// not held in registers over the loop.
-__device__ __forceinline__ int fresh(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 template <typename T>
 __device__ __forceinline__ T ld_const(const T* p) {  // wave-uniform address: a scalar load
   return *(const __attribute__((address_space(4))) T*)p;
