@@ -135,6 +135,12 @@ __device__ __forceinline__ void load_to_lds16(const void* g, lds_u8* base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(g) : "memory", "m0");
 }
 
+// The same with 4 bytes a lane, at base + 4 * lane.
+__device__ __forceinline__ void load_to_lds4(const void* g, lds_u8* base) {
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(g) : "memory", "m0");
+}
+
 __device__ __forceinline__ void wait_lds_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }

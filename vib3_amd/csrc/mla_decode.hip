@@ -8,7 +8,7 @@
 //   k_mla_attend   the attention in the latent space, over equal shares of all rows' cached tokens
 //   k_mla_finish   rows that several workgroups shared are joined, and W_uv applied
 //
-// The plan: tokens are taken 64 at a time (a unit), heads in groups of up to 64. All units of all items
+// The plan: tokens are taken 32 at a time (a unit), heads in groups of up to 64. All units of all items
 // (row, head group) in order are cut into kShares equal runs, one workgroup each, whatever the rows' lengths: a long row is
 // shared by many workgroups, a run covers many short rows. Nothing on the host depends on the lengths, so a captured
 // launch follows them.
@@ -17,7 +17,7 @@
 namespace vib3 {
 
 constexpr int kMlaMaxRows = 65536;
-constexpr int kUnit = 64;      // cached tokens of one step
+constexpr int kUnit = 32;      // cached tokens of one step
 constexpr int kShares = 256;   // workgroups of the attention launch, one per CU (its LDS tiles fill one)
 constexpr int kMinUnits = 1;   // units of a share at least
 
@@ -39,13 +39,16 @@ struct DecodeWs {
   Item* items;        // [items + 1]
   Share* shares;      // [kShares]
   uint16_t* ql;       // [rows][heads][rank]
-  uint16_t* ol;       // [rows][heads][rank] weighted latent of items that one share covers
+  uint16_t* ol;       // [rows][padded heads][rank] weighted latent of items that one share covers
   float* part;        // [2 kShares][heads of a group][rank] unnormalised sums
   float2* stat;       // [2 kShares][heads of a group] running maximum (of scores in log2 units) and sum
 };
 
 __host__ __device__ inline int head_groups(int heads) { return (heads + 63) / 64; }
-__host__ __device__ inline int group_heads(int heads) { return heads < 64 ? heads : 64; }
+__host__ __device__ inline int head_blocks(int heads) { return heads <= 16 ? 1 : heads <= 32 ? 2 : 4; }  // of 16, a group's
+// Heads that a row of weighted latents and a slot of parts have room for: whole blocks, so that nothing is cut off in storing.
+__host__ __device__ inline int padded_heads(int heads) { return heads <= 64 ? head_blocks(heads) * 16 : 128; }
+__host__ __device__ inline int group_heads(int heads) { return head_blocks(heads) * 16; }
 
 inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   size_t at = 0;
@@ -60,7 +63,7 @@ inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   r.items = (Item*)take(sizeof(Item) * ((size_t)a.rows * head_groups(a.heads) + 1));
   r.shares = (Share*)take(sizeof(Share) * kShares);
   r.ql = (uint16_t*)take(a.kv_b ? 2 * row * a.rows : 0);
-  r.ol = (uint16_t*)take(2 * row * a.rows);
+  r.ol = (uint16_t*)take(2 * (size_t)padded_heads(a.heads) * a.cache.rank * a.rows);
   r.part = (float*)take(4 * (size_t)group_heads(a.heads) * a.cache.rank * 2 * kShares);
   r.stat = (float2*)take(8 * (size_t)group_heads(a.heads) * 2 * kShares);
   if (w) *w = r;
@@ -198,19 +201,23 @@ __global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks
 // What masked tokens read instead of the cache: their probability is 0, and 0 times whatever lies there must be 0.
 __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 
-// A workgroup is eight waves, two per SIMD, and takes HB blocks of 16 heads (1, 2 or 4; more than 64 heads are groups of 64,
-// planned like rows of their own). For a unit of 64 tokens it forms the scores S^T = K . Q^T, the waves dealt over
-// (head block, 16 tokens), so that a lane holds one head's scores of 4 tokens; the running maximum of a head over
-// the unit is joined through LDS; the probabilities go to LDS, and each wave adds to the sums O^T = C^T . P^T of all heads for an
-// eighth of the latent's columns, C^T by transposing reads of the same LDS rows. Splitting the columns keeps a
-// wave's sums at 64 registers (heads x 64 columns), so that next to the 72 of its queries enough remain for LDS reads in
-// flight, and every cached row is read from LDS once for all heads' sums.
+// A workgroup takes HB blocks of 16 heads (1, 2 or 4; more than 64 heads are groups of 64, planned like rows of their own)
+// with eight waves, one of either kind on each SIMD, that work on neighbouring units of 32 tokens between the same two barriers:
+//   waves 0-3  form the scores and probabilities of unit k, 16 heads each. S^T = K . Q^T: a lane holds one head's scores of 4
+//              tokens per 16, so that the running maximum and sum stay within the wave; the probabilities go to LDS.
+//   waves 4-7  add to the sums O^T = C^T . P^T of all heads for unit k - 1, a quarter of the latent's columns each (C^T by
+//              transposing reads), and load unit k + 2.
+// With one barrier a unit, and each SIMD with vector work of one wave next to products of the other, a unit takes some
+// 1600 cycles at 64 heads, less than half of what its rows (37 KB) take to arrive at 6 TB/s; all eight waves going through the same
+// phases, with three barriers, took 4600.
 //
-// Rows go from the pages straight to LDS (16 bytes a lane), double-buffered: while a unit is worked on, the next, of
-// this item or the share's next one, is in flight (74 KB a CU, 19 MB over the chip). The latent parts of the rows and the rotary parts lie apart, so
-// that one load instruction covers whole rows. Chunk c (16 bytes) of a latent part lies at c ^ row_swizzle(row): the
-// rows' stride is a multiple of all 64 banks, and so the 16 rows of a score operand, and the 8 rows of half a transposing
-// read, fall into different banks; a rotary part has 128 bytes whatever its width, chunk c at c ^ (row / 2) % 8.
+// Rows go from the pages straight to LDS (16 bytes a lane) into a ring of four units, two in use and two in flight (74 KB a CU,
+// 19 MB over the chip); the stream runs on from one item of the share to the next. The page numbers travel the same way, two
+// units ahead of the rows, so that no load is ever waited for but in the order of the ring (one count, kLoads a unit).
+// The latent parts of the rows and the rotary parts lie apart, so that one load instruction covers whole rows. Chunk c (16 bytes)
+// of a latent part lies at c ^ row_swizzle(row): the rows' stride is a multiple of all 64 banks, and so the 16 rows of a score
+// operand, and the 8 rows of half a transposing read, fall into different banks; a rotary part has 128 bytes whatever its
+// width, chunk c at c ^ (row / 2) % 8.
 __device__ __forceinline__ int row_swizzle(int row) { return ((row & 3) << 1) | (((row >> 3) & 1) << 3) | ((row >> 2) & 1); }
 
 template <typename T>
@@ -224,87 +231,198 @@ __device__ __forceinline__ const uint8_t* lane_ptr(uint64_t p, int lane) {  // a
   return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
-// Maximum over the four lanes that share lane % 16.
+// Maximum and sum over the four lanes that share lane % 16.
 __device__ __forceinline__ float max_over_rows(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+__device__ __forceinline__ float sum_over_rows(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The items of a share one after the other: units of the current one and the length of its row.
+struct Walk {
+  const Item* items;
+  int64_t left;   // units of the share after the current item
+  int item, unit, units, len;
+  __device__ __forceinline__ explicit Walk(const DecodeWs& w, const Share* s)
+      : items(w.items), left(ld_const(&s->total) - ld_const(&s->left)), item(ld_const(&s->item)), unit(ld_const(&s->unit)),
+        units(ld_const(&s->left)), len(ld_const(&s->len)) {}
+  __device__ __forceinline__ int next() const {  // (only where left > 0)
+    int x = item;
+    do x++;
+    while (ld_const(&items[x].len) == 0);
+    return x;
+  }
+  __device__ __forceinline__ bool step() {
+    if (left == 0) return false;
+    item = next();
+    len = ld_const(&items[item].len);
+    unit = 0;
+    units = (int)min((int64_t)((len + kUnit - 1) / kUnit), left);
+    left -= units;
+    return true;
+  }
+};
 
 template <int DT, int R, int P, int HB>
 __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
-  constexpr int kWaves = 8;
-  constexpr int kTpw = kUnit / kWaves;                 // rows a wave loads: 8, eight lanes for each
+  constexpr int kRing = 4;
+  constexpr int kTpw = kUnit / 4;                      // rows that one of the four loading waves loads: 8, eight lanes for each
   constexpr int RC = R / 8, PC = P / 8;                // 16-byte chunks of the two parts of a row
   constexpr int kPer = 64 / RC;                        // latent parts of one load instruction: 1 or 2
-  constexpr int NB = HB == 4 ? 2 : 1;                  // 16-token blocks of a wave's scores (HB = 1: four waves have none)
-  constexpr int CB = R / 16 / kWaves;                  // 16-column blocks of a wave's sums
-  __shared__ __align__(1024) uint8_t lat[2][kUnit * R * 2];
-  __shared__ __align__(1024) uint8_t rot[2][kUnit * 128];
-  __shared__ __align__(16) uint8_t prob[HB * 16 * kUnit * 2];  // [head][token], chunk c of a row at c ^ (head / 2) % 8
-  __shared__ float tops[4][HB * 16];                   // maximum of 16 tokens' scores per head; at the end their sums
-  __shared__ float fade[HB * 16];                      // factor of a head's earlier sums
-  __shared__ float last_top[HB * 16];                  // at the end: the heads' maxima
-  __shared__ __align__(16) float seen[2][kUnit];       // 1: the token is seen
+  constexpr int kLoads = kTpw / kPer + 2;              // a wave's load instructions per unit: latents, rotary parts, page numbers
+  constexpr int CB = R / 16 / 4;                       // 16-column blocks of a wave's sums
+  __shared__ __align__(1024) uint8_t lat[kRing][kUnit * R * 2];
+  __shared__ __align__(1024) uint8_t rot[kRing][kUnit * 128];
+  __shared__ __align__(16) uint8_t prob[2][HB * 16 * kUnit * 2];  // [head][token], chunk c of a row at c ^ (head / 4) % 4
+  __shared__ float fade[2][HB * 16];                   // factor of a head's earlier sums
+  __shared__ float2 stats[2][HB * 16];                 // at the end of an item: a head's maximum and sum
+  __shared__ __align__(16) float seen[kRing][kUnit];   // 1: the token is seen
+  __shared__ __align__(16) int32_t page_no[kRing][4][kTpw];  // of the rows a wave loads
+  __shared__ __align__(16) int32_t place[kRing][4][kTpw];    // their places in the pages, -1: not seen
 
   const vib3_mla_decode& a = d.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, col = lane & 15;
-  // this wave's scores: head block hb, token blocks tb .. tb + NB - 1
-  const int hb = HB == 4 ? wave >> 1 : HB == 2 ? wave >> 2 : 0;
-  const int tb = HB == 4 ? (wave & 1) * 2 : wave & 3;
-  const bool scores = HB > 1 || wave < 4;
   const int groups = head_groups(a.heads);
-  const float to_log2 = a.scale * 1.44269504088896341f;
-
   const Share* sh = d.w.shares + blockIdx.x;
-  int64_t to_load = ld_const(&sh->total);  // units of the share not yet on their way to LDS
-  if (to_load == 0) return;
+  if (ld_const(&sh->total) == 0) return;
+  Walk at(d.w, sh);
 
-  // The stream of units into LDS. Lane holds the token, page and place in the page of row wave * 8 + lane / 8 of the next unit to
-  // look up, and the page's number and place of the next unit to load (-1: not seen).
+  if (wave < 4) {
+    if (wave >= HB) {
+      for (int64_t k = ld_const(&sh->total); k >= 0; k--) __syncthreads();
+      return;
+    }
+    const int g = lane >> 4, col = lane & 15, head_in_group = wave * 16 + col;
+    const float scale = __builtin_fabsf(a.scale) * 1.44269504088896341f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale: the queries' signs instead
+    // queries: the B operand, this lane's head at k = 32 s + 8 g
+    constexpr int KS = (R + P) / 32;
+    s16x8 q[KS], q_next[KS];
+    auto load_q = [&](int x) {
+      const int r = x / groups;
+      const int64_t h = min((x - r * groups) * 64 + head_in_group, a.heads - 1);
+      const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + h) * R
+                                  : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + h * a.q_nope_head_stride;
+      const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + h * a.q_rope_head_stride;
+#pragma unroll
+      for (int s = 0; s < KS; s++) q_next[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
+    };
+    // this lane's row of a 16-token block; 16 rows further the swizzles are the same
+    const int k0 = (g ^ row_swizzle(col)) * 16, r0 = (g ^ ((col >> 1) & 7)) * 16;
+    load_q(at.item);
+    int k = 0;  // unit of the share
+    do {
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        uint4 v = __builtin_bit_cast(uint4, q_next[s]);
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        q[s] = __builtin_bit_cast(s16x8, v);
+      }
+      if (at.left > 0) load_q(at.next());  // on its way while this item is worked on
+      float m = -__builtin_huge_valf(), l = 0.0f;  // of this lane's head (unscaled scores); l over this lane's own tokens
+      for (int i = 0; i < at.units; i++, k++) {
+        __syncthreads();  // unit k is in LDS; the probabilities of unit k - 2 are done with
+        const lds_u8* t = (lds_u8*)lat[k % kRing] + col * R * 2;
+        const lds_u8* u = (lds_u8*)rot[k % kRing] + col * 128;
+        f32x4 s[2] = {};
+#pragma unroll
+        for (int c = 0; c < R / 32; c++)  // chunk (4 c + g) ^ row_swizzle(col), a constant and two bits away from that of c = 0
+#pragma unroll
+          for (int b = 0; b < 2; b++) s[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ c % 4 * 64) + c / 4 * 256), q[c], s[b]);
+#pragma unroll
+        for (int c = 0; c < P / 32; c++)
+#pragma unroll
+          for (int b = 0; b < 2; b++) s[b] = mma32<DT>(lds_read16(u + b * 16 * 128 + (r0 ^ 64 * c)), q[R / 32 + c], s[b]);
+        float top = -__builtin_huge_valf();
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const float4 v = *(const float4*)&seen[k % kRing][b * 16 + 4 * g];
+          const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            s[b][j] = vv[j] != 0.0f ? s[b][j] : -__builtin_huge_valf();
+            top = fmaxf(top, s[b][j]);
+          }
+        }
+        top = max_over_rows(top);
+        // The reference value of a head's exponentials follows its maximum only where that grew by more than 2^8 (in the
+        // result): probabilities up to 256 are as exact as ones up to 1, and the sums are seldom rescaled.
+        const bool grown = (top - m) * scale > 8.0f || (m == -__builtin_huge_valf() && top > m);
+        const float f = grown ? __builtin_amdgcn_exp2f((m - top) * scale) : 1.0f;
+        m = grown ? top : m;
+        l *= f;
+        const float base = m == -__builtin_huge_valf() ? 0.0f : m * scale;
+        if (g == 0) fade[k & 1][head_in_group] = f;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
+          l += (e[0] + e[1]) + (e[2] + e[3]);
+          // rounded for the matrix cores; the sum l takes them unrounded
+          lds_write8((lds_u8*)prob[k & 1] + head_in_group * (kUnit * 2) + ((2 * b + (g >> 1)) ^ (col >> 2)) * 16 + 8 * (g & 1),
+                     pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
+        }
+      }
+      const float sum = sum_over_rows(l);
+      if (g == 0) stats[(k - 1) & 1][head_in_group] = make_float2(m * scale, sum);
+    } while (at.step());
+    __syncthreads();
+    return;
+  }
+
+  const int pw = wave - 4;
+  // The stream of page numbers: a lane holds the token, page and place in the page of row lane % 8 of its wave's next rows.
   const int page_size = a.cache.page_size, page_step = kUnit / page_size, off_step = kUnit % page_size;
-  int s_item = ld_const(&sh->item), s_left = ld_const(&sh->left), s_len = ld_const(&sh->len);  // of the unit to look up
-  int64_t s_ahead = to_load;                                                                   // units not yet looked up
+  const int my_row = pw * kTpw + (lane & 7);
+  Walk ahead = at;
+  int s_left = at.units;
   const int32_t* s_table = a.cache.block_table + (size_t)ld_const(&sh->seq) * a.cache.max_pages;
-  int s_token = ld_const(&sh->unit) * kUnit + wave * kTpw + (lane >> 3);
+  int s_token = at.unit * kUnit + my_row;
   int s_page = s_token / page_size, s_off = s_token - s_page * page_size;
-  int id = -1, id_off = 0;
-  auto look_up = [&] {
-    if (s_left == 0 && s_ahead > 0) {
-      int units;
-      do {
-        s_item++;
-        s_len = ld_const(&d.w.items[s_item].len);
-        units = (s_len + kUnit - 1) / kUnit;
-      } while (units == 0);
-      s_left = (int)min((int64_t)units, s_ahead);
-      s_table = a.cache.block_table + (size_t)ld_const(&d.w.items[s_item].seq) * a.cache.max_pages;
-      s_token = wave * kTpw + (lane >> 3);
+  // The next unit's page numbers into ring place k % kRing.
+  auto look_up = [&](int k) {
+    if (s_left == 0 && ahead.step()) {
+      s_left = ahead.units;
+      s_table = a.cache.block_table + (size_t)ld_const(&ahead.items[ahead.item].seq) * a.cache.max_pages;
+      s_token = my_row;
       s_page = s_token / page_size;
       s_off = s_token - s_page * page_size;
     }
-    id = -1;
-    if (s_left > 0 && s_token < s_len) id = s_table[s_page];
-    id_off = s_off;
-    s_left--;
-    s_ahead--;
-    s_token += kUnit;
-    s_off += off_step;
-    s_page += page_step;
-    if (s_off >= page_size) {
-      s_off -= page_size;
-      s_page++;
+    const bool ok = s_left > 0 && s_token < ahead.len;
+    const int32_t* p = ok ? s_table + s_page : (const int32_t*)zero_row;
+    if (lane < kTpw) {
+      place[k % kRing][pw][lane] = ok ? s_off : -1;
+      load_to_lds4(p, (lds_u8*)page_no[k % kRing][pw]);
+    }
+    if (s_left > 0) {
+      s_left--;
+      s_token += kUnit;
+      s_off += off_step;
+      s_page += page_step;
+      if (s_off >= page_size) {
+        s_off -= page_size;
+        s_page++;
+      }
     }
   };
-  auto issue = [&](int slot) {
-    const bool ok = (unsigned)id < (unsigned)a.cache.num_pages;
-    const uint64_t row = ok ? (uint64_t)(uintptr_t)((const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
-                                                    (int64_t)id_off * a.cache.row_stride)
-                            : (uint64_t)(uintptr_t)zero_row;
+  // Unit k's rows into ring place k % kRing (rows of zeros once the stream is through), eight lanes finding the address of each.
+  auto issue = [&](int k) {
+    const int slot = k % kRing;
     const int ln = fresh(lane);
-    if ((ln & 7) == 0) seen[slot][wave * kTpw + (ln >> 3)] = ok ? 1.0f : 0.0f;
+    const int id = page_no[slot][pw][ln >> 3], off = place[slot][pw][ln >> 3];
+    const bool ok = off >= 0 && (unsigned)id < (unsigned)a.cache.num_pages;
+    const uint64_t row = ok ? (uint64_t)(uintptr_t)((const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
+                                                    (int64_t)off * a.cache.row_stride)
+                            : (uint64_t)(uintptr_t)zero_row;
+    if ((ln & 7) == 0) seen[slot][pw * kTpw + (ln >> 3)] = ok ? 1.0f : 0.0f;
 #pragma unroll
     for (int i = 0; i < kTpw / kPer; i++) {
       const int t = i * kPer + (kPer == 2 ? ln >> 5 : 0);
@@ -313,180 +431,86 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
         const uint8_t* p1 = lane_ptr(row, 8 * i * kPer + 8);
         p = ln >= 32 ? p1 : p;
       }
-      load_to_lds16(p + ((ln & (RC - 1)) ^ row_swizzle(wave * kTpw + t)) * 16, (lds_u8*)lat[slot] + (wave * kTpw + i * kPer) * R * 2);
+      load_to_lds16(p + ((ln & (RC - 1)) ^ row_swizzle(pw * kTpw + t)) * 16, (lds_u8*)lat[slot] + (pw * kTpw + i * kPer) * R * 2);
     }
-    const int c = (ln & 7) ^ ((ln >> 4) & 3) ^ (wave & 1) * 4;  // (row / 2) % 8 of row wave * 8 + lane / 8
-    if (PC == 8 || c < PC) load_to_lds16((const uint8_t*)(uintptr_t)row + R * 2 + c * 16, (lds_u8*)rot[slot] + wave * kTpw * 128);
+    const int c = (ln & 7) ^ ((ln >> 4) & 3) ^ (pw & 1) * 4;  // (row / 2) % 8 of row pw * 8 + lane / 8
+    if (PC == 8 || c < PC) load_to_lds16((const uint8_t*)(uintptr_t)row + R * 2 + c * 16, (lds_u8*)rot[slot] + pw * kTpw * 128);
   };
+  // Unit k's rows, and the page numbers of unit k + 2, have landed for this wave once no more than the next unit's loads are out.
+  auto landed = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory"); };
 
-  // queries: the B operand, this lane's head at k = 32 s + 8 g
-  s16x8 q[(R + P) / 32];
-  auto load_q = [&](int x) {
-    const int r = x / groups, h0 = (x - r * groups) * 64;
-    const int64_t hh = min(h0 + hb * 16 + col, a.heads - 1);
-    const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + hh) * R
-                                : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + hh * a.q_nope_head_stride;
-    const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + hh * a.q_rope_head_stride;
-#pragma unroll
-    for (int s = 0; s < (R + P) / 32; s++)
-      q[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
-  };
-
-  // this lane's places within a unit: row tb * 16 + col for the scores, rows 8 g + col / 4 (and 4 further) for the
-  // transposing reads; 16 rows further the swizzles are the same
-  const int krow = tb * 16 + col, kf = row_swizzle(krow), rf = (col >> 1) & 7;
-  const int vrow = 8 * g + (col >> 2), vf = row_swizzle(vrow);  // row_swizzle(vrow + 4) = vf | 1
-  const int pf = (col >> 1) & 7;
-
-  look_up();
-  int x = ld_const(&sh->item), unit = ld_const(&sh->unit), units = ld_const(&sh->left), len = ld_const(&sh->len);
-  int64_t left = to_load;
+  look_up(0);
+  look_up(1);
+  wait_lds_loads();
   issue(0);
-  look_up();
-  to_load--;
-  load_q(x);
-  VIB3_WAIT_VM(0);
-  int n = 0;  // unit of the share
-  for (;;) {
+  look_up(2);
+  issue(1);
+  look_up(3);
+  landed();
+  __syncthreads();
+  issue(2);
+  look_up(4);
+  int k = 1;
+  do {
     f32x4 o[HB][CB] = {};
-    float m = -__builtin_huge_valf(), l = 0.0f;  // of this lane's head; l over this lane's own tokens
-    const int first_of_share = n;
-    left -= units;
-    int next = x;
-    for (int i = 1;; i++, n++) {
-      wait_lds_loads();
-      __syncthreads();  // unit n is in LDS; everyone is done with unit n - 1
-      if (to_load > 0) {
-        issue((n + 1) & 1);
-        look_up();
-        to_load--;
+    const bool starts_share = k == 1;
+    for (int i = 0; i < at.units; i++, k++) {
+      landed();
+      __syncthreads();  // unit k and the probabilities of unit k - 1 are there; unit k - 2 is done with
+      issue(k + 2);
+      look_up(k + 4);
+      const int ln = fresh(lane), g = ln >> 4, col = ln & 15;
+      // rows vrow and vrow + 4, chunk ch ^ vf of column block c: ch = 2 (pw CB + c) + (col % 4) / 2, and vf ^ 1 in the second row
+      const int vrow = 8 * g + (col >> 2), vf = row_swizzle(vrow);
+      lds_u8* t = (lds_u8*)lat[(k - 1) % kRing] + vrow * R * 2 + 8 * (col & 1) + pw * 2 * CB / 16 * 256;
+      const int v0 = ((pw * 2 * CB % 16 + ((col & 3) >> 1)) ^ vf) * 16;
+      s16x8 pb[HB];
+      float f[HB];
+      bool changed = false;
+#pragma unroll
+      for (int h = 0; h < HB; h++) {
+        pb[h] = lds_read16((lds_u8*)prob[(k - 1) & 1] + (h * 16 + col) * (kUnit * 2) + (g ^ (col >> 2)) * 16);
+        f[h] = fade[(k - 1) & 1][h * 16 + col];
+        changed |= f[h] != 1.0f;
       }
-      f32x4 s[NB];
-      if (scores) {
-        const lds_u8* t = (lds_u8*)lat[n & 1] + krow * R * 2;
-        const lds_u8* u = (lds_u8*)rot[n & 1] + krow * 128;
-        const int k0 = fresh((g ^ kf) * 16);
-        f32x4 s0[NB] = {}, s1[NB] = {};
+      if (__any(changed)) {
 #pragma unroll
-        for (int k = 0; k < R / 32; k += 2)  // chunk (4 k + g) ^ kf, a constant and two bits away from g ^ kf
+        for (int h = 0; h < HB; h++)
 #pragma unroll
-          for (int b = 0; b < NB; b++) {
-            s0[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ k % 4 * 64) + k / 4 * 256), q[k], s0[b]);
-            s1[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ (k + 1) % 4 * 64) + k / 4 * 256), q[k + 1], s1[b]);
-          }
-#pragma unroll
-        for (int k = 0; k < P / 32; k++)
-#pragma unroll
-          for (int b = 0; b < NB; b++) s0[b] = mma32<DT>(lds_read16(u + b * 16 * 128 + ((4 * k + g) ^ rf) * 16), q[R / 32 + k], s0[b]);
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-          const float4 v = *(const float4*)&seen[n & 1][(tb + b) * 16 + 4 * g];
-          const float vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; i++) s[b][i] = vv[i] != 0.0f ? (s0[b][i] + s1[b][i]) * to_log2 : -__builtin_huge_valf();
-          const float top = max_over_rows(fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
-          if (g == 0) tops[tb + b][hb * 16 + col] = top;
-        }
+          for (int c = 0; c < CB; c++) o[h][c] *= f[h];
       }
-      __syncthreads();
-      if (scores) {
-        const int at = hb * 16 + col;
-        const float mn = fmaxf(m, fmaxf(fmaxf(tops[0][at], tops[1][at]), fmaxf(tops[2][at], tops[3][at])));
-        const float base = mn == -__builtin_huge_valf() ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        l *= f;
-        if (g == 0 && tb == 0) fade[at] = f;
-        lds_u8* const pw = (lds_u8*)prob + at * (kUnit * 2) + 8 * (g & 1);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          float e[4];
+      for (int c = 0; c < CB; c++) {
+        const s16x8 av = join(lds_read_tr(t + (v0 ^ 32 * c)), lds_read_tr(t + 8 * R + (v0 ^ 32 * c ^ 16)));
 #pragma unroll
-          for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(s[b][i] - base);
-          l += (e[0] + e[1]) + (e[2] + e[3]);
-          // rounded for the matrix cores; the sum l takes them unrounded
-          lds_write8(pw + ((2 * (tb + b) + (g >> 1)) ^ pf) * 16, pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
-        }
+        for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av, pb[h], o[h][c]);
       }
-      __syncthreads();
-      {
-        // chunk ch ^ vf of column block c, ch = 2 (wave CB + c) + (col % 4) / 2
-        lds_u8* t = (lds_u8*)lat[n & 1] + vrow * R * 2 + 8 * (col & 1) + wave * 2 * CB / 16 * 256;
-        const int v0 = fresh(((wave * 2 * CB % 16 + ((col & 3) >> 1)) ^ vf) * 16);
-        float f[HB];
-        bool changed = false;
-#pragma unroll
-        for (int h = 0; h < HB; h++) {
-          f[h] = fade[h * 16 + col];
-          changed |= f[h] != 1.0f;
-        }
-        if (__any(changed)) {
-#pragma unroll
-          for (int h = 0; h < HB; h++)
-#pragma unroll
-            for (int c = 0; c < CB; c++) o[h][c] *= f[h];
-        }
-#pragma unroll
-        for (int k = 0; k < kUnit / 32; k++) {
-          s16x8 pb[HB];
-#pragma unroll
-          for (int h = 0; h < HB; h++) pb[h] = lds_read16((lds_u8*)prob + (h * 16 + col) * (kUnit * 2) + ((4 * k + g) ^ pf) * 16);
-#pragma unroll
-          for (int c = 0; c < CB; c++) {
-            const s16x8 av = join(lds_read_tr(t + k * 64 * R + (v0 ^ 32 * c)), lds_read_tr(t + k * 64 * R + 8 * R + (v0 ^ 32 * c ^ 16)));
-#pragma unroll
-            for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av, pb[h], o[h][c]);
-          }
-        }
-      }
-      if (i == units) break;
     }
-    n++;
-    if (left > 0) {
-      do next++;
-      while (ld_const(&d.w.items[next].len) == 0);
-      load_q(next);
-    }
-
-    // the heads' sums of probabilities, over a wave's lanes and the waves of a head block
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (scores && g == 0) {
-      tops[HB == 4 ? tb >> 1 : tb][hb * 16 + col] = l;
-      if (tb == 0) last_top[hb * 16 + col] = m;
-    }
-    VIB3_WAIT_VM(0);  // the next queries, before the stores below: those are not waited for
-    __syncthreads();
-    const bool whole = unit == 0 && units == (len + kUnit - 1) / kUnit;
-    const int r = x / groups, h0 = (x - r * groups) * 64;
-    const int fcol = fresh(col), fg = fresh(g);
+    const int r = at.item / groups, h0 = (at.item - r * groups) * 64;
+    const int col = fresh(lane) & 15, c0 = pw * CB * 16 + 4 * (fresh(lane) >> 4);
+    const float2* st = stats[k & 1];  // of unit k - 2, the item's last
+    if (at.unit == 0 && at.units == (at.len + kUnit - 1) / kUnit) {
+      uint16_t* out = d.w.ol + ((size_t)r * padded_heads(a.heads) + h0 + col) * R + c0;
 #pragma unroll
-    for (int h = 0; h < HB; h++) {
-      const int at = h * 16 + fcol, head = h0 + at;
-      const float sum = HB == 4 ? tops[0][at] + tops[1][at] : (tops[0][at] + tops[1][at]) + (tops[2][at] + tops[3][at]);
-      if (head >= a.heads) continue;
-      const int c0 = wave * CB * 16 + 4 * fg;
-      if (whole) {
+      for (int h = 0; h < HB; h++) {
+        const float sum = st[h * 16 + col].y;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t* out = d.w.ol + ((size_t)r * a.heads + head) * R + c0;
 #pragma unroll
         for (int c = 0; c < CB; c++)
-          *(uint2*)(out + 16 * c) =
+          *(uint2*)(out + h * 16 * R + 16 * c) =
               make_uint2(pack2<DT>(o[h][c][0] * inv, o[h][c][1] * inv), pack2<DT>(o[h][c][2] * inv, o[h][c][3] * inv));
-      } else {
-        const size_t slot = (2 * (size_t)blockIdx.x + (first_of_share == 0 ? 0 : 1)) * group_heads(a.heads) + at;
-        float* out = d.w.part + slot * R + c0;
-#pragma unroll
-        for (int c = 0; c < CB; c++) *(float4*)(out + 16 * c) = make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
-        if (fg == 0 && wave == 0) d.w.stat[slot] = make_float2(last_top[at], sum);
       }
+    } else {
+      const size_t slot = (2 * (size_t)blockIdx.x + (starts_share ? 0 : 1)) * (HB * 16);
+      float* out = d.w.part + (slot + col) * R + c0;
+#pragma unroll
+      for (int h = 0; h < HB; h++)
+#pragma unroll
+        for (int c = 0; c < CB; c++) *(float4*)(out + h * 16 * R + 16 * c) = make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
+      if (pw == 0 && lane < HB * 16) d.w.stat[slot + lane] = st[lane];
     }
-    if (left == 0) break;
-    x = next;
-    unit = 0;
-    len = ld_const(&d.w.items[x].len);
-    units = (int)min((int64_t)((len + kUnit - 1) / kUnit), left);
-  }
+  } while (at.step());
+  wait_lds_loads();  // those of the stream's empty end: not into LDS that is no longer this workgroup's
 }
 
 // ------------------------------------------------------------------------- joined rows and W_uv
@@ -523,7 +547,7 @@ __global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
       const int w0 = (int)(lo / per), parts = (int)((hi - 1) / per) - w0 + 1;
       if (parts == 1) {
         if (mate == 0) {
-          const uint16_t* p = d.w.ol + ((size_t)r * a.heads + h) * R + lane * kCols;
+          const uint16_t* p = d.w.ol + ((size_t)r * padded_heads(a.heads) + h) * R + lane * kCols;
 #pragma unroll
           for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
         }
