@@ -86,7 +86,9 @@ __device__ __forceinline__ int row_len(const vib3_mla_decode& a, int r, int* seq
 
 // One workgroup of 256: running sums of the items' units, the share size, and the item each share starts in.
 __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
+  constexpr int kLocal = 1024;  // with more items the search below goes through memory
   __shared__ int64_t wave_total[4];
+  __shared__ int64_t begins[kLocal + 1];
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int groups = head_groups(a.heads), items = a.rows * groups;
   int64_t before = 0;
@@ -108,12 +110,16 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
       if (i < (tid >> 6)) base += wave_total[i];
       before += wave_total[i];
     }
-    if (x < items) w.items[x] = Item{base + sum - n, len, seq};
+    if (x < items) {
+      w.items[x] = Item{base + sum - n, len, seq};
+      if (x < kLocal) begins[x] = base + sum - n;
+    }
     __syncthreads();
   }
   const int64_t per = max((int64_t)kMinUnits, (before + kShares - 1) / kShares);
   if (tid == 0) {
     w.items[items] = Item{before, 0, 0};
+    if (items <= kLocal) begins[items] = before;
     w.head[0] = per;
     w.head[1] = before;
   }
@@ -124,15 +130,15 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
     w.shares[tid].total = 0;
     return;
   }
+  auto begin = [&](int x) { return items <= kLocal ? begins[x] : w.items[x].begin; };
   int lo = 0, hi = items;  // the last item that begins at or before the share's first unit: the one that holds it
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (w.items[mid].begin <= from) lo = mid;
+    if (begin(mid) <= from) lo = mid;
     else hi = mid;
   }
   const Item it = w.items[lo];
-  w.shares[tid] = Share{to - from, lo, it.seq, it.len, (int32_t)(from - it.begin),
-                        (int32_t)(min(to, w.items[lo + 1].begin) - from), 0};
+  w.shares[tid] = Share{to - from, lo, it.seq, it.len, (int32_t)(from - it.begin), (int32_t)(min(to, begin(lo + 1)) - from), 0};
 }
 
 __global__ __launch_bounds__(256) void k_mla_plan(DecodeArgs d) { make_plan(d.a, d.w); }
@@ -151,12 +157,12 @@ __device__ __forceinline__ int absorb_swizzle(int n) { return ((n & 3) << 2) ^ (
 template <int DT>
 __global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks) {
   const vib3_mla_decode& a = d.a;
-  __shared__ __align__(16) uint8_t tile[256 * kAbsorbCols * 2];
-  if ((int)blockIdx.x == a.heads * col_blocks) {
+  extern __shared__ __align__(16) uint8_t tile[];  // [nope][kAbsorbCols]
+  if (blockIdx.x == 0) {  // first: the next launch waits for it
     if (blockIdx.y == 0) make_plan(a, d.w);
     return;
   }
-  const int h = (int)blockIdx.x / col_blocks, c0 = ((int)blockIdx.x % col_blocks) * kAbsorbCols;
+  const int h = (int)(blockIdx.x - 1) / col_blocks, c0 = ((int)(blockIdx.x - 1) % col_blocks) * kAbsorbCols;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rank = a.cache.rank;
   const uint16_t* w = (const uint16_t*)a.kv_b + (size_t)h * (a.nope + a.v_dim) * rank + c0;
@@ -212,7 +218,7 @@ __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 // phases, with three barriers, took 4600.
 //
 // Rows go from the pages straight to LDS (16 bytes a lane) into a ring of four units, two in use and two in flight (74 KB a CU,
-// 19 MB over the chip); the stream runs on from one item of the share to the next. The page numbers travel the same way, two
+// 19 MB over the chip); the stream runs on from one item of the share to the next. The page numbers travel the same way, three
 // units ahead of the rows, so that no load is ever waited for but in the order of the ring (one count, kLoads a unit).
 // The latent parts of the rows and the rotary parts lie apart, so that one load instruction covers whole rows. Chunk c (16 bytes)
 // of a latent part lies at c ^ row_swizzle(row): the rows' stride is a multiple of all 64 banks, and so the 16 rows of a score
@@ -278,6 +284,7 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
   constexpr int kPer = 64 / RC;                        // latent parts of one load instruction: 1 or 2
   constexpr int kLoads = kTpw / kPer + 2;              // a wave's load instructions per unit: latents, rotary parts, page numbers
   constexpr int CB = R / 16 / 4;                       // 16-column blocks of a wave's sums
+  static_assert(CB == kTpw / kPer, "a load instruction goes with each of them");
   __shared__ __align__(1024) uint8_t lat[kRing][kUnit * R * 2];
   __shared__ __align__(1024) uint8_t rot[kRing][kUnit * 128];
   __shared__ __align__(16) uint8_t prob[2][HB * 16 * kUnit * 2];  // [head][token], chunk c of a row at c ^ (head / 4) % 4
@@ -413,43 +420,58 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
       }
     }
   };
-  // Unit k's rows into ring place k % kRing (rows of zeros once the stream is through), eight lanes finding the address of each.
-  auto issue = [&](int k) {
+  // The addresses of unit k's rows, eight lanes for each (a row of zeros for those not seen, and once the stream is through).
+  uint64_t row = 0;
+  bool row_seen = false;
+  auto aim = [&](int k) {
+    const int id = page_no[k % kRing][pw][lane >> 3], off = place[k % kRing][pw][lane >> 3];
+    row_seen = off >= 0 && (unsigned)id < (unsigned)a.cache.num_pages;
+    row = row_seen ? (uint64_t)(uintptr_t)((const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
+                                           (int64_t)off * a.cache.row_stride)
+                   : (uint64_t)(uintptr_t)zero_row;
+  };
+  // One of the loads of the unit aimed at into ring place k % kRing: latent parts i * kPer on, or at the end the rotary parts.
+  constexpr int kIssues = kTpw / kPer + 1;
+  auto issue = [&](int k, int i) {
     const int slot = k % kRing;
-    const int ln = fresh(lane);
-    const int id = page_no[slot][pw][ln >> 3], off = place[slot][pw][ln >> 3];
-    const bool ok = off >= 0 && (unsigned)id < (unsigned)a.cache.num_pages;
-    const uint64_t row = ok ? (uint64_t)(uintptr_t)((const uint16_t*)a.cache.pool + (int64_t)id * a.cache.page_stride +
-                                                    (int64_t)off * a.cache.row_stride)
-                            : (uint64_t)(uintptr_t)zero_row;
-    if ((ln & 7) == 0) seen[slot][pw * kTpw + (ln >> 3)] = ok ? 1.0f : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kTpw / kPer; i++) {
-      const int t = i * kPer + (kPer == 2 ? ln >> 5 : 0);
+    if (i < kIssues - 1) {
+      const int t = i * kPer + (kPer == 2 ? lane >> 5 : 0);
       const uint8_t* p = lane_ptr(row, 8 * i * kPer);
       if (kPer == 2) {
         const uint8_t* p1 = lane_ptr(row, 8 * i * kPer + 8);
-        p = ln >= 32 ? p1 : p;
+        p = lane >= 32 ? p1 : p;
       }
-      load_to_lds16(p + ((ln & (RC - 1)) ^ row_swizzle(pw * kTpw + t)) * 16, (lds_u8*)lat[slot] + (pw * kTpw + i * kPer) * R * 2);
+      load_to_lds16(p + ((fresh(lane) & (RC - 1)) ^ row_swizzle(pw * kTpw + t)) * 16, (lds_u8*)lat[slot] + (pw * kTpw + i * kPer) * R * 2);
+    } else {
+      const int ln = fresh(lane);
+      const int c = (ln & 7) ^ ((ln >> 4) & 3) ^ (pw & 1) * 4;  // (row / 2) % 8 of row pw * 8 + lane / 8
+      if (PC == 8 || c < PC) load_to_lds16((const uint8_t*)(uintptr_t)row + R * 2 + c * 16, (lds_u8*)rot[slot] + pw * kTpw * 128);
+      if ((ln & 7) == 0) seen[slot][pw * kTpw + (ln >> 3)] = row_seen ? 1.0f : 0.0f;
     }
-    const int c = (ln & 7) ^ ((ln >> 4) & 3) ^ (pw & 1) * 4;  // (row / 2) % 8 of row pw * 8 + lane / 8
-    if (PC == 8 || c < PC) load_to_lds16((const uint8_t*)(uintptr_t)row + R * 2 + c * 16, (lds_u8*)rot[slot] + pw * kTpw * 128);
   };
-  // Unit k's rows, and the page numbers of unit k + 2, have landed for this wave once no more than the next unit's loads are out.
+  auto issue_all = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < kIssues; i++) issue(k, i);
+  };
+  // Unit k's rows, and the page numbers of unit k + 3, have landed for this wave once no more than the next unit's loads are out.
   auto landed = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory"); };
 
   look_up(0);
   look_up(1);
-  wait_lds_loads();
-  issue(0);
   look_up(2);
-  issue(1);
+  wait_lds_loads();
+  aim(0);
+  issue_all(0);
   look_up(3);
+  aim(1);
+  issue_all(1);
+  look_up(4);
+  aim(2);
   landed();
   __syncthreads();
-  issue(2);
-  look_up(4);
+  issue_all(2);
+  look_up(5);
+  aim(3);
   int k = 1;
   do {
     f32x4 o[HB][CB] = {};
@@ -457,34 +479,40 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
     for (int i = 0; i < at.units; i++, k++) {
       landed();
       __syncthreads();  // unit k and the probabilities of unit k - 1 are there; unit k - 2 is done with
-      issue(k + 2);
-      look_up(k + 4);
       const int ln = fresh(lane), g = ln >> 4, col = ln & 15;
       // rows vrow and vrow + 4, chunk ch ^ vf of column block c: ch = 2 (pw CB + c) + (col % 4) / 2, and vf ^ 1 in the second row
       const int vrow = 8 * g + (col >> 2), vf = row_swizzle(vrow);
       lds_u8* t = (lds_u8*)lat[(k - 1) % kRing] + vrow * R * 2 + 8 * (col & 1) + pw * 2 * CB / 16 * 256;
       const int v0 = ((pw * 2 * CB % 16 + ((col & 3) >> 1)) ^ vf) * 16;
-      s16x8 pb[HB];
+      auto latents = [&](int c) { return join(lds_read_tr(t + (v0 ^ 32 * c)), lds_read_tr(t + 8 * R + (v0 ^ 32 * c ^ 16))); };
+      s16x8 pb[HB], av[CB];
       float f[HB];
       bool changed = false;
 #pragma unroll
-      for (int h = 0; h < HB; h++) {
-        pb[h] = lds_read16((lds_u8*)prob[(k - 1) & 1] + (h * 16 + col) * (kUnit * 2) + (g ^ (col >> 2)) * 16);
-        f[h] = fade[(k - 1) & 1][h * 16 + col];
-        changed |= f[h] != 1.0f;
-      }
+      for (int h = 0; h < HB; h++) f[h] = fade[(k - 1) & 1][h * 16 + col];
+#pragma unroll
+      for (int h = 0; h < HB; h++) pb[h] = lds_read16((lds_u8*)prob[(k - 1) & 1] + (h * 16 + col) * (kUnit * 2) + (g ^ (col >> 2)) * 16);
+      av[0] = latents(0);
+      av[1] = latents(1);
+#pragma unroll
+      for (int h = 0; h < HB; h++) changed |= f[h] != 1.0f;
       if (__any(changed)) {
 #pragma unroll
         for (int h = 0; h < HB; h++)
 #pragma unroll
           for (int c = 0; c < CB; c++) o[h][c] *= f[h];
       }
+      // the products, with the loads of unit k + 2 spread among them
 #pragma unroll
       for (int c = 0; c < CB; c++) {
-        const s16x8 av = join(lds_read_tr(t + (v0 ^ 32 * c)), lds_read_tr(t + 8 * R + (v0 ^ 32 * c ^ 16)));
+        issue(k + 2, c);
+        if (c + 2 < CB) av[c + 2] = latents(c + 2);
 #pragma unroll
-        for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av, pb[h], o[h][c]);
+        for (int h = 0; h < HB; h++) o[h][c] = mma32<DT>(av[c], pb[h], o[h][c]);
       }
+      issue(k + 2, CB);
+      look_up(k + 5);
+      aim(k + 3);
     }
     const int r = at.item / groups, h0 = (at.item - r * groups) * 64;
     const int col = fresh(lane) & 15, c0 = pw * CB * 16 + 4 * (fresh(lane) >> 4);
@@ -516,33 +544,28 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
 // ------------------------------------------------------------------------- joined rows and W_uv
 
 // A workgroup takes up to 16 rows of one head. Its 16 waves are dealt over the rows: a wave, or where there are fewer rows
-// several, joins a row's parts (the weights of all parts first, then the parts' sums, several loads in flight). The rows' weighted latents
-// go to LDS in 16 bits, and v_dim / 16 waves multiply them by 16 rows of W_uv each, which they have loaded before the join. Without W_uv the weighted latents are the result.
+// several, joins a row's parts. Their statistics and the first parts' sums are read at the same time (a part's place does not
+// depend on its weight). The rows' weighted latents go to LDS in 16 bits, and v_dim / 16 waves multiply them by 16 rows of W_uv
+// each. Without W_uv the weighted latents are the result. Bound by latency: the plan, the parts, W_uv, one after the other; 64
+// registers a lane let two workgroups share a CU, so that up to 512 run at once.
 template <int DT, int R>
-__global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
+__global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
   const vib3_mla_decode& a = d.a;
   constexpr int kStride = R + 8;  // 16 bytes more: rows start in different banks
   constexpr int kCols = R / 64;   // columns of a lane
+  constexpr int kAhead = 2;       // parts in flight
   __shared__ __align__(16) uint16_t lat[16 * kStride];
   __shared__ __align__(16) float sums[16][R];
   const int h = (int)blockIdx.x, r0 = (int)blockIdx.y * 16;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, col = lane & 15;
   const int rows = min(16, a.rows - r0);
-  const uint16_t* wv = (const uint16_t*)a.kv_b + ((size_t)h * (a.nope + a.v_dim) + a.nope + col) * R + 8 * g;
-  s16x8 first[R / 32];
-  const bool product = a.kv_b && wave * 16 < a.v_dim;
-  if (product) {
-#pragma unroll
-    for (int k = 0; k < R / 32; k++) first[k] = *(const s16x8*)(wv + (size_t)wave * 16 * R + k * 32);
-  }
   const int teams = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;  // rows joined at a time
   const int per_row = 16 / teams, i = wave / per_row, mate = wave % per_row;
   {
     const int r = r0 + i, x = r * head_groups(a.heads) + h / 64;
     float o[kCols] = {};
-    const int64_t per = d.w.head[0];
-    const int64_t lo = i < rows ? d.w.items[x].begin : 0, hi = i < rows ? d.w.items[x + 1].begin : 0;
+    const int64_t per = ld_const(d.w.head);
+    const int64_t lo = i < rows ? ld_const(&d.w.items[x].begin) : 0, hi = i < rows ? ld_const(&d.w.items[x + 1].begin) : 0;
     if (hi > lo) {
       const int w0 = (int)(lo / per), parts = (int)((hi - 1) / per) - w0 + 1;
       if (parts == 1) {
@@ -556,6 +579,14 @@ __global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
         const bool late = lo != w0 * per;
         const int hg = group_heads(a.heads), hh = h % 64;
         auto place = [&](int j) { return ((size_t)2 * (w0 + j) + (j == 0 && late ? 1 : 0)) * hg + hh; };
+        float4 ahead[kAhead][kCols / 4];
+        auto fetch = [&](int j, float4* v) {
+          const float* p = d.w.part + place(min(j, parts - 1)) * R + lane * kCols;
+#pragma unroll
+          for (int c = 0; c < kCols / 4; c++) v[c] = *(const float4*)(p + 4 * c);
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) fetch(mate + k * per_row, ahead[k]);
         float2 st[kShares / 64];  // lane l: parts l, l + 64, ...
         float m = -__builtin_huge_valf();
 #pragma unroll
@@ -574,19 +605,26 @@ __global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
         }
         l = wave_sum(l);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int j0 = mate; j0 < parts; j0 += kAhead * per_row) {
 #pragma unroll
-        for (int k = 0; k < kShares / 64; k++) {
-#pragma unroll 4
-          for (int j = 64 * k + mate; j < min(parts, 64 * k + 64); j += per_row) {
-            const float f = __shfl(st[k].x, j - 64 * k) * inv;
-            const float* p = d.w.part + place(j) * R + lane * kCols;
+          for (int k = 0; k < kAhead; k++) {
+            const int j = j0 + k * per_row;
+            float w = st[0].x;
 #pragma unroll
-            for (int c = 0; c < kCols; c += 4) {
-              const float4 v = *(const float4*)(p + c);
-              o[c] += f * v.x;
-              o[c + 1] += f * v.y;
-              o[c + 2] += f * v.z;
-              o[c + 3] += f * v.w;
+            for (int q = 1; q < kShares / 64; q++) w = j >> 6 == q ? st[q].x : w;
+            const float f = j < parts ? __shfl(w, j & 63) * inv : 0.0f;
+            float4 v[kCols / 4];
+#pragma unroll
+            for (int c = 0; c < kCols / 4; c++) v[c] = ahead[k][c];
+            fetch(j + kAhead * per_row, ahead[k]);
+            if (j < parts) {
+#pragma unroll
+              for (int c = 0; c < kCols / 4; c++) {
+                o[4 * c] += f * v[c].x;
+                o[4 * c + 1] += f * v[c].y;
+                o[4 * c + 2] += f * v[c].z;
+                o[4 * c + 3] += f * v[c].w;
+              }
             }
           }
         }
@@ -595,6 +633,13 @@ __global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
 #pragma unroll
     for (int c = 0; c < kCols; c += 4) *(float4*)&sums[wave][lane * kCols + c] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
   }
+  // half of the W_uv rows of this wave meanwhile
+  const int g = lane >> 4, col = lane & 15;
+  const bool product = a.kv_b && wave * 16 < a.v_dim;
+  const uint16_t* wv = (const uint16_t*)a.kv_b + ((size_t)h * (a.nope + a.v_dim) + a.nope + wave * 16 + col) * R + 8 * g;
+  s16x8 first[R / 64];
+#pragma unroll
+  for (int k = 0; k < R / 64; k++) first[k] = product ? *(const s16x8*)(wv + k * 32) : s16x8{};
   __syncthreads();
   for (int at = tid; at < rows * R; at += 1024) {
     const int k = at / R, c = at % R;
@@ -608,9 +653,12 @@ __global__ __launch_bounds__(1024) void k_mla_finish(DecodeArgs d) {
   if (!product) return;
   const int row = min(col, rows - 1);
   f32x4 acc = {};
+  // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
 #pragma unroll
-  for (int k = 0; k < R / 32; k++)  // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
-    acc = mma32<DT>(first[k], *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
+  for (int k = 0; k < R / 64; k++) acc = mma32<DT>(first[k], *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
+#pragma unroll
+  for (int k = R / 64; k < R / 32; k++)
+    acc = mma32<DT>(*(const s16x8*)(wv + k * 32), *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
   if (col < rows)
     *(uint2*)((uint16_t*)a.out + (int64_t)(r0 + col) * a.out_row_stride + (int64_t)h * a.out_head_stride + wave * 16 + 4 * g) =
         make_uint2(pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3]));
@@ -621,8 +669,8 @@ int launch_decode(const DecodeArgs& d, hipStream_t st) {
   const vib3_mla_decode& a = d.a;
   if (a.kv_b) {
     const int col_blocks = R / kAbsorbCols;
-    hipLaunchKernelGGL(k_mla_absorb<DT>, dim3((unsigned)(a.heads * col_blocks + 1), (unsigned)((a.rows + kAbsorbRows - 1) / kAbsorbRows)), dim3(256), 0, st,
-                       d, col_blocks);
+    hipLaunchKernelGGL(k_mla_absorb<DT>, dim3((unsigned)(a.heads * col_blocks + 1), (unsigned)((a.rows + kAbsorbRows - 1) / kAbsorbRows)), dim3(256),
+                       (unsigned)(a.nope * kAbsorbCols * 2), st, d, col_blocks);
   } else {
     hipLaunchKernelGGL(k_mla_plan, dim3(1), dim3(256), 0, st, d);
   }
