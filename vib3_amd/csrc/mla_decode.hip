@@ -9,9 +9,9 @@
 //   k_mla_finish   rows that several workgroups shared are joined, and W_uv applied
 //
 // The plan: tokens are taken 32 at a time (a unit), heads in groups of up to 64. All units of all items
-// (row, head group) in order are cut into kShares equal runs, one workgroup each, whatever the rows' lengths: a long row is
-// shared by many workgroups, a run covers many short rows. Nothing on the host depends on the lengths, so a captured
-// launch follows them.
+// (row, head group) in order, with kItemCost units' time in front of each item for taking it up and storing its sums, are
+// cut into kShares equal runs, one workgroup each, whatever the rows' lengths: a long row is shared by many workgroups, a run
+// covers many short rows. Nothing on the host depends on the lengths, so a captured launch follows them.
 #include "mla.h"
 
 namespace vib3 {
@@ -19,14 +19,16 @@ namespace vib3 {
 constexpr int kMlaMaxRows = 65536;
 constexpr int kUnit = 32;      // cached tokens of one step
 constexpr int kShares = 256;   // workgroups of the attention launch, one per CU (its LDS tiles fill one)
-constexpr int kMinUnits = 1;   // units of a share at least
+constexpr int kItemCost = 3;   // an item's fixed time, in units
 
 // Device workspace. Slot 2w holds the part of the item that share w starts in the middle of, or that it covers the
 // middle of; slot 2w + 1 the part of the item it ends in (if it starts that item).
 struct Item {
-  int64_t begin;      // units before the item
+  int64_t begin;      // where the item begins, in units and fixed times of the items before
   int32_t len, seq;   // visible tokens of its row, and their sequence
 };
+
+__host__ __device__ inline int64_t unit_count(int64_t len) { return (len + kUnit - 1) / kUnit; }
 
 struct Share {        // what a workgroup starts with
   int64_t total;      // its units
@@ -35,7 +37,7 @@ struct Share {        // what a workgroup starts with
 };
 
 struct DecodeWs {
-  int64_t* head;      // [2]: units per share, all units
+  int64_t* head;      // length of a share, in units and fixed times
   Item* items;        // [items + 1]
   Share* shares;      // [kShares]
   uint16_t* ql;       // [rows][heads][rank]
@@ -84,7 +86,8 @@ __device__ __forceinline__ int row_len(const vib3_mla_decode& a, int r, int* seq
 
 // ------------------------------------------------------------------------- the plan
 
-// One workgroup of 256: running sums of the items' units, the share size, and the item each share starts in.
+// One workgroup of 256: where the items begin, the share length, and what each share starts with. An item without tokens has
+// no extent; of any other, the units come after the fixed time, so that a share that ends within that has none of them.
 __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
   constexpr int kLocal = 1024;  // with more items the search below goes through memory
   __shared__ int64_t wave_total[4];
@@ -96,7 +99,7 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
     const int x = x0 + tid;
     int seq = 0;
     const int len = x < items ? row_len(a, x / groups, &seq) : 0;
-    const int64_t n = ((int64_t)len + kUnit - 1) / kUnit;
+    const int64_t n = len > 0 ? unit_count(len) + kItemCost : 0;
     int64_t sum = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -116,29 +119,36 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
     }
     __syncthreads();
   }
-  const int64_t per = max((int64_t)kMinUnits, (before + kShares - 1) / kShares);
+  const int64_t per = max((int64_t)1, (before + kShares - 1) / kShares);
   if (tid == 0) {
     w.items[items] = Item{before, 0, 0};
     if (items <= kLocal) begins[items] = before;
     w.head[0] = per;
-    w.head[1] = before;
   }
   __syncthreads();
   static_assert(kShares == 256, "a thread per share");
   const int64_t from = tid * per, to = min(from + per, before);
-  if (from >= before) {
-    w.shares[tid].total = 0;
-    return;
+  Share sh{0, 0, 0, 0, 0, 0, 0};
+  if (from < before) {
+    auto begin = [&](int x) { return items <= kLocal ? begins[x] : w.items[x].begin; };
+    int lo = 0, hi = items;  // the last item that begins at or before the share
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (begin(mid) <= from) lo = mid;
+      else hi = mid;
+    }
+    const Item it = w.items[lo];
+    const int64_t first = max((int64_t)0, from - it.begin - kItemCost);
+    sh.item = lo;
+    sh.seq = it.seq;
+    sh.len = it.len;
+    sh.unit = (int32_t)first;
+    sh.left = (int32_t)max((int64_t)0, min(to - it.begin - kItemCost, unit_count(it.len)) - first);
+    sh.total = sh.left;
+    for (int x = lo + 1; x < items && begin(x) < to; x++)  // the units of the items that begin in the share
+      sh.total += max((int64_t)0, min(to, begin(x + 1)) - begin(x) - kItemCost);
   }
-  auto begin = [&](int x) { return items <= kLocal ? begins[x] : w.items[x].begin; };
-  int lo = 0, hi = items;  // the last item that begins at or before the share's first unit: the one that holds it
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (begin(mid) <= from) lo = mid;
-    else hi = mid;
-  }
-  const Item it = w.items[lo];
-  w.shares[tid] = Share{to - from, lo, it.seq, it.len, (int32_t)(from - it.begin), (int32_t)(min(to, begin(lo + 1)) - from), 0};
+  w.shares[tid] = sh;
 }
 
 __global__ __launch_bounds__(256) void k_mla_plan(DecodeArgs d) { make_plan(d.a, d.w); }
@@ -567,7 +577,7 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
     const int64_t per = ld_const(d.w.head);
     const int64_t lo = i < rows ? ld_const(&d.w.items[x].begin) : 0, hi = i < rows ? ld_const(&d.w.items[x + 1].begin) : 0;
     if (hi > lo) {
-      const int w0 = (int)(lo / per), parts = (int)((hi - 1) / per) - w0 + 1;
+      const int w0 = (int)((lo + kItemCost) / per), parts = (int)((hi - 1) / per) - w0 + 1;
       if (parts == 1) {
         if (mate == 0) {
           const uint16_t* p = d.w.ol + ((size_t)r * padded_heads(a.heads) + h) * R + lane * kCols;
@@ -576,7 +586,7 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
         }
       } else {
         // part j: slot 2 (w0 + j), but the first one 2 w0 + 1 where its share began with another item
-        const bool late = lo != w0 * per;
+        const bool late = w0 * per < lo;
         const int hg = group_heads(a.heads), hh = h % 64;
         auto place = [&](int j) { return ((size_t)2 * (w0 + j) + (j == 0 && late ? 1 : 0)) * hg + hh; };
         float4 ahead[kAhead][kCols / 4];
