@@ -2,11 +2,11 @@
 // shared key and of the queries' rotary part, in one launch.
 //
 // Bound: bytes for prompts (every value read and written once), the launch for single tokens.
-// A wave takes one kv row: lane l holds rank / 64 neighbouring latent elements, the sum of squares
-// is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the
-// rest takes (part of) the heads of one token: its first rope / 2 threads form the cosines and sines
-// once (the angle and its reduction in 64 bits: positions reach 10^6 radians, where f32 angles are
-// off by 0.03), and each thread turns eight pairs, 32 bytes, of one head at a time.
+// A wave takes one kv row: lane l holds eight neighbouring latent elements (16 bytes; with rank 256 half the lanes), the sum of squares
+// is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the rest takes (part of) the heads of one
+// token: its first rope / 2 threads form the cosines and sines once (the angle and its reduction in 64 bits: positions reach 10^6
+// radians, where f32 angles are off by 0.03) while the queries are on their way, and each thread turns eight pairs, 32 bytes, of
+// one head at a time.
 #include "mla.h"
 
 namespace vib3 {
@@ -45,21 +45,18 @@ __global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGri
       x0 = load_act(a.kv, a.kv_dtype, at + rank + i0);
       x1 = load_act(a.kv, a.kv_dtype, at + rank + i1);
     }
-    // latent: 8 (rank 512) or 4 elements a lane
-    const int n = rank >> 6;
-    float c[8];
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      c[i] = i < n ? load_act(a.kv, a.kv_dtype, at + (size_t)lane * n + i) : 0.0f;
-      ss = __builtin_fmaf(c[i], c[i], ss);
-    }
+    const bool mine = lane * 8 < rank;
+    float c[8] = {};
+    if (mine) load8(a.kv, a.kv_dtype, at + lane * 8, c);
     if (a.norm_weight) {
+      float w[8] = {}, ss = 0.0f;
+      if (mine) unpack8<VIB3_DT_F16>(*(const uint4*)((const uint16_t*)a.norm_weight + lane * 8), w);
+#pragma unroll
+      for (int i = 0; i < 8; i++) ss = __builtin_fmaf(c[i], c[i], ss);
       ss = wave_sum(ss);
       const float inv = 1.0f / sqrtf(ss / (float)rank + a.norm_eps);
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (i < n) c[i] = c[i] * inv * f16_to_f32(((const uint16_t*)a.norm_weight)[lane * n + i]);
+      for (int i = 0; i < 8; i++) c[i] = c[i] * inv * w[i];
     }
     float2 cs = make_float2(0.0f, 0.0f);
     if (lane < half) cs = turn_of(p, a.inv_freq[lane], a.rope_scale);
@@ -68,9 +65,7 @@ __global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGri
     for (int k = 0; k < 2; k++) {
       uint16_t* dst = k ? copy : row;
       if (!dst) continue;
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (i < n) dst[lane * n + i] = from_f32<DT>(c[i]);
+      if (mine) *(uint4*)(dst + lane * 8) = pack8<DT>(c);
       if (lane < half) {
         dst[rank + i0] = y0;
         dst[rank + i1] = y1;
@@ -84,27 +79,41 @@ __global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGri
   const int p = a.positions[t];
   if ((unsigned)a.seqs[t] >= (unsigned)a.cache.num_seqs || p < 0) return;
   __shared__ float2 cs[32];
-  if (tid < half) cs[tid] = turn_of(p, a.inv_freq[tid], a.rope_scale);
-  __syncthreads();
   const int units = half / 8;  // threads on one head
-  const int h1 = min(a.heads, h0 + grid.heads_each);
+  const int h1 = min(a.heads, h0 + grid.heads_each), total = (h1 - h0) * units;
   const uint16_t* q = (const uint16_t*)a.q_rope + (int64_t)t * a.q_token_stride;
   uint16_t* o = (uint16_t*)a.q_out + (int64_t)t * a.q_out_token_stride;
-  for (int u = tid; u < (h1 - h0) * units; u += 256) {
-    const int h = h0 + u / units, j = u % units;  // pairs 8j .. 8j + 7 of head h
-    const int e0 = a.interleaved ? 16 * j : 8 * j, e1 = a.interleaved ? 16 * j + 8 : 8 * j + half;
+  // pairs 8j .. 8j + 7 of head h0 + u / units: two runs of eight elements
+  auto first = [&](int u) { return a.interleaved ? 16 * (u % units) : 8 * (u % units); };
+  const int second = a.interleaved ? 8 : half;
+  uint4 x0, x1;
+  auto fetch = [&](int u) {
+    const uint16_t* p = q + (int64_t)(h0 + u / units) * a.q_head_stride + first(u);
+    x0 = *(const uint4*)p;
+    x1 = *(const uint4*)(p + second);
+  };
+  if (tid < total) fetch(tid);
+  if (tid < half) cs[tid] = turn_of(p, a.inv_freq[tid], a.rope_scale);
+  __syncthreads();
+  for (int u = tid; u < total; u += 256) {
     float x[16], y[16];
-    unpack8<DT>(*(const uint4*)(q + (int64_t)h * a.q_head_stride + e0), x);
-    unpack8<DT>(*(const uint4*)(q + (int64_t)h * a.q_head_stride + e1), x + 8);
+    unpack8<DT>(x0, x);
+    unpack8<DT>(x1, x + 8);
+    uint16_t* to = o + (int64_t)(h0 + u / units) * a.q_out_head_stride + first(u);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float2 w = cs[8 * j + i];
-      const int k0 = a.interleaved ? 2 * i : i, k1 = a.interleaved ? 2 * i + 1 : i + 8;
-      y[k0] = x[k0] * w.x - x[k1] * w.y;
-      y[k1] = x[k0] * w.y + x[k1] * w.x;
+      const float2 w = cs[8 * (u % units) + i];
+      if (a.interleaved) {
+        y[2 * i] = x[2 * i] * w.x - x[2 * i + 1] * w.y;
+        y[2 * i + 1] = x[2 * i] * w.y + x[2 * i + 1] * w.x;
+      } else {
+        y[i] = x[i] * w.x - x[i + 8] * w.y;
+        y[i + 8] = x[i] * w.y + x[i + 8] * w.x;
+      }
     }
-    *(uint4*)(o + (int64_t)h * a.q_out_head_stride + e0) = pack8<DT>(y);
-    *(uint4*)(o + (int64_t)h * a.q_out_head_stride + e1) = pack8<DT>(y + 8);
+    if (u + 256 < total) fetch(u + 256);
+    *(uint4*)to = pack8<DT>(y);
+    *(uint4*)(to + second) = pack8<DT>(y + 8);
   }
 }
 
