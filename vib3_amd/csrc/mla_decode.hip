@@ -21,8 +21,9 @@ constexpr int kUnit = 32;      // cached tokens of one step
 constexpr int kShares = 256;   // workgroups of the attention launch, one per CU (its LDS tiles fill one)
 constexpr int kItemCost = 3;   // an item's fixed time, in units
 
-// Device workspace. Slot 2w holds the part of the item that share w starts in the middle of, or that it covers the
-// middle of; slot 2w + 1 the part of the item it ends in (if it starts that item).
+// Device workspace. Slot w holds the part of the item that share w starts with (where it does not cover all of it), slot
+// kShares + w that of the item it ends in, if that is another one. A slot is followed by 2 KB, so that one head's parts, which
+// one workgroup joins, do not all lie in the same memory channels.
 struct Item {
   int64_t begin;      // where the item begins, in units and fixed times of the items before
   int32_t len, seq;   // visible tokens of its row, and their sequence
@@ -42,8 +43,8 @@ struct DecodeWs {
   Share* shares;      // [kShares]
   uint16_t* ql;       // [rows][heads][rank]
   uint16_t* ol;       // [rows][padded heads][rank] weighted latent of items that one share covers
-  float* part;        // [2 kShares][heads of a group][rank] unnormalised sums
-  float2* stat;       // [2 kShares][heads of a group] running maximum (of scores in log2 units) and sum
+  float* part;        // [2 kShares][heads of a group][rank] (and the gap) unnormalised sums
+  float2* stat;       // [heads of a group][2 kShares] reference value (of scores in log2 units) and sum
 };
 
 __host__ __device__ inline int head_groups(int heads) { return (heads + 63) / 64; }
@@ -51,6 +52,7 @@ __host__ __device__ inline int head_blocks(int heads) { return heads <= 16 ? 1 :
 // Heads that a row of weighted latents and a slot of parts have room for: whole blocks, so that nothing is cut off in storing.
 __host__ __device__ inline int padded_heads(int heads) { return heads <= 64 ? head_blocks(heads) * 16 : 128; }
 __host__ __device__ inline int group_heads(int heads) { return head_blocks(heads) * 16; }
+constexpr int kSlotGap = 512;  // floats
 
 inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   size_t at = 0;
@@ -66,7 +68,7 @@ inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   r.shares = (Share*)take(sizeof(Share) * kShares);
   r.ql = (uint16_t*)take(a.kv_b ? 2 * row * a.rows : 0);
   r.ol = (uint16_t*)take(2 * (size_t)padded_heads(a.heads) * a.cache.rank * a.rows);
-  r.part = (float*)take(4 * (size_t)group_heads(a.heads) * a.cache.rank * 2 * kShares);
+  r.part = (float*)take(4 * ((size_t)group_heads(a.heads) * a.cache.rank + kSlotGap) * 2 * kShares);
   r.stat = (float2*)take(8 * (size_t)group_heads(a.heads) * 2 * kShares);
   if (w) *w = r;
   return at;
@@ -539,13 +541,13 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
               make_uint2(pack2<DT>(o[h][c][0] * inv, o[h][c][1] * inv), pack2<DT>(o[h][c][2] * inv, o[h][c][3] * inv));
       }
     } else {
-      const size_t slot = (2 * (size_t)blockIdx.x + (starts_share ? 0 : 1)) * (HB * 16);
-      float* out = d.w.part + (slot + col) * R + c0;
+      const size_t slot = blockIdx.x + (starts_share ? 0 : kShares);
+      float* out = d.w.part + slot * (HB * 16 * R + kSlotGap) + col * R + c0;
 #pragma unroll
       for (int h = 0; h < HB; h++)
 #pragma unroll
         for (int c = 0; c < CB; c++) *(float4*)(out + h * 16 * R + 16 * c) = make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
-      if (pw == 0 && lane < HB * 16) d.w.stat[slot + lane] = st[lane];
+      if (pw == 0 && lane < HB * 16) d.w.stat[lane * (2 * kShares) + slot] = st[lane];
     }
   } while (at.step());
   wait_lds_loads();  // those of the stream's empty end: not into LDS that is no longer this workgroup's
@@ -563,9 +565,10 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
   const vib3_mla_decode& a = d.a;
   constexpr int kStride = R + 8;  // 16 bytes more: rows start in different banks
   constexpr int kCols = R / 64;   // columns of a lane
-  constexpr int kAhead = 2;       // parts in flight
+  constexpr int kAhead = 4;       // parts in flight
   __shared__ __align__(16) uint16_t lat[16 * kStride];
   __shared__ __align__(16) float sums[16][R];
+  __shared__ float weight[16][kShares];  // of the parts of a wave's row
   const int h = (int)blockIdx.x, r0 = (int)blockIdx.y * 16;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = min(16, a.rows - r0);
@@ -585,29 +588,31 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
           for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
         }
       } else {
-        // part j: slot 2 (w0 + j), but the first one 2 w0 + 1 where its share began with another item
+        // part j: slot w0 + j, but the first one kShares + w0 where its share began with another item
         const bool late = w0 * per < lo;
         const int hg = group_heads(a.heads), hh = h % 64;
-        auto place = [&](int j) { return ((size_t)2 * (w0 + j) + (j == 0 && late ? 1 : 0)) * hg + hh; };
-        float4 ahead[kAhead][kCols / 4];
-        auto fetch = [&](int j, float4* v) {
-          const float* p = d.w.part + place(min(j, parts - 1)) * R + lane * kCols;
-#pragma unroll
-          for (int c = 0; c < kCols / 4; c++) v[c] = *(const float4*)(p + 4 * c);
-        };
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) fetch(mate + k * per_row, ahead[k]);
-        float2 st[kShares / 64];  // lane l: parts l, l + 64, ...
-        float m = -__builtin_huge_valf();
+        auto slot = [&](int j) { return (size_t)(w0 + j + (j == 0 && late ? kShares : 0)); };
+        float2 st[kShares / 64];  // lane l: parts l, l + 64, ... (asked for first: loads come back in order)
 #pragma unroll
         for (int k = 0; k < kShares / 64; k++) {
-          st[k] = lane + 64 * k < parts ? d.w.stat[place(lane + 64 * k)] : make_float2(-__builtin_huge_valf(), 0.0f);
-          m = fmaxf(m, st[k].x);
+          st[k] = make_float2(-__builtin_huge_valf(), 0.0f);
+          if (lane + 64 * k < parts) st[k] = d.w.stat[hh * (2 * kShares) + slot(lane + 64 * k)];
         }
+        // kAhead parts at a time, without a branch around a load (past the end: the last one again, with weight 0)
+        float4 v[kAhead][kCols / 4];
+        auto fetch = [&](int j0) {
+#pragma unroll
+          for (int k = 0; k < kAhead; k++) {
+            const float* p = d.w.part + slot(min(j0 + k * per_row, parts - 1)) * (hg * R + kSlotGap) + hh * R + lane * kCols;
+#pragma unroll
+            for (int c = 0; c < kCols / 4; c++) v[k][c] = *(const float4*)(p + 4 * c);
+          }
+        };
+        fetch(mate);
+        float m = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), l = 0.0f;
 #pragma unroll
         for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
         const float base = m == -__builtin_huge_valf() ? 0.0f : m;
-        float l = 0.0f;
 #pragma unroll
         for (int k = 0; k < kShares / 64; k++) {
           st[k].x = __builtin_amdgcn_exp2f(st[k].x - base);
@@ -615,28 +620,25 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
         }
         l = wave_sum(l);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        for (int j0 = mate; j0 < parts; j0 += kAhead * per_row) {
+#pragma unroll
+        for (int k = 0; k < kShares / 64; k++) weight[wave][lane + 64 * k] = st[k].x * inv;
+        for (int j0 = mate;;) {
 #pragma unroll
           for (int k = 0; k < kAhead; k++) {
             const int j = j0 + k * per_row;
-            float w = st[0].x;
+            const float f = j < parts ? weight[wave][j] : 0.0f;
+            if (f == 0.0f) continue;  // (a weight of 0 says nothing about what lies there)
 #pragma unroll
-            for (int q = 1; q < kShares / 64; q++) w = j >> 6 == q ? st[q].x : w;
-            const float f = j < parts ? __shfl(w, j & 63) * inv : 0.0f;
-            float4 v[kCols / 4];
-#pragma unroll
-            for (int c = 0; c < kCols / 4; c++) v[c] = ahead[k][c];
-            fetch(j + kAhead * per_row, ahead[k]);
-            if (j < parts) {
-#pragma unroll
-              for (int c = 0; c < kCols / 4; c++) {
-                o[4 * c] += f * v[c].x;
-                o[4 * c + 1] += f * v[c].y;
-                o[4 * c + 2] += f * v[c].z;
-                o[4 * c + 3] += f * v[c].w;
-              }
+            for (int c = 0; c < kCols / 4; c++) {
+              o[4 * c] += f * v[k][c].x;
+              o[4 * c + 1] += f * v[k][c].y;
+              o[4 * c + 2] += f * v[k][c].z;
+              o[4 * c + 3] += f * v[k][c].w;
             }
           }
+          j0 += kAhead * per_row;
+          if (j0 >= parts) break;
+          fetch(j0);
         }
       }
     }
