@@ -485,7 +485,8 @@ int vib3_launch_moe_mxfp4_batched(const vib3_moe_mxfp4_batch *batch, void *strea
  * (VIB3_ERR_BAD_POINTER otherwise), and the innermost dimension of every tensor is contiguous.
  * Index tensors are int32 on the device and read while the kernels run: an index that is out of
  * its range is never followed (each launcher says what happens instead). Launches are safe inside
- * HIP graph capture and keep no state between calls.
+ * HIP graph capture and keep no state between calls. scale may be any finite number
+ * (VIB3_ERR_UNSUPPORTED otherwise); a row whose scores are all -infinity gives zeros.
  * ---------------------------------------------------------------------------------------- */
 typedef struct vib3_mla_cache {
     void *pool;                 /* [num_pages][page_size][rank + rope] */

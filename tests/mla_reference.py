@@ -99,7 +99,7 @@ def prefill(q_nope, q_rope, kv, k_rope, nq, nk, nope, scale, u):
             k = torch.cat([kv[k0:k0 + b, h, :nope], k_rope[k0:k0 + b]], -1).double()
             q = torch.cat([q_nope[q0:q0 + a, h], q_rope[q0:q0 + a, h]], -1).double()
             seen = torch.arange(b, device=kv.device) <= torch.arange(a, device=kv.device)[:, None] + (b - a)
-            s = torch.where(seen, scale * (q @ k.t()), torch.full((), -math.inf, dtype=torch.float64, device=kv.device))
+            s = (scale * (q @ k.t())).masked_fill(~seen, -math.inf)
             p = softmax(s)
             v = kv[k0:k0 + b, h, nope:].double()
             v = torch.where(torch.isfinite(v), v, torch.zeros_like(v))  # values that only masked places hold

@@ -208,6 +208,31 @@ def test_decode_large_scores(dtype):
     check_decode(c, run_decode(c))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1e-30])
+def test_decode_other_scales(scale):
+    """A scale of 0 (plain averages), a negative one, and one that leaves nothing of the scores; with a masked whole part."""
+    c = decode_case(WIDE, BF16, 20, 16, [900, 50], [(0, 900), (1, 50), (0, 0), (0, 333)], seed=17)
+    c["scale"] = scale
+    c["table"][0, 4:30] = -1
+    check_decode(c, run_decode(c), hole=lambda s, j: s == 0 and 64 <= j < 480)
+
+
+@pytest.mark.parametrize("heads,n", [(8, 1300), (128, 700)])
+def test_decode_more_rows_than_the_plan_keeps_at_hand(heads, n):
+    lens = [(i * 29) % 70 if i % 3 else 0 for i in range(n)]
+    lens[n // 2] = 6000
+    c = decode_case(NARROW, BF16, heads, 16, lens, [(i, m) for i, m in enumerate(lens)], seed=18)
+    check_decode(c, run_decode(c))
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 8, 9, 17, 33])
+def test_decode_row_counts(n):
+    """Rows that share a finishing workgroup, each in many parts."""
+    lens = [700 + 13 * i for i in range(n)]
+    c = decode_case(WIDE, F16, 9, 32, lens, [(i, m) for i, m in enumerate(lens)], seed=19)
+    check_decode(c, run_decode(c))
+
+
 def test_decode_missing_pages_are_not_seen():
     """Pages that are not resident (in the middle, at the end, all of them) count as masked."""
     ps = 16
@@ -370,6 +395,23 @@ def test_prefill_longer_prompt():
 
 def test_prefill_large_scores():
     c = prefill_case(WIDE, F16, 2, [300], [300], seed=5, q_scale=60.0)
+    check_prefill(c, run_prefill(c))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05])
+def test_prefill_other_scales(scale):
+    from vib3_amd import mla
+    c = prefill_case(WIDE, BF16, 2, [200, 9], [230, 4], seed=12)
+    got = mla.mla_prefill(c["q"][..., :128], c["q"][..., 128:], c["kv"], c["rows"][:, 512:], offsets(c["nq"]), offsets(c["nk"]), scale)
+    want, tol = R.prefill(c["q"][..., :128], c["q"][..., 128:], c["kv"], c["rows"][:, 512:], c["nq"], c["nk"], 128, scale,
+                          R.half_step(BF16))
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("n", [2100, 4200])
+def test_prefill_many_blocks(n):
+    """Enough queries and heads for the wide workgroups."""
+    c = prefill_case(NARROW, BF16, 64, [n], [n], seed=13)
     check_prefill(c, run_prefill(c))
 
 

@@ -84,6 +84,7 @@ def test_append_refusals(kw, code):
     (dict(v_dim=288), UNSUPPORTED), (dict(v_dim=0), UNSUPPORTED), (dict(lens=None), BAD_POINTER), (dict(q_nope=AT + 2), BAD_POINTER),
     (dict(q_rope=None), BAD_POINTER), (dict(kv_b=AT + 8), BAD_POINTER), (dict(out=None), BAD_POINTER),
     (dict(q_nope_head_stride=100), BAD_POINTER), (dict(out_row_stride=1023), BAD_POINTER), (dict(workspace=None), BAD_POINTER),
+    (dict(scale=float("nan")), UNSUPPORTED), (dict(scale=float("inf")), UNSUPPORTED),
     (dict(workspace=AT + 16), BAD_POINTER), (dict(workspace_bytes=0), WORKSPACE), (dict(rows=2 ** 30), BAD_COUNT),
 ])
 def test_decode_refusals(kw, code):
@@ -97,6 +98,7 @@ def test_decode_refusals(kw, code):
     (dict(q_rope=AT + 2), BAD_POINTER), (dict(kv=None), BAD_POINTER), (dict(k_rope=None), BAD_POINTER), (dict(out=AT + 8), BAD_POINTER),
     (dict(kv_head_stride=252), BAD_POINTER), (dict(k_rope_stride=60), BAD_POINTER), (dict(out_head_stride=129), BAD_POINTER),
     (dict(q_tokens=2 ** 31 - 1, heads=65535), BAD_COUNT),
+    (dict(scale=float("-inf")), UNSUPPORTED),
 ])
 def test_prefill_refusals(kw, code):
     refused("vib3_launch_mla_prefill", prefill(**kw), code)

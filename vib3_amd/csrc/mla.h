@@ -67,6 +67,13 @@ __device__ __forceinline__ int clamp_len(const vib3_mla_cache& c, int n) {
   return n <= 0 ? 0 : n > cap ? (int)cap : n;
 }
 
+// The factor of scores as exponents of two. A negative scale goes into the queries' signs (sign_flip); one of 0 becomes the smallest
+// number, so that an empty maximum (-infinity) times it stays what it is.
+__device__ __forceinline__ float exponent_scale(float scale) {
+  return fmaxf(__builtin_fabsf(scale) * 1.44269504088896341f, 1.17549435e-38f);
+}
+__device__ __forceinline__ uint32_t sign_flip(float scale) { return scale < 0.0f ? 0x80008000u : 0u; }
+
 // Host checks shared by the launchers.
 inline bool mla_aligned(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
 inline bool mla_stride(int64_t s) { return s % 8 == 0; }
@@ -90,14 +97,12 @@ namespace vib3 {
 
 // ------------------------------------------------------------------------- matrix cores
 //
-// Operand layouts of the 16x16 products: lane l holds row (A) or column (B) l % 16 at
-// k = 8 (l / 16) + 0..7 (k = 4 (l / 16) + 0..3 for the 16-deep one); of the result, column l % 16 of rows
-// 4 (l / 16) + 0..3.
+// Operand layouts of the 16x16x32 products: lane l holds row (A) or column (B) l % 16 at k = 8 (l / 16) + 0..7; of the
+// result, column l % 16 of rows 4 (l / 16) + 0..3.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -107,13 +112,6 @@ __device__ __forceinline__ f32x4 mma32(s16x8 a, s16x8 b, f32x4 c) {
   if (DT == VIB3_DT_F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <int DT>
-__device__ __forceinline__ f32x4 mma16(s16x4 a, s16x4 b, f32x4 c) {
-  if (DT == VIB3_DT_F16)
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
 }
 
 // Two f32 rounded to a pair of 16-bit elements (nearest even).

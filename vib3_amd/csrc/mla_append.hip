@@ -3,19 +3,13 @@
 //
 // Bound: bytes for prompts (every value read and written once), the launch for single tokens.
 // A wave takes one kv row: lane l holds eight neighbouring latent elements (16 bytes; with rank 256 half the lanes), the sum of squares
-// is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the rest takes (part of) the heads of one
+// is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the rest takes the heads of one
 // token: its first rope / 2 threads form the cosines and sines once (the angle and its reduction in 64 bits: positions reach 10^6
 // radians, where f32 angles are off by 0.03) while the queries are on their way, and each thread turns eight pairs, 32 bytes, of
 // one head at a time.
 #include "mla.h"
 
 namespace vib3 {
-
-struct AppendGrid {
-  int kv_blocks;    // workgroups of four kv rows
-  int splits;       // workgroups over one token's heads
-  int heads_each;   // heads of each of them
-};
 
 // Cosine and sine of p * inv_freq, times g.
 __device__ __forceinline__ float2 turn_of(int p, float inv_freq, float g) {
@@ -27,10 +21,10 @@ __device__ __forceinline__ float2 turn_of(int p, float inv_freq, float g) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGrid grid) {
+__global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, int kv_blocks) {
   const int tid = (int)threadIdx.x;
   const int rank = a.cache.rank, rope = a.cache.rope, half = rope / 2;
-  if ((int)blockIdx.x < grid.kv_blocks) {
+  if ((int)blockIdx.x < kv_blocks) {
     const int t = (int)blockIdx.x * 4 + (tid >> 6), lane = tid & 63;
     if (t >= a.tokens) return;
     const int s = a.seqs[t], p = a.positions[t];
@@ -74,21 +68,20 @@ __global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGri
     return;
   }
   // the queries' rotary part
-  const int b = (int)blockIdx.x - grid.kv_blocks;
-  const int t = b / grid.splits, h0 = (b - t * grid.splits) * grid.heads_each;
+  const int t = (int)blockIdx.x - kv_blocks;
   const int p = a.positions[t];
   if ((unsigned)a.seqs[t] >= (unsigned)a.cache.num_seqs || p < 0) return;
   __shared__ float2 cs[32];
   const int units = half / 8;  // threads on one head
-  const int h1 = min(a.heads, h0 + grid.heads_each), total = (h1 - h0) * units;
+  const int total = a.heads * units;
   const uint16_t* q = (const uint16_t*)a.q_rope + (int64_t)t * a.q_token_stride;
   uint16_t* o = (uint16_t*)a.q_out + (int64_t)t * a.q_out_token_stride;
-  // pairs 8j .. 8j + 7 of head h0 + u / units: two runs of eight elements
+  // pairs 8 (u % units) .. + 7 of head u / units: two runs of eight elements
   auto first = [&](int u) { return a.interleaved ? 16 * (u % units) : 8 * (u % units); };
   const int second = a.interleaved ? 8 : half;
   uint4 x0, x1;
   auto fetch = [&](int u) {
-    const uint16_t* p = q + (int64_t)(h0 + u / units) * a.q_head_stride + first(u);
+    const uint16_t* p = q + (int64_t)(u / units) * a.q_head_stride + first(u);
     x0 = *(const uint4*)p;
     x1 = *(const uint4*)(p + second);
   };
@@ -99,7 +92,7 @@ __global__ __launch_bounds__(256) void k_mla_append(vib3_mla_append a, AppendGri
     float x[16], y[16];
     unpack8<DT>(x0, x);
     unpack8<DT>(x1, x + 8);
-    uint16_t* to = o + (int64_t)(h0 + u / units) * a.q_out_head_stride + first(u);
+    uint16_t* to = o + (int64_t)(u / units) * a.q_out_head_stride + first(u);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const float2 w = cs[8 * (u % units) + i];
@@ -126,23 +119,21 @@ extern "C" int vib3_launch_mla_append(const vib3_mla_append* args, void* stream)
   const vib3_mla_append& a = *args;
   if (const int rc = check_cache(a.cache)) return rc;
   if (a.kv_dtype != VIB3_DT_F32 && !mla_dtype(a.kv_dtype)) return VIB3_ERR_UNSUPPORTED;
-  if (a.tokens < 0 || (a.q_rope && a.heads < 1)) return VIB3_ERR_BAD_COUNT;
+  if (a.tokens < 0 || (a.q_rope && (a.heads < 1 || a.heads > 65535))) return VIB3_ERR_BAD_COUNT;
   if (a.tokens == 0) return 0;
   if (!a.seqs || !a.positions || !a.inv_freq || !mla_aligned(a.kv) || !mla_stride(a.kv_stride))
     return VIB3_ERR_BAD_POINTER;
   if (a.norm_weight && !mla_aligned(a.norm_weight)) return VIB3_ERR_BAD_POINTER;
   if (a.kv_out && (!mla_aligned(a.kv_out) || !mla_stride(a.kv_out_stride))) return VIB3_ERR_BAD_POINTER;
-  AppendGrid g{(a.tokens + 3) / 4, 1, 0};
-  int64_t blocks = g.kv_blocks;
+  const int kv_blocks = (a.tokens + 3) / 4;
   if (a.q_rope) {
     if (!mla_aligned(a.q_rope) || !mla_aligned(a.q_out) || !mla_stride(a.q_token_stride) || !mla_stride(a.q_head_stride) ||
         !mla_stride(a.q_out_token_stride) || !mla_stride(a.q_out_head_stride))
       return VIB3_ERR_BAD_POINTER;
-    g.heads_each = a.heads;
-    blocks += (int64_t)a.tokens * g.splits;
   }
+  const int64_t blocks = kv_blocks + (a.q_rope ? (int64_t)a.tokens : 0);
   if (blocks > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
   auto kernel = a.cache.dtype == VIB3_DT_F16 ? k_mla_append<VIB3_DT_F16> : k_mla_append<VIB3_DT_BF16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, g);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, kv_blocks);
   VIB3_RETURN_LAUNCH();
 }

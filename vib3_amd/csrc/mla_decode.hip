@@ -21,9 +21,6 @@ constexpr int kUnit = 32;      // cached tokens of one step
 constexpr int kShares = 256;   // workgroups of the attention launch, one per CU (its LDS tiles fill one)
 constexpr int kItemCost = 3;   // an item's fixed time, in units
 
-// Device workspace. Slot w holds the part of the item that share w starts with (where it does not cover all of it), slot
-// kShares + w that of the item it ends in, if that is another one. A slot is followed by 2 KB, so that one head's parts, which
-// one workgroup joins, do not all lie in the same memory channels.
 struct Item {
   int64_t begin;      // where the item begins, in units and fixed times of the items before
   int32_t len, seq;   // visible tokens of its row, and their sequence
@@ -34,9 +31,11 @@ __host__ __device__ inline int64_t unit_count(int64_t len) { return (len + kUnit
 struct Share {        // what a workgroup starts with
   int64_t total;      // its units
   int32_t item, seq, len, unit, left;  // the first item, its units before the share and in it
-  int32_t pad;
 };
 
+// Device workspace. Slot w of the parts holds that of the item that share w starts with (where it does not cover all of it), slot
+// kShares + w that of the item it ends in, if that is another one. A slot is followed by 2 KB, so that one head's parts, which
+// one workgroup joins, do not all lie in the same memory channels.
 struct DecodeWs {
   int64_t* head;      // length of a share, in units and fixed times
   Item* items;        // [items + 1]
@@ -130,7 +129,7 @@ __device__ void make_plan(const vib3_mla_decode& a, const DecodeWs& w) {
   __syncthreads();
   static_assert(kShares == 256, "a thread per share");
   const int64_t from = tid * per, to = min(from + per, before);
-  Share sh{0, 0, 0, 0, 0, 0, 0};
+  Share sh{};
   if (from < before) {
     auto begin = [&](int x) { return items <= kLocal ? begins[x] : w.items[x].begin; };
     int lo = 0, hi = items;  // the last item that begins at or before the share
@@ -319,8 +318,8 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
       return;
     }
     const int g = lane >> 4, col = lane & 15, head_in_group = wave * 16 + col;
-    const float scale = __builtin_fabsf(a.scale) * 1.44269504088896341f;
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale: the queries' signs instead
+    const float scale = exponent_scale(a.scale);
+    const uint32_t flip = sign_flip(a.scale);
     // queries: the B operand, this lane's head at k = 32 s + 8 g
     constexpr int KS = (R + P) / 32;
     s16x8 q[KS], q_next[KS];
@@ -723,6 +722,7 @@ extern "C" int vib3_launch_mla_decode(const vib3_mla_decode* args, void* stream)
   const vib3_mla_decode& a = *args;
   if (const int rc = check_cache(a.cache)) return rc;
   if (!decode_counts(a)) return VIB3_ERR_BAD_COUNT;
+  if (!__builtin_isfinite(a.scale)) return VIB3_ERR_UNSUPPORTED;
   if (a.kv_b && (a.nope < 32 || a.nope > 256 || a.nope % 32 || a.v_dim < 32 || a.v_dim > 256 || a.v_dim % 32))
     return VIB3_ERR_UNSUPPORTED;
   if (a.rows == 0) return 0;

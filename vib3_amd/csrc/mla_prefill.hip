@@ -134,8 +134,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
   const int first_masked = max(bl.first + shift + 1, 0) / kKeys;       // from here on some query does not see all of a tile
 
   // queries: the B operand, this lane's query at k = 16 s + 8 half
-  const float scale = __builtin_fabsf(a.scale) * 1.44269504088896341f;
-  const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;             // a negative scale: the queries' signs instead
+  const float scale = exponent_scale(a.scale);
+  const uint32_t flip = sign_flip(a.scale);
   s16x8 q[KS];
   {
     const int64_t t = bl.q0 + min(qi, bl.nq - 1);
@@ -362,6 +362,7 @@ extern "C" int vib3_launch_mla_prefill(const vib3_mla_prefill* args, void* strea
   if (!mla_dtype(a.dtype) || (a.nope != 64 && a.nope != 128) || (a.v_dim != 64 && a.v_dim != 128) ||
       (a.rope != 32 && a.rope != 64))
     return VIB3_ERR_UNSUPPORTED;
+  if (!__builtin_isfinite(a.scale)) return VIB3_ERR_UNSUPPORTED;
   if (a.heads < 1 || a.heads > 65535 || a.num_seqs < 0 || a.q_tokens < 0 || a.k_tokens < 0) return VIB3_ERR_BAD_COUNT;
   if (a.q_tokens == 0 || a.num_seqs == 0) return 0;
   if (!a.cu_q || !a.cu_k || !mla_aligned(a.q_nope) || !mla_aligned(a.q_rope) || !mla_aligned(a.out) ||
