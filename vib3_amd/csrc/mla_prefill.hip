@@ -330,11 +330,13 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
 
 template <int DT, int N, int P, int V>
 int launch_prefill(const vib3_mla_prefill& a, hipStream_t st) {
-  // Sequences' blocks number at most this many; surplus workgroups end at once.
+  // Sequences' blocks number at most this many; surplus workgroups end at once. 256 queries a workgroup where those fill the
+  // card's 256 CUs (a tile then serves twice the queries: 48 against 53 us at 1000 tokens of 64 heads, 761 against 1060 us at
+  // 6000), 128 where twice the CUs count for more (25 against 28 us at 500, 13 against 15 us at 173).
   const int64_t wide = (a.q_tokens / 256 + a.num_seqs) * (int64_t)a.heads;
   const int64_t narrow = (a.q_tokens / 128 + a.num_seqs) * (int64_t)a.heads;
   if (narrow > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
-  if (wide >= 512)
+  if (wide >= 256)
     hipLaunchKernelGGL((k_mla_prefill<DT, N, P, V, 8>), dim3((unsigned)wide), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((k_mla_prefill<DT, N, P, V, 4>), dim3((unsigned)narrow), dim3(256), 0, st, a);
