@@ -1,13 +1,13 @@
 """The latent-attention operators written out in 64 bits, and how far 16-bit kernels may be off.
 
 A rounding to 16 bits is off by at most u = eps / 2 relative to the value, and by u / sqrt(3) in the mean
-square. The kernels round, beyond their result: the latent query (decode), the probabilities, and the
-weighted latent (decode). With y_j the value that token j brings to an output (W_uv . c_j, or v_j) and Var_p the
+square. The kernels round, beyond their result, the probabilities; the latent query and the weighted latent (decode) are
+held as two 16-bit numbers, off by at most u^2. With y_j the value that token j brings to an output (W_uv . c_j, or v_j) and Var_p the
 variance over the probabilities, the output's mean square error is at most u^2 / 3 times
 
-    scale^2 Var_p(y) sum_i ql_i^2 Var_p(c_i)     the query's (|Cov_p(c_i, y)| <= sd_p(c_i) sd_p(y)),
-  + sum_j p_j^2 y_j^2                            the probabilities',
-  + sum_i o_i^2 W_uv[i]^2                        the weighted latent's.
+    sum_j p_j^2 y_j^2                                  the probabilities',
+  + u^2 scale^2 Var_p(y) sum_i ql_i^2 Var_p(c_i)       the query's (|Cov_p(c_i, y)| <= sd_p(c_i) sd_p(y)),
+  + u^2 sum_i o_i^2 W_uv[i]^2                          the weighted latent's.
 
 Six times its root (the errors are sums of many independent ones, or bounded by sqrt(3) of it where one term is
 all), the result's own rounding u |ref|, and (2^-16 + 96 2^-24 B) sum_j p_j |y_j| for the f32 work bound the difference: B is
@@ -84,7 +84,7 @@ def decode_row(q_nope, q_rope, kv_b, nope, c, kr, scale, u):
         from_p = (y.square() * p.square()[:, None]).sum(-1)
         from_o = torch.bmm(w_uv.square().contiguous(), o.square()[..., None].contiguous())[..., 0]
         size = (y.abs() * p[:, None]).sum(-1)
-    rms = u / math.sqrt(3) * (from_q[:, None] * var_y + from_p + from_o).sqrt()
+    rms = u / math.sqrt(3) * (from_p + u * u * (from_q[:, None] * var_y + from_o)).sqrt()
     return out, u * out.abs() + 6 * rms + f32 * size + tiny(u)
 
 

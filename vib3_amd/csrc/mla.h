@@ -121,6 +121,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
+// Two f32 as pairs of 16-bit elements, each number the sum of its rounding and (but for 2^-16 of it in bf16) the rest.
+struct Halves {
+  uint32_t hi, lo;
+};
+template <int DT>
+__device__ __forceinline__ Halves split2(float a, float b) {
+  const uint32_t hi = pack2<DT>(a, b);
+  const float x = a - to_f32<DT>((uint16_t)(hi & 0xffff)), y = b - to_f32<DT>((uint16_t)(hi >> 16));
+  return Halves{hi, pack2<DT>(__builtin_isfinite(x) ? x : 0.0f, __builtin_isfinite(y) ? y : 0.0f)};
+}
+
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 // 16 bytes a lane from global memory to LDS at base + 16 * lane (base wave-uniform), without passing

@@ -40,8 +40,8 @@ struct DecodeWs {
   int64_t* head;      // length of a share, in units and fixed times
   Item* items;        // [items + 1]
   Share* shares;      // [kShares]
-  uint16_t* ql;       // [rows][heads][rank]
-  uint16_t* ol;       // [rows][padded heads][rank] weighted latent of items that one share covers
+  uint16_t* ql;       // [rows][heads][2][rank] latent queries: rounded to 16 bits, and what the rounding left
+  float* ol;          // [rows][padded heads][rank] weighted latent of items that one share covers
   float* part;        // [2 kShares][heads of a group][rank] (and the gap) unnormalised sums
   float2* stat;       // [heads of a group][2 kShares] reference value (of scores in log2 units) and sum
 };
@@ -65,8 +65,8 @@ inline size_t decode_ws(const vib3_mla_decode& a, DecodeWs* w, void* base) {
   r.head = (int64_t*)take(16);
   r.items = (Item*)take(sizeof(Item) * ((size_t)a.rows * head_groups(a.heads) + 1));
   r.shares = (Share*)take(sizeof(Share) * kShares);
-  r.ql = (uint16_t*)take(a.kv_b ? 2 * row * a.rows : 0);
-  r.ol = (uint16_t*)take(2 * (size_t)padded_heads(a.heads) * a.cache.rank * a.rows);
+  r.ql = (uint16_t*)take(a.kv_b ? 4 * row * a.rows : 0);
+  r.ol = (float*)take(4 * (size_t)padded_heads(a.heads) * a.cache.rank * a.rows);
   r.part = (float*)take(4 * ((size_t)group_heads(a.heads) * a.cache.rank + kSlotGap) * 2 * kShares);
   r.stat = (float2*)take(8 * (size_t)group_heads(a.heads) * 2 * kShares);
   if (w) *w = r;
@@ -206,10 +206,15 @@ __global__ __launch_bounds__(256) void k_mla_absorb(DecodeArgs d, int col_blocks
     }
   }
   if (r < a.rows) {
-    uint16_t* o = d.w.ql + ((size_t)r * a.heads + h) * rank + c0 + 4 * g;
+    uint16_t* o = d.w.ql + ((size_t)r * a.heads + h) * 2 * rank + c0 + 4 * g;
+    // A rounding of the latent query alone would double the result's error (0.0034 against 0.0017 relative in bf16, together
+    // with one of the weighted latent); the remainder costs products, but no further reads of the cached rows.
 #pragma unroll
-    for (int blk = 0; blk < 8; blk++)  // rounded for the matrix cores: relative error half a step
-      *(uint2*)(o + 16 * blk) = make_uint2(pack2<DT>(acc[blk][0], acc[blk][1]), pack2<DT>(acc[blk][2], acc[blk][3]));
+    for (int blk = 0; blk < 8; blk++) {
+      const Halves x = split2<DT>(acc[blk][0], acc[blk][1]), y = split2<DT>(acc[blk][2], acc[blk][3]);
+      *(uint2*)(o + 16 * blk) = make_uint2(x.hi, y.hi);
+      *(uint2*)(o + rank + 16 * blk) = make_uint2(x.lo, y.lo);
+    }
   }
 }
 
@@ -318,32 +323,28 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
       return;
     }
     const int g = lane >> 4, col = lane & 15, head_in_group = wave * 16 + col;
-    const float scale = exponent_scale(a.scale);
-    const uint32_t flip = sign_flip(a.scale);
-    // queries: the B operand, this lane's head at k = 32 s + 8 g
+    const float scale = exponent_scale(a.scale), sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    // queries: the B operand, this lane's head at k = 32 s + 8 g; the latent part in two summands
     constexpr int KS = (R + P) / 32;
-    s16x8 q[KS], q_next[KS];
+    s16x8 q[KS], q_low[R / 32] = {};
     auto load_q = [&](int x) {
       const int r = x / groups;
       const int64_t h = min((x - r * groups) * 64 + head_in_group, a.heads - 1);
-      const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + h) * R
+      const uint16_t* ql = a.kv_b ? d.w.ql + ((size_t)r * a.heads + h) * 2 * R
                                   : (const uint16_t*)a.q_nope + r * a.q_nope_row_stride + h * a.q_nope_head_stride;
       const uint16_t* qr = (const uint16_t*)a.q_rope + r * a.q_rope_row_stride + h * a.q_rope_head_stride;
 #pragma unroll
-      for (int s = 0; s < KS; s++) q_next[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
+      for (int s = 0; s < KS; s++) q[s] = *(const s16x8*)(s < R / 32 ? ql + 32 * s + 8 * g : qr + 32 * (s - R / 32) + 8 * g);
+      if (a.kv_b) {
+#pragma unroll
+        for (int s = 0; s < R / 32; s++) q_low[s] = *(const s16x8*)(ql + R + 32 * s + 8 * g);
+      }
     };
     // this lane's row of a 16-token block; 16 rows further the swizzles are the same
     const int k0 = (g ^ row_swizzle(col)) * 16, r0 = (g ^ ((col >> 1) & 7)) * 16;
     load_q(at.item);
     int k = 0;  // unit of the share
     do {
-#pragma unroll
-      for (int s = 0; s < KS; s++) {
-        uint4 v = __builtin_bit_cast(uint4, q_next[s]);
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-        q[s] = __builtin_bit_cast(s16x8, v);
-      }
-      if (at.left > 0) load_q(at.next());  // on its way while this item is worked on
       float m = -__builtin_huge_valf(), l = 0.0f;  // of this lane's head (unscaled scores); l over this lane's own tokens
       for (int i = 0; i < at.units; i++, k++) {
         __syncthreads();  // unit k is in LDS; the probabilities of unit k - 2 are done with
@@ -353,11 +354,16 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
 #pragma unroll
         for (int c = 0; c < R / 32; c++)  // chunk (4 c + g) ^ row_swizzle(col), a constant and two bits away from that of c = 0
 #pragma unroll
-          for (int b = 0; b < 2; b++) s[b] = mma32<DT>(lds_read16(t + b * 32 * R + (k0 ^ c % 4 * 64) + c / 4 * 256), q[c], s[b]);
+          for (int b = 0; b < 2; b++) {
+            const s16x8 key = lds_read16(t + b * 32 * R + (k0 ^ c % 4 * 64) + c / 4 * 256);
+            s[b] = mma32<DT>(key, q[c], s[b]);
+            s[b] = mma32<DT>(key, q_low[c], s[b]);
+          }
 #pragma unroll
         for (int c = 0; c < P / 32; c++)
 #pragma unroll
           for (int b = 0; b < 2; b++) s[b] = mma32<DT>(lds_read16(u + b * 16 * 128 + (r0 ^ 64 * c)), q[R / 32 + c], s[b]);
+        if (i + 1 == at.units && at.left > 0) load_q(at.next());  // on its way during what follows
         float top = -__builtin_huge_valf();
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
           const float vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            s[b][j] = vv[j] != 0.0f ? s[b][j] : -__builtin_huge_valf();
+            s[b][j] = vv[j] != 0.0f ? s[b][j] * sign : -__builtin_huge_valf();
             top = fmaxf(top, s[b][j]);
           }
         }
@@ -529,15 +535,14 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
     const int col = fresh(lane) & 15, c0 = pw * CB * 16 + 4 * (fresh(lane) >> 4);
     const float2* st = stats[k & 1];  // of unit k - 2, the item's last
     if (at.unit == 0 && at.units == (at.len + kUnit - 1) / kUnit) {
-      uint16_t* out = d.w.ol + ((size_t)r * padded_heads(a.heads) + h0 + col) * R + c0;
+      float* out = d.w.ol + ((size_t)r * padded_heads(a.heads) + h0 + col) * R + c0;
 #pragma unroll
       for (int h = 0; h < HB; h++) {
         const float sum = st[h * 16 + col].y;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int c = 0; c < CB; c++)
-          *(uint2*)(out + h * 16 * R + 16 * c) =
-              make_uint2(pack2<DT>(o[h][c][0] * inv, o[h][c][1] * inv), pack2<DT>(o[h][c][2] * inv, o[h][c][3] * inv));
+          *(float4*)(out + h * 16 * R + 16 * c) = make_float4(o[h][c][0] * inv, o[h][c][1] * inv, o[h][c][2] * inv, o[h][c][3] * inv);
       }
     } else {
       const size_t slot = blockIdx.x + (starts_share ? 0 : kShares);
@@ -556,8 +561,8 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
 
 // A workgroup takes up to 16 rows of one head. Its 16 waves are dealt over the rows: a wave, or where there are fewer rows
 // several, joins a row's parts. Their statistics and the first parts' sums are read at the same time (a part's place does not
-// depend on its weight). The rows' weighted latents go to LDS in 16 bits, and v_dim / 16 waves multiply them by 16 rows of W_uv
-// each. Without W_uv the weighted latents are the result. Bound by latency: the plan, the parts, W_uv, one after the other; 64
+// depend on its weight). The rows' weighted latents go to LDS in two 16-bit summands (a rounding alone would show in the result, see
+// k_mla_absorb), and v_dim / 16 waves multiply them by 16 rows of W_uv each. Without W_uv the weighted latents are the result. Bound by latency: the plan, the parts, W_uv, one after the other; 64
 // registers a lane let two workgroups share a CU, so that up to 512 run at once.
 template <int DT, int R>
 __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
@@ -567,7 +572,10 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
   constexpr int kAhead = 4;       // parts in flight
   __shared__ __align__(16) uint16_t lat[16 * kStride];
   __shared__ __align__(16) float sums[16][R];
-  __shared__ float weight[16][kShares];  // of the parts of a wave's row
+  // weights of the parts of a wave's row; later the weighted latents' remainders
+  __shared__ __align__(16) uint8_t both[16 * (kStride * 2 > kShares * 4 ? kStride * 2 : kShares * 4)];
+  float(*const weight)[kShares] = (float(*)[kShares])both;
+  uint16_t* const lat_low = (uint16_t*)both;
   const int h = (int)blockIdx.x, r0 = (int)blockIdx.y * 16;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = min(16, a.rows - r0);
@@ -582,9 +590,9 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
       const int w0 = (int)((lo + kItemCost) / per), parts = (int)((hi - 1) / per) - w0 + 1;
       if (parts == 1) {
         if (mate == 0) {
-          const uint16_t* p = d.w.ol + ((size_t)r * padded_heads(a.heads) + h) * R + lane * kCols;
+          const float* p = d.w.ol + ((size_t)r * padded_heads(a.heads) + h) * R + lane * kCols;
 #pragma unroll
-          for (int c = 0; c < kCols; c++) o[c] = to_f32<DT>(p[c]);
+          for (int c = 0; c < kCols; c += 4) *(float4*)(o + c) = *(const float4*)(p + c);
         }
       } else {
         // part j: slot w0 + j, but the first one kShares + w0 where its share began with another item
@@ -656,8 +664,12 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
     const int k = at / R, c = at % R;
     float v = 0.0f;
     for (int s = 0; s < per_row; s++) v += sums[k * per_row + s][c];
-    if (a.kv_b) lat[k * kStride + c] = from_f32<DT>(v);
-    else ((uint16_t*)a.out)[(int64_t)(r0 + k) * a.out_row_stride + (int64_t)h * a.out_head_stride + c] = from_f32<DT>(v);
+    if (a.kv_b) {
+      const Halves x = split2<DT>(v, 0.0f);
+      lat[k * kStride + c] = (uint16_t)x.hi;
+      lat_low[k * kStride + c] = (uint16_t)x.lo;
+    } else
+      ((uint16_t*)a.out)[(int64_t)(r0 + k) * a.out_row_stride + (int64_t)h * a.out_head_stride + c] = from_f32<DT>(v);
   }
   if (!a.kv_b) return;
   __syncthreads();
@@ -666,10 +678,11 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
   f32x4 acc = {};
   // rows of W_uv times the rows' latents: a lane ends with 4 outputs of one row
 #pragma unroll
-  for (int k = 0; k < R / 64; k++) acc = mma32<DT>(first[k], *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
-#pragma unroll
-  for (int k = R / 64; k < R / 32; k++)
-    acc = mma32<DT>(*(const s16x8*)(wv + k * 32), *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
+  for (int k = 0; k < R / 32; k++) {
+    const s16x8 w = k < R / 64 ? first[k] : *(const s16x8*)(wv + k * 32);
+    acc = mma32<DT>(w, *(const s16x8*)(lat + row * kStride + k * 32 + 8 * g), acc);
+    acc = mma32<DT>(w, *(const s16x8*)(lat_low + row * kStride + k * 32 + 8 * g), acc);
+  }
   if (col < rows)
     *(uint2*)((uint16_t*)a.out + (int64_t)(r0 + col) * a.out_row_stride + (int64_t)h * a.out_head_stride + wave * 16 + 4 * g) =
         make_uint2(pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3]));
