@@ -543,7 +543,8 @@ int vib3_launch_mla_append(const vib3_mla_append *args, void *stream);
  * ([rows][heads][rank]). Tokens on pages that are not resident are not seen; a row that sees no
  * token (lens[r] <= 0, a sequence outside [0, num_seqs)) is zero; lens[r] beyond the block table
  * counts as its capacity. Softmax statistics and sums in f32; the probabilities are rounded to the
- * cache's dtype for the matrix cores, ql and the weighted latent go there as two numbers of it. */
+ * cache's dtype for the matrix cores, ql and the weighted latent go there as two numbers of it
+ * (and have to lie within its range). */
 typedef struct vib3_mla_decode {
     vib3_mla_cache cache;
     int rows, heads;                   /* rows <= 65536, heads 1..128 */

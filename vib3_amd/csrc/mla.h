@@ -67,8 +67,8 @@ __device__ __forceinline__ int clamp_len(const vib3_mla_cache& c, int n) {
   return n <= 0 ? 0 : n > cap ? (int)cap : n;
 }
 
-// The factor of scores as exponents of two. A negative scale goes into the queries' signs (sign_flip); one of 0 becomes the smallest
-// number, so that an empty maximum (-infinity) times it stays what it is.
+// The factor of scores as exponents of two, without its sign: that goes into the queries (sign_flip) or the scores. A scale of 0
+// becomes the smallest number, so that an empty maximum (-infinity) times it stays what it is.
 __device__ __forceinline__ float exponent_scale(float scale) {
   return fmaxf(__builtin_fabsf(scale) * 1.44269504088896341f, 1.17549435e-38f);
 }
@@ -121,7 +121,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
-// Two f32 as pairs of 16-bit elements, each number the sum of its rounding and (but for 2^-16 of it in bf16) the rest.
+// Two f32 as pairs of 16-bit elements: each number's rounding and, rounded again, what that left (in bf16 off by at most 2^-16 of
+// the number, in f16 by 2^-22 of it or 2^-25). A number that rounds to infinity has no rest.
 struct Halves {
   uint32_t hi, lo;
 };

@@ -1,7 +1,8 @@
 // mla_append.hip — new tokens into the paged latent cache: RMSNorm of the latent, rotation of the
 // shared key and of the queries' rotary part, in one launch.
 //
-// Bound: bytes for prompts (every value read and written once), the launch for single tokens.
+// Bound: bytes for prompts (every value read and written once; 6201 tokens of 64 heads, 122 MB, in 28 us: 4.3 TB/s of the 5.0 that
+// a large copy reaches), the launch for single tokens (3.2 us on the device, 12 us a call from Python).
 // A wave takes one kv row: lane l holds eight neighbouring latent elements (16 bytes; with rank 256 half the lanes), the sum of squares
 // is one wave reduction, and the first rope / 2 lanes turn one pair each. A workgroup of the rest takes the heads of one
 // token: its first rope / 2 threads form the cosines and sines once (the angle and its reduction in 64 bits: positions reach 10^6

@@ -7,11 +7,14 @@
 //   k_mla_absorb   ql for all rows, on the matrix cores; one more workgroup plans the next launch
 //   k_mla_attend   the attention in the latent space, over equal shares of all rows' cached tokens
 //   k_mla_finish   rows that several workgroups shared are joined, and W_uv applied
+// At 64 heads of 128 x 512, bf16, the launches' own times: one row of 777 tokens 5 + 14 + 8 us; one of 131072 5 + 45 + 16;
+// 96 rows of 2048 to 12288 (654 MB) 12 + 141 to 157 + 20.
 //
 // The plan: tokens are taken 32 at a time (a unit), heads in groups of up to 64. All units of all items
 // (row, head group) in order, with kItemCost units' time in front of each item for taking it up and storing its sums, are
 // cut into kShares equal runs, one workgroup each, whatever the rows' lengths: a long row is shared by many workgroups, a run
-// covers many short rows. Nothing on the host depends on the lengths, so a captured launch follows them.
+// covers many short rows (without the fixed time 41 rows of 1 to 4100 tokens took 28 us, with it 19). Nothing on the host
+// depends on the lengths, so a captured launch follows them.
 #include "mla.h"
 
 namespace vib3 {
@@ -229,13 +232,15 @@ __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 //              tokens per 16, so that the running maximum and sum stay within the wave; the probabilities go to LDS.
 //   waves 4-7  add to the sums O^T = C^T . P^T of all heads for unit k - 1, a quarter of the latent's columns each (C^T by
 //              transposing reads), and load unit k + 2.
-// With one barrier a unit, and each SIMD with vector work of one wave next to products of the other, a unit takes some
-// 1600 cycles at 64 heads, less than half of what its rows (37 KB) take to arrive at 6 TB/s; all eight waves going through the same
-// phases, with three barriers, took 4600.
+// With one barrier a unit, and each SIMD with vector work of one wave next to products of the other, 96 rows of 64 heads
+// took 133 us; all eight waves going through the same phases, with three barriers, 163. The latent queries' second summand
+// (below) made it 141 to 157: 4.1 to 4.5 TB/s, of the 6.0 that reading alone reaches. Bound by both: a unit's rows come at that rate
+// in 1.6 us, and its reads from LDS (each row once per 16 heads for the scores, and once for the sums) fill some 1400 cycles of
+// the 2 us that it takes, the products 1100.
 //
 // Rows go from the pages straight to LDS (16 bytes a lane) into a ring of four units, two in use and two in flight (74 KB a CU,
 // 19 MB over the chip); the stream runs on from one item of the share to the next. The page numbers travel the same way, three
-// units ahead of the rows, so that no load is ever waited for but in the order of the ring (one count, kLoads a unit).
+// units ahead of the rows' loads, so that no load is ever waited for but in the order of the ring (one count, kLoads a unit).
 // The latent parts of the rows and the rotary parts lie apart, so that one load instruction covers whole rows. Chunk c (16 bytes)
 // of a latent part lies at c ^ row_swizzle(row): the rows' stride is a multiple of all 64 banks, and so the 16 rows of a score
 // operand, and the 8 rows of half a transposing read, fall into different banks; a rotary part has 128 bytes whatever its
@@ -562,8 +567,9 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
 // A workgroup takes up to 16 rows of one head. Its 16 waves are dealt over the rows: a wave, or where there are fewer rows
 // several, joins a row's parts. Their statistics and the first parts' sums are read at the same time (a part's place does not
 // depend on its weight). The rows' weighted latents go to LDS in two 16-bit summands (a rounding alone would show in the result, see
-// k_mla_absorb), and v_dim / 16 waves multiply them by 16 rows of W_uv each. Without W_uv the weighted latents are the result. Bound by latency: the plan, the parts, W_uv, one after the other; 64
-// registers a lane let two workgroups share a CU, so that up to 512 run at once.
+// k_mla_absorb), and v_dim / 16 waves multiply them by 16 rows of W_uv each. Without W_uv the weighted latents are the result.
+// Bound by latency: the plan, the parts, W_uv, one after the other; 64 registers a lane let two workgroups share a CU, so that
+// up to 512 run at once. 8 us for one short row of 64 heads, 16 where 256 parts (34 MB) are joined, 20 for 96 rows.
 template <int DT, int R>
 __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
   const vib3_mla_decode& a = d.a;
