@@ -3,8 +3,8 @@
 // Bound by the matrix cores: 2 (nope + rope + v_dim) flops per visible (query, key, head), 640 at 128 + 64 + 128, against
 // bytes that are read once per 256 queries. 12288 tokens of 64 heads (3.09 TFLOP, bf16): 3.0 to 3.2 ms, 0.97 to 1.03 PFLOP/s, where a
 // large library product reaches 1.22; shorter prompts end unevenly (a workgroup a CU). The reads from LDS, 32 queries a wave,
-// take as long as the products, 2600 cycles a tile of eight waves. A workgroup takes 32 queries of one head per wave and walks over the keys, 64 at a time,
-// with a running maximum and sum per query.
+// take as long as the products, 2600 cycles a tile of eight waves. A workgroup takes 32 queries of one head per wave and walks over
+// the keys, 64 at a time, with a running maximum and sum per query.
 //
 // Scores are formed transposed, S^T = K . Q^T, so that a lane holds one query's scores of 32 of the 64 keys (the other lane
 // of the pair l, l + 32 the rest): the maximum and sum are almost all within a lane, and the probabilities, packed in pairs of
