@@ -74,6 +74,17 @@ __device__ __forceinline__ float exponent_scale(float scale) {
 }
 __device__ __forceinline__ uint32_t sign_flip(float scale) { return scale < 0.0f ? 0x80008000u : 0u; }
 
+// Probabilities are formed as 2^(kProbShift + (score - reference) in log2 units) and rounded to 16 bits for the matrix cores, sums are
+// divided by the sum of the same. The reference of a row follows its running maximum only where that grew by more than kLag: sums are
+// seldom rescaled, and what lies up to 2^kLag above the reference is as exact as what lies below. f16 has steps down to 2^-24 only
+// (below 2^-14 they no longer shrink with the number), and up to 2^16: with 2^(11 + 4) as the largest probability, those down to
+// 2^-25 of the reference keep all of their bits, and no other is off by more than 2^-36 of it. (Without the shift one key 18 nats above
+// 8192 others, which hold the values, took them to 0.) bf16 has f32's range.
+template <int DT>
+constexpr float kProbShift = DT == VIB3_DT_F16 ? 11.0f : 0.0f;
+template <int DT>
+constexpr float kLag = DT == VIB3_DT_F16 ? 4.0f : 8.0f;
+
 // Host checks shared by the launchers.
 inline bool mla_aligned(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
 inline bool mla_stride(int64_t s) { return s % 8 == 0; }

@@ -381,13 +381,12 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
           }
         }
         top = max_over_rows(top);
-        // The reference value of a head's exponentials follows its maximum only where that grew by more than 2^8 (in the
-        // result): probabilities up to 256 are as exact as ones up to 1, and the sums are seldom rescaled.
-        const bool grown = (top - m) * scale > 8.0f || (m == -__builtin_huge_valf() && top > m);
+        // The reference value of a head's exponentials follows its maximum only where that grew by more than kLag.
+        const bool grown = (top - m) * scale > kLag<DT> || (m == -__builtin_huge_valf() && top > m);
         const float f = grown ? __builtin_amdgcn_exp2f((m - top) * scale) : 1.0f;
         m = grown ? top : m;
         l *= f;
-        const float base = m == -__builtin_huge_valf() ? 0.0f : m * scale;
+        const float base = (m == -__builtin_huge_valf() ? 0.0f : m * scale) - kProbShift<DT>;
         if (g == 0) fade[k & 1][head_in_group] = f;
 #pragma unroll
         for (int b = 0; b < 2; b++) {

@@ -253,10 +253,9 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
 #pragma unroll
     for (int i = 0; i < 16; i++) top = fmaxf(top, s[1][i]);
     top = pair_max(top);
-    // The reference value of a query's exponentials follows its maximum only where that grew by more than 2^8 (in the result):
-    // probabilities up to 256 are as exact as ones up to 1, and the sums are seldom rescaled. (Each query by itself: what
-    // others of the wave see does not change its result.)
-    const bool grown = (top - m) * scale > 8.0f || (m == -__builtin_huge_valf() && top > m);
+    // The reference value of a query's exponentials follows its maximum only where that grew by more than kLag. (Each query by
+    // itself: what others of the wave see does not change its result.)
+    const bool grown = (top - m) * scale > kLag<DT> || (m == -__builtin_huge_valf() && top > m);
     if (__any(grown)) {
       const float f = grown ? __builtin_amdgcn_exp2f((m - top) * scale) : 1.0f;
       m = grown ? top : m;
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
 #pragma unroll
       for (int c = 0; c < VB; c++) o[c] *= f;
     }
-    const float base = m == -__builtin_huge_valf() ? 0.0f : m * scale;
+    const float base = (m == -__builtin_huge_valf() ? 0.0f : m * scale) - kProbShift<DT>;
     uint32_t p[16];
 #pragma unroll
     for (int b = 0; b < 2; b++)
