@@ -1,10 +1,13 @@
-"""GPU tests of latent attention (vib3_amd.mla) at the ends of the values' range: long tails behind one key. Results are compared with the definition in 64 bits.
+"""GPU tests of latent attention (vib3_amd.mla) at the ends of the values' range: long tails behind one key, scales far
+above 1. Results are compared with the definition in 64 bits.
 
 Where all of a row's probabilities are of one size, they are rounded alike, and the errors do not average out: the tolerances
 here count a whole half step u of sum_j p_j |y_j| for them, u |result| for the result's own rounding, and 2^-16 sum_j p_j |y_j| for the
 f32 work (mla_reference). In f16, steps end at 2^-24: a probability goes to the matrix cores as 2^11 times its ratio to a
 reference that is no larger than the row's largest, so its error is at most 2^-25 / 2^11 = 2^-36 of the sum of all, whatever
 its size."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -17,6 +20,12 @@ BF16, F16 = torch.bfloat16, torch.float16
 
 def ints(v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def whole(shape, top, dtype, seed):
+    """Whole numbers of -top..top: their products' sums are exact in f32."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-top, top + 1, shape, generator=g, device="cuda").to(dtype)
 
 
 def normal(*shape, dtype, seed):
@@ -138,3 +147,52 @@ def test_largest_key_comes_last(dtype):
             y = rows[:lens[r], :512].double()
             p = R.softmax(y[:, 0] * scale)
             close(got[r, 0], p @ y, flat_tol(p, y, p @ y, R.half_step(dtype)), f"scale {scale}, row {r}")
+
+
+# ------------------------------------------------------------------------------- large scales
+
+
+def best(s, y):
+    """The limit of large scales: the mean of y over the tokens with the highest (whole-numbered) score, in 64 bits."""
+    p = (s == s.amax(-1, keepdim=True)).double()
+    p = p / p.sum(-1, keepdim=True)
+    return p @ y, p @ y.abs()
+
+
+@pytest.mark.parametrize("scale", [1e7, 1e8, -1e9, 1e20, 1e37, 3.4e38, -3.4e38])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("latent", [False, True])
+def test_decode_large_scales(dtype, scale, latent):
+    """Scores are whole numbers, so that from a scale of some hundreds on only the highest ones count. (Without the latent form,
+    W_uk and W_uv each pass 128 columns on as they are.)"""
+    heads, n = 20, 3000
+    rows = whole((n, 576), 3, dtype, 5)
+    q = whole((3, heads, (512 if latent else 128) + 64), 3, dtype, 6)
+    kv_b = None
+    if not latent:
+        kv_b = torch.zeros(heads, 256, 512, device="cuda", dtype=dtype)
+        i = torch.arange(128, device="cuda")
+        kv_b[:, i, i + 100] = 1.0
+        kv_b[:, 128 + i, i + 300] = 1.0
+    lens = [n, 50, 1]
+    got = decode(rows, q, lens, scale, kv_b=kv_b)
+    u = R.half_step(dtype)
+    for r, m in enumerate(lens):
+        x, c = q[r].double(), rows[:m].double()
+        s = (x[:, :512] @ c[:, :512].t() if latent else x[:, :128] @ c[:, 100:228].t()) + x[:, -64:] @ c[:, 512:].t()
+        want, size = best(s if scale > 0 else -s, c[:, :512] if latent else c[:, 300:428])
+        close(got[r], want, u * want.abs() + 2.0 ** -16 * size, f"row {r}")
+
+
+@pytest.mark.parametrize("scale", [1e7, 1e8, -1e9, 1e20, 1e37, 3.4e38, -3.4e38])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads", [3, 128])
+def test_prefill_large_scales(dtype, scale, heads):
+    nq, nk = 530, 700
+    q, kv, kr = whole((nq, heads, 192), 3, dtype, 7), whole((nk, heads, 256), 3, dtype, 8), whole((nk, 64), 3, dtype, 9)
+    got = prefill(q, kv, kr, 128, scale)
+    seen = torch.arange(nk, device="cuda") <= torch.arange(nq, device="cuda")[:, None] + nk - nq
+    for h in range(0, heads, max(1, heads // 4)):
+        s = q[:, h, :128].double() @ kv[:, h, :128].double().t() + q[:, h, 128:].double() @ kr.double().t()
+        want, size = best((s if scale > 0 else -s).masked_fill(~seen, -math.inf), kv[:, h, 128:].double())
+        close(got[:, h], want, R.half_step(dtype) * want.abs() + 2.0 ** -16 * size, f"head {h}")

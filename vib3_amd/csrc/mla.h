@@ -68,10 +68,13 @@ __device__ __forceinline__ int clamp_len(const vib3_mla_cache& c, int n) {
 }
 
 // The factor of scores as exponents of two, without its sign: that goes into the queries (sign_flip) or the scores. A scale of 0
-// becomes the smallest number, so that an empty maximum (-infinity) times it stays what it is.
+// becomes the smallest number, so that an empty maximum (-infinity) times it stays what it is, and one past f32's range the largest.
 __device__ __forceinline__ float exponent_scale(float scale) {
-  return fmaxf(__builtin_fabsf(scale) * 1.44269504088896341f, 1.17549435e-38f);
+  return fminf(fmaxf(__builtin_fabsf(scale) * 1.44269504088896341f, 1.17549435e-38f), 3.40282347e+38f);
 }
+// Exponents are formed as fma(score, scale, -m * scale), one operation, with the rounding of m * scale in all that a reference m
+// serves: 2^-17 for products up to this. Beyond (by 2^27 it would leave f16's range), m is taken off the scores first.
+constexpr float kFarExponent = 256.0f;
 __device__ __forceinline__ uint32_t sign_flip(float scale) { return scale < 0.0f ? 0x80008000u : 0u; }
 
 // Probabilities are formed as 2^(kProbShift + (score - reference) in log2 units) and rounded to 16 bits for the matrix cores, sums are

@@ -46,7 +46,7 @@ struct DecodeWs {
   uint16_t* ql;       // [rows][heads][2][rank] latent queries: rounded to 16 bits, and what the rounding left
   float* ol;          // [rows][padded heads][rank] weighted latent of items that one share covers
   float* part;        // [2 kShares][heads of a group][rank] (and the gap) unnormalised sums
-  float2* stat;       // [heads of a group][2 kShares] reference value (of scores in log2 units) and sum
+  float2* stat;       // [heads of a group][2 kShares] reference value (of unscaled scores) and sum
 };
 
 __host__ __device__ inline int head_groups(int heads) { return (heads + 63) / 64; }
@@ -386,7 +386,15 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
         const float f = grown ? __builtin_amdgcn_exp2f((m - top) * scale) : 1.0f;
         m = grown ? top : m;
         l *= f;
-        const float base = (m == -__builtin_huge_valf() ? 0.0f : m * scale) - kProbShift<DT>;
+        float base = m == -__builtin_huge_valf() ? 0.0f : m * scale;
+        const bool far = __builtin_fabsf(base) > kFarExponent;
+        if (__any(far)) {
+          const float off = far ? m : 0.0f;
+          base = far ? 0.0f : base;
+#pragma unroll
+          for (int b = 0; b < 2; b++) s[b] -= off;
+        }
+        base -= kProbShift<DT>;
         if (g == 0) fade[k & 1][head_in_group] = f;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -400,7 +408,7 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
         }
       }
       const float sum = sum_over_rows(l);
-      if (g == 0) stats[(k - 1) & 1][head_in_group] = make_float2(m * scale, sum);
+      if (g == 0) stats[(k - 1) & 1][head_in_group] = make_float2(m, sum);
     } while (at.step());
     __syncthreads();
     return;
@@ -624,10 +632,10 @@ __global__ __launch_bounds__(1024, 8) void k_mla_finish(DecodeArgs d) {
         float m = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), l = 0.0f;
 #pragma unroll
         for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
-        const float base = m == -__builtin_huge_valf() ? 0.0f : m;
+        const float base = m == -__builtin_huge_valf() ? 0.0f : m, scale = exponent_scale(a.scale);
 #pragma unroll
         for (int k = 0; k < kShares / 64; k++) {
-          st[k].x = __builtin_amdgcn_exp2f(st[k].x - base);
+          st[k].x = __builtin_amdgcn_exp2f((st[k].x - base) * scale);
           l += st[k].x * st[k].y;
         }
         l = wave_sum(l);

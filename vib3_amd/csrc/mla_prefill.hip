@@ -263,7 +263,17 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
 #pragma unroll
       for (int c = 0; c < VB; c++) o[c] *= f;
     }
-    const float base = (m == -__builtin_huge_valf() ? 0.0f : m * scale) - kProbShift<DT>;
+    float base = m == -__builtin_huge_valf() ? 0.0f : m * scale;
+    const bool far = __builtin_fabsf(base) > kFarExponent;
+    if (__any(far)) {
+      const float off = far ? m : 0.0f;
+      base = far ? 0.0f : base;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[b][i] -= off;
+    }
+    base -= kProbShift<DT>;
     uint32_t p[16];
 #pragma unroll
     for (int b = 0; b < 2; b++)
