@@ -1,5 +1,5 @@
-"""GPU tests of latent attention (vib3_amd.mla) at the ends of the values' range: long tails behind one key, scales far
-above 1. Results are compared with the definition in 64 bits.
+"""GPU tests of latent attention (vib3_amd.mla) at the ends of the values' range: long tails behind one key, scales far above
+1, infinities that are seen. Results are compared with the definition in 64 bits.
 
 Where all of a row's probabilities are of one size, they are rounded alike, and the errors do not average out: the tolerances
 here count a whole half step u of sum_j p_j |y_j| for them, u |result| for the result's own rounding, and 2^-16 sum_j p_j |y_j| for the
@@ -196,3 +196,26 @@ def test_prefill_large_scales(dtype, scale, heads):
         s = q[:, h, :128].double() @ kv[:, h, :128].double().t() + q[:, h, 128:].double() @ kr.double().t()
         want, size = best((s if scale > 0 else -s).masked_fill(~seen, -math.inf), kv[:, h, 128:].double())
         close(got[:, h], want, R.half_step(dtype) * want.abs() + 2.0 ** -16 * size, f"head {h}")
+
+
+# ------------------------------------------------------------------------------- infinities that are seen
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,at", [(8, 40), (64, 700), (128, 3)])
+def test_decode_infinite_latent_that_is_seen(dtype, heads, at):
+    """Latent form: a seen token whose latent is -infinity in one column scores -infinity. That column is 0 * infinity, and all
+    others are what the other tokens make them."""
+    n, column = 900, 77
+    rows = normal(n, 576, dtype=dtype, seed=10)
+    rows[at, column] = -math.inf
+    q = normal(2, heads, 576, dtype=dtype, seed=11)
+    q[..., column] = 1.0
+    scale, lens, u = 0.05, [n, at + 1], R.half_step(dtype)
+    got = decode(rows, q, lens, scale)
+    rest = [c for c in range(512) if c != column]
+    for r, m in enumerate(lens):
+        keep = torch.tensor([j for j in range(m) if j != at], device="cuda")
+        want, tol = R.decode_row(q[r, :, :512], q[r, :, 512:], None, 128, rows[keep, :512], rows[keep, 512:], scale, u)
+        close(got[r][:, rest], want[:, rest], tol[:, rest], f"row {r}")
+        assert bool(got[r][:, column].isnan().all())

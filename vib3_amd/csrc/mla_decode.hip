@@ -15,6 +15,8 @@
 // cut into kShares equal runs, one workgroup each, whatever the rows' lengths: a long row is shared by many workgroups, a run
 // covers many short rows (without the fixed time 41 rows of 1 to 4100 tokens took 28 us, with it 19). Nothing on the host
 // depends on the lengths, so a captured launch follows them.
+#include <type_traits>
+
 #include "mla.h"
 
 namespace vib3 {
@@ -329,9 +331,10 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
     }
     const int g = lane >> 4, col = lane & 15, head_in_group = wave * 16 + col;
     const float scale = exponent_scale(a.scale), sign = a.scale < 0.0f ? -1.0f : 1.0f;
-    // queries: the B operand, this lane's head at k = 32 s + 8 g; the latent part in two summands
+    // queries: the B operand, this lane's head at k = 32 s + 8 g; the latent part in two summands where
+    // it was formed by W_uk
     constexpr int KS = (R + P) / 32;
-    s16x8 q[KS], q_low[R / 32] = {};
+    s16x8 q[KS], q_low[R / 32];
     auto load_q = [&](int x) {
       const int r = x / groups;
       const int64_t h = min((x - r * groups) * 64 + head_in_group, a.heads - 1);
@@ -356,14 +359,19 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
         const lds_u8* t = (lds_u8*)lat[k % kRing] + col * R * 2;
         const lds_u8* u = (lds_u8*)rot[k % kRing] + col * 128;
         f32x4 s[2] = {};
+        auto latent_scores = [&](auto summands) {  // chunk (4 c + g) ^ row_swizzle(col), a constant and two bits away from that of c = 0
 #pragma unroll
-        for (int c = 0; c < R / 32; c++)  // chunk (4 c + g) ^ row_swizzle(col), a constant and two bits away from that of c = 0
+          for (int c = 0; c < R / 32; c++)
 #pragma unroll
-          for (int b = 0; b < 2; b++) {
-            const s16x8 key = lds_read16(t + b * 32 * R + (k0 ^ c % 4 * 64) + c / 4 * 256);
-            s[b] = mma32<DT>(key, q[c], s[b]);
-            s[b] = mma32<DT>(key, q_low[c], s[b]);
-          }
+            for (int b = 0; b < 2; b++) {
+              const s16x8 key = lds_read16(t + b * 32 * R + (k0 ^ c % 4 * 64) + c / 4 * 256);
+              s[b] = mma32<DT>(key, q[c], s[b]);
+              if (decltype(summands)::value == 2) s[b] = mma32<DT>(key, q_low[c], s[b]);
+            }
+        };
+        // (queries that are latent already have no second summand, and its zeros would make NaN of an infinite latent)
+        if (a.kv_b) latent_scores(std::integral_constant<int, 2>{});
+        else latent_scores(std::integral_constant<int, 1>{});
 #pragma unroll
         for (int c = 0; c < P / 32; c++)
 #pragma unroll
