@@ -219,3 +219,48 @@ def test_decode_infinite_latent_that_is_seen(dtype, heads, at):
         want, tol = R.decode_row(q[r, :, :512], q[r, :, 512:], None, 128, rows[keep, :512], rows[keep, 512:], scale, u)
         close(got[r][:, rest], want[:, rest], tol[:, rest], f"row {r}")
         assert bool(got[r][:, column].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads", [2, 64])
+@pytest.mark.parametrize("at,scale", [(10, 0.07), (70, 0.07), (127, -0.07), (300, 0.07), (900, -0.07), (1299, 0.07)])
+def test_prefill_infinite_value_with_probability_zero(dtype, heads, at, scale):
+    """A seen key that scores -infinity beside a value of infinity in one column is 0 * infinity there, in tiles that some queries
+    do not see all of as in others; the queries before it, and the other columns, are as without that token."""
+    n, column = 1300, 37
+    q, kv, kr = (normal(*s, dtype=dtype, seed=12 + i) for i, s in enumerate([(n, heads, 192), (n, heads, 256), (n, 64)]))
+    q[..., 128] = 1.0
+    kr[at, 0] = math.copysign(math.inf, -scale)
+    kv[at, :, 128 + column] = math.inf
+    got = prefill(q, kv, kr, 128, scale)
+    clean, sane = kv.clone(), kr.clone()
+    sane[at] = 0.0
+    clean[at] = 0.0
+    seen = torch.arange(n, device="cuda") <= torch.arange(n, device="cuda")[:, None]
+    seen[:, at] = False
+    rest = [c for c in range(128) if c != column]
+    u = R.half_step(dtype)
+    for h in range(0, heads, max(1, heads // 2)):
+        x, v = q[:, h].double(), clean[:, h, 128:].double()
+        k = torch.cat([clean[:, h, :128], sane], -1).double()
+        s = (scale * (x @ k.t())).masked_fill(~seen, -math.inf)
+        p = R.softmax(s)
+        want = p @ v
+        f32 = R.f32_part(torch.where(seen, abs(scale) * (x.abs() @ k.abs().t()), torch.zeros_like(s)))
+        tol = u * want.abs() + 6 * u / math.sqrt(3) * (p.square() @ v.square()).sqrt() + f32 * (p @ v.abs()) + R.tiny(u)
+        close(got[:, h][:, rest], want[:, rest], tol[:, rest], f"head {h}")
+        close(got[:at, h, column], want[:at, column], tol[:at, column], f"head {h}, before the token")
+        assert bool(got[at:, h, column].isnan().all()), f"head {h}, from the token on"
+
+
+@pytest.mark.parametrize("heads", [2, 64])
+def test_prefill_infinite_value_that_counts(heads):
+    """With ordinary scores: the column is infinite for the queries that see the value."""
+    n, column = 900, 100
+    q, kv, kr = (normal(*s, dtype=BF16, seed=20 + i) for i, s in enumerate([(n, heads, 192), (n, heads, 256), (n, 64)]))
+    for at, value in ((130, math.inf), (650, -math.inf)):
+        x = kv.clone()
+        x[at, :, 128 + column] = value
+        got = prefill(q, x, kr, 128, 0.01)
+        assert bool((got[at:, :, column] == value).all())
+        assert bool(got[:at].isfinite().all()) and bool(got[..., :column].isfinite().all())

@@ -299,18 +299,38 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
       int odd = 0;
 #pragma unroll
       for (int w = 0; w < WAVES; w++) odd |= odd_values[n & 1][w];
-      if (__builtin_amdgcn_readfirstlane(odd)) {  // what was cleared, for the queries that do see it
+      if (__builtin_amdgcn_readfirstlane(odd)) {
+        // What was cleared, for the queries that do see it: infinities times a probability of 0 are NaN, as in other tiles.
+        // (Whether it is 0 is formed again from memory, so that the ordinary path holds nothing for this one.)
         const int keys = min(kKeys, bl.nk - n * kKeys);
+        const int64_t t = bl.q0 + min(qi, bl.nq - 1);
+        const uint16_t* qn = (const uint16_t*)a.q_nope + t * a.q_nope_token_stride + (int64_t)h * a.q_nope_head_stride;
+        const uint16_t* qr = (const uint16_t*)a.q_rope + t * a.q_rope_token_stride + (int64_t)h * a.q_rope_head_stride;
+        const float off = m == -__builtin_huge_valf() ? 0.0f : m;
 #pragma unroll 1
         for (int j = 0; j < keys; j++) {
-          const uint16_t* x = kv + (int64_t)(n * kKeys + j) * a.kv_token_stride + N + 4 * half;
+          const uint16_t* row = kv + (int64_t)(n * kKeys + j) * a.kv_token_stride;
+          const uint16_t* rot = kr + (int64_t)(n * kKeys + j) * a.k_rope_stride;
+          float score = 0.0f;
+#pragma unroll 1
+          for (int c = half; c < NC + PC; c += 2) {  // the other chunks are the pair's other lane's
+            float x[8], y[8];
+            unpack8<DT>(*(const uint4*)(c < NC ? qn + 8 * c : qr + 8 * (c - NC)), x);
+            unpack8<DT>(*(const uint4*)(c < NC ? row + 8 * c : rot + 8 * (c - NC)), y);
+#pragma unroll
+            for (int i = 0; i < 8; i++) score = __builtin_fmaf(x[i], y[i], score);
+          }
+          score = a.scale < 0.0f ? -pair_sum(score) : pair_sum(score);
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score - off, scale, kProbShift<DT>));
           if (n * kKeys + j > limit) continue;
+          const bool some = pack2<DT>(e, e) != 0;
+          const uint16_t* x = row + N + 4 * half;
 #pragma unroll
           for (int c = 0; c < VB; c++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
               const uint16_t y = x[32 * c + 8 * (i >> 2) + (i & 3)];
-              if (finite_only<DT>(y) != y) o[c][i] += to_f32<DT>(y);
+              if (finite_only<DT>(y) != y) o[c][i] += some ? to_f32<DT>(y) : __builtin_nanf("");
             }
         }
       }
