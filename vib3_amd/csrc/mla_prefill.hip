@@ -362,13 +362,21 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_mla_prefill(vib3_mla_
 
 template <int DT, int N, int P, int V>
 int launch_prefill(const vib3_mla_prefill& a, hipStream_t st) {
-  // Sequences' blocks number at most this many; surplus workgroups end at once. 256 queries a workgroup where those fill the
-  // card's 256 CUs (a tile then serves twice the queries: 48 against 53 us at 1000 tokens of 64 heads, 761 against 1060 us at
-  // 6000), 128 where twice the CUs count for more (25 against 28 us at 500, 13 against 15 us at 173).
-  const int64_t wide = (a.q_tokens / 256 + a.num_seqs) * (int64_t)a.heads;
-  const int64_t narrow = (a.q_tokens / 128 + a.num_seqs) * (int64_t)a.heads;
+  // Sequences' blocks number at most this many (each ends in one that is not full); surplus workgroups end at once. Measured with
+  // 128 + 64 + 128 in bf16, us with 256 queries a workgroup / with 128 (one workgroup a CU in both forms):
+  //   one prompt, by the count `wide`   128: 27 / 24 (500 tokens of 64 heads), 19 / 17 (256 of 128); 192: 33 / 34 (700 of 64), 108 / 100
+  //                                     (3000 of 16); 240: 62 / 66 (1500 of 40); 256: 46 / 51 (1000 of 64); 512: 104 / 151 (2048 of 64)
+  //   few queries over many keys        701 / 778 (32 of 1 query over 3000 keys, 64 heads), 118 / 130 (4 over 4000): twice the waves
+  //                                     load the tiles
+  //   one long prompt among others      131 / 121 (4096 tokens and 31 single queries, 8 heads): the host does not know the lengths,
+  //                                     and takes the blocks that there may be
+  // With 64 + 32 + 64 the forms are within 4 % of one another for one prompt to 2000 tokens, and 256 queries better by up to 10 %
+  // (16 for 8 or 16 heads of 6000) beyond; many short sequences would be better off with 128 (502 / 331 for the 32 over 3000, 38 / 27
+  // for 20 prompts of 100), of which two workgroups fit in a CU, four over 4000 keys not (85 / 105).
+  const int64_t wide = (a.q_tokens + 255 * (int64_t)a.num_seqs) / 256 * a.heads;
+  const int64_t narrow = (a.q_tokens + 127 * (int64_t)a.num_seqs) / 128 * a.heads;
   if (narrow > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
-  if (wide >= 256)
+  if (wide >= 224)  // of 256 CUs
     hipLaunchKernelGGL((k_mla_prefill<DT, N, P, V, 8>), dim3((unsigned)wide), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((k_mla_prefill<DT, N, P, V, 4>), dim3((unsigned)narrow), dim3(256), 0, st, a);
