@@ -486,7 +486,11 @@ int vib3_launch_moe_mxfp4_batched(const vib3_moe_mxfp4_batch *batch, void *strea
  * Index tensors are int32 on the device and read while the kernels run: an index that is out of
  * its range is never followed (each launcher says what happens instead). Launches are safe inside
  * HIP graph capture and keep no state between calls. scale may be any finite number
- * (VIB3_ERR_UNSUPPORTED otherwise); a row whose scores are all -infinity gives zeros.
+ * (VIB3_ERR_UNSUPPORTED otherwise); a row whose scores are all -infinity gives zeros. What a row
+ * does not see leaves it as it is, infinities and NaN included; where it sees some, it is what the
+ * formula gives in f32 (0 times infinity is NaN). Probabilities go to the matrix cores in the 16-bit
+ * type: in f16 with all of its bits down to 2^-25 of the row's largest, and off by at most 2^-36 of
+ * that below.
  * ---------------------------------------------------------------------------------------- */
 typedef struct vib3_mla_cache {
     void *pool;                 /* [num_pages][page_size][rank + rope] */

@@ -8,7 +8,7 @@
 //   k_mla_attend   the attention in the latent space, over equal shares of all rows' cached tokens
 //   k_mla_finish   rows that several workgroups shared are joined, and W_uv applied
 // At 64 heads of 128 x 512, bf16, the launches' own times: one row of 777 tokens 5 + 14 + 8 us; one of 131072 5 + 45 + 16;
-// 96 rows of 2048 to 12288 (654 MB) 12 + 141 to 157 + 20.
+// 96 rows of 2048 to 12288 (654 MB) 12 + 140 to 159 + 20.
 //
 // The plan: tokens are taken 32 at a time (a unit), heads in groups of up to 64. All units of all items
 // (row, head group) in order, with kItemCost units' time in front of each item for taking it up and storing its sums, are
@@ -236,7 +236,7 @@ __device__ const uint4 zero_row[(512 + 64) / 8] = {};
 //              transposing reads), and load unit k + 2.
 // With one barrier a unit, and each SIMD with vector work of one wave next to products of the other, 96 rows of 64 heads
 // took 133 us; all eight waves going through the same phases, with three barriers, 163. The latent queries' second summand
-// (below) made it 141 to 157: 4.1 to 4.5 TB/s, of the 6.0 that reading alone reaches. Bound by both: a unit's rows come at that rate
+// (below) made it 140 to 159: 4.0 to 4.5 TB/s, of the 6.0 that reading alone reaches. Bound by both: a unit's rows come at that rate
 // in 1.6 us, and its reads from LDS (each row once per 16 heads for the scores, and once for the sums) fill some 1400 cycles of
 // the 2 us that it takes, the products 1100.
 //
@@ -410,7 +410,8 @@ __global__ __launch_bounds__(512, 2) void k_mla_attend(DecodeArgs d) {
 #pragma unroll
           for (int j = 0; j < 4; j++) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
           l += (e[0] + e[1]) + (e[2] + e[3]);
-          // rounded for the matrix cores; the sum l takes them unrounded
+          // Rounded for the matrix cores; the sum l takes them unrounded. (A remainder as a second summand takes 8 KB more, of
+          // which the ring leaves 5. Without it the result is off by 0.0017 to 0.0021 in bf16, a single rounding by 0.0017.)
           lds_write8((lds_u8*)prob[k & 1] + head_in_group * (kUnit * 2) + ((2 * b + (g >> 1)) ^ (col >> 2)) * 16 + 8 * (g & 1),
                      pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
         }
