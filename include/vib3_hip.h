@@ -599,6 +599,180 @@ typedef struct vib3_mla_prefill {
 int vib3_launch_mla_prefill(const vib3_mla_prefill *args, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Grouped-query attention (GQA), the same sublayer for models with a key and a value per group of
+ * heads (additive launchers): head h reads the key/value head h / (heads / kv_heads). The cache is
+ * two pools of pages, keys and values, of page_size tokens; a sequence's token j is token
+ * j % page_size of page block_table[seq][j / page_size] in both.
+ *
+ * For all three launchers: dtype is VIB3_DT_F16 or VIB3_DT_BF16, dim 64, 128 or 256, heads a
+ * multiple of kv_heads; strides are in elements and multiples of 8, tensor addresses are 16-byte
+ * aligned (VIB3_ERR_BAD_POINTER otherwise), and the innermost dimension of every tensor is
+ * contiguous. Index tensors are int32 on the device and read while the kernels run: an index that
+ * is out of its range is never followed (each launcher says what happens instead). Launches are
+ * safe inside HIP graph capture and keep no state between calls.
+ *
+ * What a query at position p sees: the tokens j <= p and, with window > 0, of those only the newest
+ * window (j > p - window) and the first sinks (j < sinks); tokens on pages that are not resident
+ * are not seen. scale may be any finite number (VIB3_ERR_UNSUPPORTED otherwise). A query that sees
+ * no token, or whose scores are all -infinity, gives zeros. What it does not see leaves it as it
+ * is, infinities and NaN included; where it sees some, it is what the formula gives in f32 (0
+ * times infinity is NaN). Statistics and sums are f32; probabilities go to the matrix cores in the
+ * 16-bit type, in f16 with all of its bits down to 2^-25 of the row's largest, and off by at most
+ * 2^-36 of that below.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct vib3_gqa_cache {
+    void *keys, *values;        /* [num_pages][page_size][kv_heads][dim] each */
+    int dtype;
+    int num_pages, page_size;   /* page_size 1..65536 */
+    int kv_heads, dim;
+    int64_t page_stride, token_stride, head_stride; /* of both pools; any order of the dimensions */
+    const int32_t *block_table; /* [num_seqs][max_pages] page numbers, contiguous; an entry
+                                   outside [0, num_pages) is a page that is not resident */
+    int num_seqs, max_pages;
+} vib3_gqa_cache;
+
+/* New tokens into the cache. Token t is token positions[t] of sequence seqs[t]:
+ *   key   = rot(k[t][g] * k_norm / sqrt(mean(k[t][g]^2) + norm_eps), positions[t])
+ *   value = v[t][g]
+ * and, if q is given, q_out[t][h] = the same of q[t][h] with q_norm (q_out may be q itself, where their
+ * types are one). A norm that is NULL leaves its rows as they are. rot(x, p) turns the pair i of
+ * the first rot elements (2i and 2i + 1 if interleaved, else i and i + rot / 2) by the angle
+ * p * inv_freq[i] (64-bit) and multiplies by rope_scale; the rest of the head stays. rot is a
+ * multiple of 16 up to dim, or 0. Sums in f32, one rounding at the end.
+ * A token with seqs[t] outside [0, num_seqs) or a negative position is padding: nothing of it is
+ * written. A token whose page is not resident, or lies past max_pages, is not cached; its q_out row
+ * is written. The (sequence, position) pairs of a call must differ (of equal ones the cached
+ * token may be a mixture). */
+typedef struct vib3_gqa_append {
+    vib3_gqa_cache cache;
+    int tokens, heads;                 /* heads is not read without q */
+    const int32_t *seqs, *positions;   /* [tokens] */
+    int src_dtype;                     /* of q, k and v: f32, f16 or bf16 */
+    const void *q;                     /* [tokens][heads][dim], or NULL */
+    int64_t q_token_stride, q_head_stride;
+    const void *k;                     /* [tokens][kv_heads][dim] */
+    int64_t k_token_stride, k_head_stride;
+    const void *v;                     /* [tokens][kv_heads][dim] */
+    int64_t v_token_stride, v_head_stride;
+    const void *q_norm, *k_norm;       /* [dim] in norm_dtype, or NULL */
+    int norm_dtype;                    /* f32, f16 or bf16 */
+    float norm_eps;
+    const float *inv_freq;             /* [rot / 2] */
+    int rot;
+    float rope_scale;
+    int interleaved;
+    void *q_out;                       /* [tokens][heads][dim] in the cache's dtype */
+    int64_t q_out_token_stride, q_out_head_stride;
+} vib3_gqa_append;
+
+int vib3_launch_gqa_append(const vib3_gqa_append *args, void *stream);
+
+/* Attention of single query tokens: row r is the newest of the first lens[r] cached tokens of
+ * sequence seqs[r] (position lens[r] - 1; several tokens of a sequence are several rows):
+ *   out[r][h] = sum_j softmax_j(scale * q[r][h] . key_j) value_j   over what it sees.
+ * A row with lens[r] <= 0 or a sequence outside [0, num_seqs) is zero; lens[r] beyond the block
+ * table counts as its capacity. */
+typedef struct vib3_gqa_decode {
+    vib3_gqa_cache cache;
+    int rows, heads;                   /* rows <= 65536, heads <= 1024 */
+    const int32_t *seqs;               /* [rows], or NULL: row r reads sequence r */
+    const int32_t *lens;               /* [rows] */
+    const void *q;                     /* [rows][heads][dim] */
+    int64_t q_row_stride, q_head_stride;
+    float scale;
+    int window, sinks;                 /* window 0: none */
+    void *out;                         /* [rows][heads][dim] */
+    int64_t out_row_stride, out_head_stride;
+    void *workspace;                   /* vib3_gqa_decode_workspace_bytes() bytes, 256-byte
+                                          aligned; calls that may overlap need one each */
+    size_t workspace_bytes;
+} vib3_gqa_decode;
+
+size_t vib3_gqa_decode_workspace_bytes(const vib3_gqa_decode *args);
+int vib3_launch_gqa_decode(const vib3_gqa_decode *args, void *stream);
+
+/* Attention of the newest tokens of each sequence (a prompt, its next chunk, drafted tokens) over
+ * the cache, which holds them already. Sequence s (a row of the block table) has the queries
+ * [cu_q[s], cu_q[s+1]) and the first lens[s] cached tokens; with nq of them, query i has the position
+ * lens[s] - nq + i (a negative one sees nothing). The sum is vib3_launch_gqa_decode's. Queries behind
+ * cu_q[num_seqs] are left as they were; offsets are cut to [0, q_tokens], lens[s] to the block
+ * table's capacity. */
+typedef struct vib3_gqa_chunk {
+    vib3_gqa_cache cache;
+    int heads, q_tokens;               /* heads <= 1024 */
+    const int32_t *cu_q;               /* [num_seqs + 1] */
+    const int32_t *lens;               /* [num_seqs] */
+    const void *q;                     /* [q_tokens][heads][dim] */
+    int64_t q_token_stride, q_head_stride;
+    float scale;
+    int window, sinks;                 /* window 0: none */
+    void *out;                         /* [q_tokens][heads][dim] */
+    int64_t out_token_stride, out_head_stride;
+    void *workspace;                   /* vib3_gqa_chunk_workspace_bytes() bytes, 256-byte
+                                          aligned; calls that may overlap need one each */
+    size_t workspace_bytes;
+} vib3_gqa_chunk;
+
+size_t vib3_gqa_chunk_workspace_bytes(const vib3_gqa_chunk *args);
+int vib3_launch_gqa_chunk(const vib3_gqa_chunk *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The pages of a cache (latent or grouped-query) in all of its pools at once (additive launchers).
+ * A pool's page is runs * page_size * token_bytes bytes: token t of run r lies at
+ * base + page * page_stride + r * run_stride + t * token_stride (a run is a head, where a page holds
+ * head after head). All in bytes and multiples of 16, base 16-byte aligned. The array of pools is
+ * read by the call, index tensors (int32 on the device) by the kernels; an index that is out
+ * of its range is never followed. Both launchers are safe inside HIP graph capture.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct vib3_page_pool {
+    void *base;
+    int64_t page_stride, run_stride, token_stride;
+    int runs, token_bytes;
+} vib3_page_pool;
+
+/* Sequences that go on from another's tokens. For each i, with n = lens[parents[i]] (at most the
+ * block table's capacity) and full = n / page_size: row children[i] of the table becomes the first
+ * `full` entries of row parents[i] (pages that both then share), new_pages[i] (where the row has room for it) and -1
+ * from there on; the first n % page_size tokens of the parent's entry `full` are copied to page
+ * new_pages[i] in every pool. Nothing is copied from or to a page that is not resident, and a pair whose
+ * parent or child is outside [0, num_seqs) is left out. lens is not written. Children must differ from one another and
+ * from the parents, and so must new pages from one another and from the pages in use (rows or pages
+ * may be a mixture otherwise). */
+typedef struct vib3_fork_pages {
+    const vib3_page_pool *pools;       /* host array */
+    int num_pools, num_pages, page_size;
+    int32_t *block_table;              /* [num_seqs][max_pages] */
+    int num_seqs, max_pages;
+    const int32_t *lens;               /* [num_seqs] */
+    int count;
+    const int32_t *parents, *children, *new_pages; /* [count] */
+} vib3_fork_pages;
+
+int vib3_launch_fork_pages(const vib3_fork_pages *args, void *stream);
+
+/* The pages in use to the front. In use are the pages (of [0, num_pages)) among each sequence's
+ * first ceil(lens[s] / page_size) entries; live is their number. Those numbered live and more take, in
+ * order, the places below live that are not in use: their bytes are copied there in every pool, and
+ * out_table receives the block table with the new numbers and -1 in entries that are not in use (entries that are no page stay).
+ * out_table may be block_table. Pages from *live on are free afterwards; other pages than the moved
+ * ones' new places keep their bytes. */
+typedef struct vib3_compact_pages {
+    const vib3_page_pool *pools;       /* host array */
+    int num_pools, num_pages, page_size; /* num_pages <= 2^20 */
+    const int32_t *block_table;        /* [num_seqs][max_pages] */
+    int num_seqs, max_pages;
+    const int32_t *lens;               /* [num_seqs] */
+    int32_t *out_table;                /* [num_seqs][max_pages] */
+    int32_t *live;                     /* [1] */
+    void *workspace;                   /* vib3_compact_pages_workspace_bytes() bytes, 256-byte
+                                          aligned; calls that may overlap need one each */
+    size_t workspace_bytes;
+} vib3_compact_pages;
+
+size_t vib3_compact_pages_workspace_bytes(const vib3_compact_pages *args);
+int vib3_launch_compact_pages(const vib3_compact_pages *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * The .vib3 model file (host side; format.rs). The file is memory-mapped read-only; page data
  * is returned as host pointers into the mapping, for the caller to upload where its page pool
  * lives. vib3_build_page_table then writes the fused layer's page table from the catalog.

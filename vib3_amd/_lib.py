@@ -127,6 +127,88 @@ class MlaPrefillDesc(C.Structure):
     ]
 
 
+class GqaCacheDesc(C.Structure):
+    """vib3_gqa_cache (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("keys", C.c_void_p), ("values", C.c_void_p), ("dtype", C.c_int), ("num_pages", C.c_int),
+        ("page_size", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int),
+        ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("block_table", C.c_void_p), ("num_seqs", C.c_int), ("max_pages", C.c_int),
+    ]
+
+
+class GqaAppendDesc(C.Structure):
+    """vib3_gqa_append (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("cache", GqaCacheDesc), ("tokens", C.c_int), ("heads", C.c_int), ("seqs", C.c_void_p),
+        ("positions", C.c_void_p), ("src_dtype", C.c_int),
+        ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("k", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v", C.c_void_p), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("norm_dtype", C.c_int),
+        ("norm_eps", C.c_float), ("inv_freq", C.c_void_p), ("rot", C.c_int),
+        ("rope_scale", C.c_float), ("interleaved", C.c_int),
+        ("q_out", C.c_void_p), ("q_out_token_stride", C.c_int64), ("q_out_head_stride", C.c_int64),
+    ]
+
+
+class GqaDecodeDesc(C.Structure):
+    """vib3_gqa_decode (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("cache", GqaCacheDesc), ("rows", C.c_int), ("heads", C.c_int), ("seqs", C.c_void_p),
+        ("lens", C.c_void_p), ("q", C.c_void_p), ("q_row_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int),
+        ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class GqaChunkDesc(C.Structure):
+    """vib3_gqa_chunk (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("cache", GqaCacheDesc), ("heads", C.c_int), ("q_tokens", C.c_int), ("cu_q", C.c_void_p),
+        ("lens", C.c_void_p), ("q", C.c_void_p), ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int),
+        ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class PagePoolDesc(C.Structure):
+    """vib3_page_pool (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("base", C.c_void_p), ("page_stride", C.c_int64), ("run_stride", C.c_int64),
+        ("token_stride", C.c_int64), ("runs", C.c_int), ("token_bytes", C.c_int),
+    ]
+
+
+class ForkPagesDesc(C.Structure):
+    """vib3_fork_pages (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("pools", C.POINTER(PagePoolDesc)), ("num_pools", C.c_int), ("num_pages", C.c_int),
+        ("page_size", C.c_int), ("block_table", C.c_void_p), ("num_seqs", C.c_int),
+        ("max_pages", C.c_int), ("lens", C.c_void_p), ("count", C.c_int), ("parents", C.c_void_p),
+        ("children", C.c_void_p), ("new_pages", C.c_void_p),
+    ]
+
+
+class CompactPagesDesc(C.Structure):
+    """vib3_compact_pages (include/vib3_hip.h)."""
+
+    _fields_ = [
+        ("pools", C.POINTER(PagePoolDesc)), ("num_pools", C.c_int), ("num_pages", C.c_int),
+        ("page_size", C.c_int), ("block_table", C.c_void_p), ("num_seqs", C.c_int),
+        ("max_pages", C.c_int), ("lens", C.c_void_p), ("out_table", C.c_void_p),
+        ("live", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/vib3_hip.h
 P, I, F, S, U64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
 SIGNATURES = {
@@ -161,6 +243,14 @@ SIGNATURES = {
     "vib3_mla_decode_workspace_bytes": (S, [C.POINTER(MlaDecodeDesc)]),
     "vib3_launch_mla_decode": (I, [C.POINTER(MlaDecodeDesc), P]),
     "vib3_launch_mla_prefill": (I, [C.POINTER(MlaPrefillDesc), P]),
+    "vib3_launch_gqa_append": (I, [C.POINTER(GqaAppendDesc), P]),
+    "vib3_gqa_decode_workspace_bytes": (S, [C.POINTER(GqaDecodeDesc)]),
+    "vib3_launch_gqa_decode": (I, [C.POINTER(GqaDecodeDesc), P]),
+    "vib3_gqa_chunk_workspace_bytes": (S, [C.POINTER(GqaChunkDesc)]),
+    "vib3_launch_gqa_chunk": (I, [C.POINTER(GqaChunkDesc), P]),
+    "vib3_launch_fork_pages": (I, [C.POINTER(ForkPagesDesc), P]),
+    "vib3_compact_pages_workspace_bytes": (S, [C.POINTER(CompactPagesDesc)]),
+    "vib3_launch_compact_pages": (I, [C.POINTER(CompactPagesDesc), P]),
     "vib3_hip_zero": (I, [P, S, P]),
     "vib3_synth_bytes": (I, [P, S, U64, U64, S, P]),
     "vib3_synth_normal": (I, [P, I, S, U64, U64, S, F, P]),

@@ -1,0 +1,273 @@
+// cache_pages.hip — a cache's pages forked and compacted, in all of its pools at once.
+//
+// Bound by the bytes copied, read once and written once. A copied page is cut into pieces of 16 KB, a workgroup each; pools go with the
+// launch's arguments, kPools at a time.
+#include "kernels.h"
+
+namespace vib3 {
+
+constexpr int kPools = 64;
+constexpr int kPiece = 1024;  // 16-byte chunks of a piece
+constexpr int kMaxCompact = 1 << 20;
+
+struct Pools {
+  vib3_page_pool pool[kPools];
+};
+
+__host__ __device__ inline int64_t page_chunks(const vib3_page_pool& p, int page_size) {
+  return (int64_t)p.runs * page_size * (p.token_bytes / 16);
+}
+
+// One piece of a page, of its first `tokens` tokens, to another page (256 threads).
+__device__ void copy_piece(const vib3_page_pool& p, int page_size, int tokens, int from, int to, int piece) {
+  const uint8_t* src = (const uint8_t*)p.base + (int64_t)from * p.page_stride;
+  uint8_t* dst = (uint8_t*)p.base + (int64_t)to * p.page_stride;
+  const uint32_t per = (uint32_t)p.token_bytes / 16, run = per * (uint32_t)page_size, all = run * (uint32_t)p.runs;
+  uint4 v[kPiece / 256];
+  int64_t at[kPiece / 256];
+#pragma unroll
+  for (int i = 0; i < kPiece / 256; i++) {
+    const uint32_t c = (uint32_t)piece * kPiece + i * 256 + threadIdx.x;
+    const uint32_t r = c / run, in = c - r * run, t = in / per;
+    at[i] = c < all && t < (uint32_t)tokens ? (int64_t)r * p.run_stride + (int64_t)t * p.token_stride + (int64_t)(in - t * per) * 16 : -1;
+    if (at[i] >= 0) v[i] = *(const uint4*)(src + at[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kPiece / 256; i++)
+    if (at[i] >= 0) *(uint4*)(dst + at[i]) = v[i];
+}
+
+// ------------------------------------------------------------------------- fork
+
+// Workgroups 0..count - 1 write the children's rows of the table (in the first launch of a call), the others copy.
+__global__ __launch_bounds__(256) void k_fork_pages(vib3_fork_pages a, Pools pools, int num_pools, int pieces, int table_blocks) {
+  const int b = (int)blockIdx.x - table_blocks;
+  const int i = b < 0 ? (int)blockIdx.x : b / pieces % a.count;
+  const int p = a.parents[i], c = a.children[i], fresh = a.new_pages[i];
+  if ((unsigned)p >= (unsigned)a.num_seqs || (unsigned)c >= (unsigned)a.num_seqs) return;
+  const int64_t cap = min((int64_t)a.max_pages * a.page_size, (int64_t)0x7fffffff);
+  const int n = a.lens[p], len = n <= 0 ? 0 : n > cap ? (int)cap : n;
+  const int full = len / a.page_size, rest = len - full * a.page_size;
+  const int32_t* parent = a.block_table + (size_t)p * a.max_pages;
+  if (b < 0) {
+    int32_t* child = a.block_table + (size_t)c * a.max_pages;
+    for (int k = (int)threadIdx.x; k < a.max_pages; k += 256) child[k] = k < full ? parent[k] : k == full ? fresh : -1;
+    return;
+  }
+  if (rest == 0) return;
+  const int from = parent[full];
+  if ((unsigned)from >= (unsigned)a.num_pages || (unsigned)fresh >= (unsigned)a.num_pages) return;
+  copy_piece(pools.pool[b / pieces / a.count], a.page_size, rest, from, fresh, b % pieces);
+}
+
+// ------------------------------------------------------------------------- compaction
+
+// Device workspace: the number of moves, their pages, and the pages' new numbers (of those that move).
+struct CompactWs {
+  int32_t* count;
+  int32_t *from, *to;  // [num_pages / 2]: a move takes a page in use and one that is not
+  int32_t* place;      // [num_pages]
+};
+
+inline size_t compact_ws(int num_pages, CompactWs* w, void* base) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return (int32_t*)((uint8_t*)base + p);
+  };
+  CompactWs r;
+  r.count = take(4);
+  r.from = take(4 * (size_t)(num_pages / 2));
+  r.to = take(4 * (size_t)(num_pages / 2));
+  r.place = take(4 * (size_t)num_pages);
+  if (w) *w = r;
+  return at;
+}
+
+__device__ __forceinline__ int used_entries(const vib3_compact_pages& a, int s) {
+  const int n = a.lens[s];
+  return n <= 0 ? 0 : min((n - 1) / a.page_size + 1, a.max_pages);
+}
+
+// Sum of v over the threads before this one, of 1024 threads; *all: over all of them.
+__device__ int block_scan(int v, int* wave_sums, int* all) {
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int up = __shfl_up(sum, d);
+    if (lane >= d) sum += up;
+  }
+  __syncthreads();
+  if (lane == 63) wave_sums[tid >> 6] = sum;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int i = 0; i < 16; i++) {
+    if (i < tid >> 6) before += wave_sums[i];
+    total += wave_sums[i];
+  }
+  *all = total;
+  return before + sum - v;
+}
+
+// One workgroup: a bit for each page in use, in LDS; the ranks of pages among those in use by a scan over its words.
+__global__ __launch_bounds__(1024) void k_compact_plan(vib3_compact_pages a, CompactWs w) {
+  __shared__ uint32_t bits[kMaxCompact / 32];
+  __shared__ int sums[16];
+  __shared__ int below;
+  const int tid = (int)threadIdx.x;
+  const int words = (a.num_pages + 31) / 32, per = (words + 1023) / 1024;
+  for (int k = tid; k < words; k += 1024) bits[k] = 0;
+  __syncthreads();
+  for (int s = tid >> 6; s < a.num_seqs; s += 16) {
+    const int n = used_entries(a, s);
+    const int32_t* row = a.block_table + (size_t)s * a.max_pages;
+    for (int k = tid & 63; k < n; k += 64) {
+      const int id = row[k];
+      if ((unsigned)id < (unsigned)a.num_pages) atomicOr(&bits[id / 32], 1u << (id % 32));
+    }
+  }
+  __syncthreads();
+  // a thread's words, in order
+  const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
+  int mine = 0, live;
+  for (int k = w0; k < w1; k++) mine += __popc(bits[k]);
+  const int before = block_scan(mine, sums, &live);
+  // pages in use below `live`: the first of those from there on moves to the first place that is not in use
+  {
+    int n = before;
+    for (int k = w0; k < w1; k++) {
+      if (live >= 32 * k && live < 32 * k + 32) below = n + __popc(bits[k] & ((1u << (live % 32)) - 1));
+      n += __popc(bits[k]);
+    }
+    if (tid == 0 && live >= 32 * words) below = live;  // all pages are in use
+  }
+  __syncthreads();
+  const int kept = below;
+  int n = before;
+  for (int k = w0; k < w1; k++) {
+    const uint32_t word = bits[k];
+    for (int i = 0; i < 32; i++) {
+      const int page = 32 * k + i;
+      const bool used = word >> i & 1;
+      if (used && page >= live) w.from[n - kept] = page;
+      if (!used && page < live) w.to[page - n] = page;
+      n += used;
+    }
+  }
+  __syncthreads();
+  const int moves = live - kept;
+  for (int k = tid; k < moves; k += 1024) w.place[w.from[k]] = w.to[k];
+  if (tid == 0) {
+    *w.count = moves;
+    *a.live = live;
+  }
+}
+
+// Workgroups 0..table_blocks - 1 write the table (in the first launch of a call), the others go through the pieces of all moves.
+__global__ __launch_bounds__(256) void k_compact_move(vib3_compact_pages a, CompactWs w, Pools pools, int num_pools, int pieces,
+                                                      int table_blocks) {
+  const int live = *a.live;
+  if ((int)blockIdx.x < table_blocks) {
+    for (int s = (int)blockIdx.x; s < a.num_seqs; s += table_blocks) {
+      const int n = used_entries(a, s);
+      const size_t row = (size_t)s * a.max_pages;
+      for (int k = (int)threadIdx.x; k < a.max_pages; k += 256) {
+        int id = -1;
+        if (k < n) {
+          id = a.block_table[row + k];
+          if (id >= live && id < a.num_pages) id = w.place[id];
+        }
+        a.out_table[row + k] = id;
+      }
+    }
+    return;
+  }
+  const int64_t all = (int64_t)*w.count * num_pools * pieces;
+  for (int64_t b = (int)blockIdx.x - table_blocks; b < all; b += gridDim.x - table_blocks) {
+    const int move = (int)(b / ((int64_t)num_pools * pieces)), rest = (int)(b - (int64_t)move * num_pools * pieces);
+    copy_piece(pools.pool[rest / pieces], a.page_size, a.page_size, w.from[move], w.to[move], rest % pieces);
+  }
+}
+
+// The most pieces of a page in pools [first, first + n), and these as arguments.
+int gather_pools(const vib3_page_pool* pools, int n, int page_size, Pools* out) {
+  int64_t most = 1;
+  for (int i = 0; i < n; i++) {
+    out->pool[i] = pools[i];
+    const int64_t c = page_chunks(pools[i], page_size);
+    most = c > most ? c : most;
+  }
+  return (int)((most + kPiece - 1) / kPiece);
+}
+
+int check_pools(const vib3_page_pool* pools, int num_pools, int num_pages, int page_size, int num_seqs, int max_pages) {
+  if (num_pools < 0 || num_pages < 0 || page_size < 1 || page_size > 65536 || num_seqs < 0 || max_pages < 0) return VIB3_ERR_BAD_COUNT;
+  if (num_pools && !pools) return VIB3_ERR_BAD_POINTER;
+  for (int i = 0; i < num_pools; i++) {
+    const vib3_page_pool& p = pools[i];
+    if (p.runs < 1 || p.token_bytes < 16 || p.page_stride < 0 || p.run_stride < 0 || p.token_stride < 0) return VIB3_ERR_BAD_COUNT;
+    if ((num_pages && !p.base) || ((uintptr_t)p.base & 15) || p.token_bytes % 16 || p.page_stride % 16 || p.run_stride % 16 ||
+        p.token_stride % 16)
+      return VIB3_ERR_BAD_POINTER;
+    if (page_chunks(p, page_size) > 0x7fffffff - kPiece) return VIB3_ERR_BAD_COUNT;
+  }
+  return 0;
+}
+
+}  // namespace vib3
+
+using namespace vib3;
+
+extern "C" int vib3_launch_fork_pages(const vib3_fork_pages* args, void* stream) {
+  if (!args) return VIB3_ERR_BAD_POINTER;
+  const vib3_fork_pages& a = *args;
+  if (const int rc = check_pools(a.pools, a.num_pools, a.num_pages, a.page_size, a.num_seqs, a.max_pages)) return rc;
+  if (a.count < 0) return VIB3_ERR_BAD_COUNT;
+  if (a.count == 0 || a.num_seqs == 0 || a.max_pages == 0) return 0;
+  if (!a.block_table || !a.lens || !a.parents || !a.children || !a.new_pages) return VIB3_ERR_BAD_POINTER;
+  int first = 0;
+  do {
+    const int n = a.num_pools - first < kPools ? a.num_pools - first : kPools;
+    Pools pools{};
+    const int pieces = gather_pools(a.pools + first, n, a.page_size, &pools);
+    const int table_blocks = first == 0 ? a.count : 0;
+    const int64_t blocks = table_blocks + (int64_t)a.count * n * pieces;
+    if (blocks > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
+    hipLaunchKernelGGL(k_fork_pages, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, pools, n, pieces, table_blocks);
+    first += n;
+  } while (first < a.num_pools);
+  VIB3_RETURN_LAUNCH();
+}
+
+extern "C" size_t vib3_compact_pages_workspace_bytes(const vib3_compact_pages* args) {
+  if (!args || args->num_pages < 0 || args->num_pages > kMaxCompact) return 0;
+  return compact_ws(args->num_pages, nullptr, nullptr);
+}
+
+extern "C" int vib3_launch_compact_pages(const vib3_compact_pages* args, void* stream) {
+  if (!args) return VIB3_ERR_BAD_POINTER;
+  const vib3_compact_pages& a = *args;
+  if (const int rc = check_pools(a.pools, a.num_pools, a.num_pages, a.page_size, a.num_seqs, a.max_pages)) return rc;
+  if (a.num_pages > kMaxCompact) return VIB3_ERR_BAD_COUNT;
+  if (!a.live || !a.workspace || ((uintptr_t)a.workspace & 255)) return VIB3_ERR_BAD_POINTER;
+  if (a.num_seqs && (!a.lens || (a.max_pages && (!a.block_table || !a.out_table)))) return VIB3_ERR_BAD_POINTER;
+  if (a.workspace_bytes < vib3_compact_pages_workspace_bytes(&a)) return VIB3_ERR_WORKSPACE;
+  CompactWs w;
+  compact_ws(a.num_pages, &w, a.workspace);
+  hipLaunchKernelGGL(k_compact_plan, dim3(1), dim3(1024), 0, (hipStream_t)stream, a, w);
+  int first = 0;
+  do {
+    const int n = a.num_pools - first < kPools ? a.num_pools - first : kPools;
+    Pools pools{};
+    const int pieces = gather_pools(a.pools + first, n, a.page_size, &pools);
+    const int table_blocks = first == 0 ? (a.num_seqs < 256 ? a.num_seqs : 256) : 0;
+    const int64_t most = (int64_t)(a.num_pages / 2) * n * pieces;
+    const int64_t blocks = table_blocks + (most < 2048 ? most : 2048);
+    if (blocks)
+      hipLaunchKernelGGL(k_compact_move, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, w, pools, n, pieces, table_blocks);
+    first += n;
+  } while (first < a.num_pools);
+  VIB3_RETURN_LAUNCH();
+}
