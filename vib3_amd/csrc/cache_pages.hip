@@ -5,6 +5,7 @@
 #include "kernels.h"
 
 namespace vib3 {
+namespace {
 
 constexpr int kPools = 64;
 constexpr int kPiece = 1024;  // 16-byte chunks of a piece
@@ -216,6 +217,7 @@ int check_pools(const vib3_page_pool* pools, int num_pools, int num_pages, int p
   return 0;
 }
 
+}  // namespace
 }  // namespace vib3
 
 using namespace vib3;

@@ -6,6 +6,7 @@
 #include "gqa.h"
 
 namespace vib3 {
+namespace {
 
 template <int DT, int D>
 __global__ __launch_bounds__(256) void k_gqa_append(vib3_gqa_append a) {
@@ -86,6 +87,7 @@ void launch_append(const vib3_gqa_append& a, hipStream_t st) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.tokens), dim3(256), 0, st, a);
 }
 
+}  // namespace
 }  // namespace vib3
 
 using namespace vib3;

@@ -2,6 +2,7 @@
 #include "gqa_simple.h"
 
 namespace vib3 {
+namespace {
 
 template <int DT, int D>
 __global__ __launch_bounds__(256) void k_gqa_chunk(vib3_gqa_chunk a) {
@@ -24,6 +25,7 @@ void launch_chunk(const vib3_gqa_chunk& a, hipStream_t st) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.q_tokens * a.heads + 3) / 4)), dim3(256), 0, st, a);
 }
 
+}  // namespace
 }  // namespace vib3
 
 using namespace vib3;
