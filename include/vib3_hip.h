@@ -696,7 +696,7 @@ int vib3_launch_gqa_decode(const vib3_gqa_decode *args, void *stream);
  * [cu_q[s], cu_q[s+1]) and the first lens[s] cached tokens; with nq of them, query i has the position
  * lens[s] - nq + i (a negative one sees nothing). The sum is vib3_launch_gqa_decode's. Queries behind
  * cu_q[num_seqs] are left as they were; offsets are cut to [0, q_tokens], lens[s] to the block
- * table's capacity. */
+ * table's capacity. Offsets must not decrease (rows may be left out otherwise). */
 typedef struct vib3_gqa_chunk {
     vib3_gqa_cache cache;
     int heads, q_tokens;               /* heads <= 1024 */

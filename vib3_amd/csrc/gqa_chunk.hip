@@ -1,28 +1,731 @@
 // gqa_chunk.hip — causal attention of each sequence's newest tokens over the paged key/value cache.
-#include "gqa_simple.h"
+//
+// Bound by the matrix cores for prompts, 4 dim flops per visible (query, token, head), by the cache's bytes for a few queries over
+// many tokens. The queries of a sequence times the heads of one key/value head's group are rows; a block is 32 NB rows of each wave of a
+// workgroup, which walks over the tokens, 64 at a time (a tile), with a running maximum and sum per row.
+//
+// Scores are formed transposed, S^T = K . Q^T, so that a lane holds one row's scores of 32 of the 64 tokens (the other lane
+// of the pair l, l + 32 the rest): the maximum and sum are almost all within a lane, and the probabilities, packed in pairs of
+// 16 bits, are as they stand the B operand of O^T = V^T . P^T (the tokens' order along k is free as long as V^T is read in the
+// same one, which the transposing LDS reads allow). The scores of the next tile are formed next to the softmax of this one, so that
+// the matrix cores and the vector units have work of one wave at a time.
+//
+// Keys and values go straight from memory to LDS, double-buffered. Each wave looks up the pages of a tile's 64 tokens, a token a
+// lane, three tiles ahead, and hands the addresses to the lanes that load. 16-byte chunk c of an LDS row lies at c ^ a function of
+// the row, which spreads the reads over the banks.
+//
+// Many blocks: a workgroup each, the longest of a sequence first. Few blocks: their tiles in order, with kBlockCost tiles' time in front of
+// each block, are cut into equal runs, one for each workgroup that fits the card, which a causal mask's unequal blocks and long caches
+// under few queries need alike; what a run has of a block goes to the workspace as it lies in registers, and a second launch
+// joins the parts. The runs follow from the lengths alone, which every workgroup reads for itself, so a captured launch follows them.
+#include <type_traits>
+
+#include "gqa.h"
 
 namespace vib3 {
 namespace {
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void k_gqa_chunk(vib3_gqa_chunk a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.q_tokens * a.heads) return;
-  const int t = (int)(w / a.heads), h = (int)(w % a.heads);
-  for (int s = 0; s < a.cache.num_seqs; s++) {
-    const int q0 = min(max(a.cu_q[s], 0), a.q_tokens), q1 = min(a.cu_q[s + 1], a.q_tokens);
-    if (t < q0 || t >= q1) continue;
-    attend_simple<DT, D>(a.cache, s, gqa_len(a.cache, a.lens[s]) - (q1 - t), h / (a.heads / a.cache.kv_heads),
-                         (const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride, a.scale, a.window, a.sinks,
-                         (uint16_t*)a.out + t * a.out_token_stride + h * a.out_head_stride);
-    return;
+constexpr int kTile = 64;         // tokens of one step
+constexpr int kMaxBlocks = 1024;  // of a launch in runs, and its most sequences
+constexpr int kBlockCost = 2;     // a block's fixed time, in tiles
+constexpr int kRuns = 256;
+
+// What tokens that are not seen are read from.
+__device__ const uint4 zero_token[256 / 8] = {};
+
+// Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
+// column l % 32, element i in row 8 (i / 4) + 4 (l / 32) + i % 4.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ f32x16 mma_wide(s16x8 a, s16x8 b, f32x16 c) {
+  if (DT == VIB3_DT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Where chunk 0 of a row lies, for rows of C chunks: 16 (or 8) rows in a row-wise read of one chunk fall into different banks.
+template <int C>
+__device__ __forceinline__ int key_swizzle(int row) {
+  return C >= 16 ? row & 15 : (row >> 1) & 7;
+}
+
+// The same for values, of which a transposing read takes 64 bytes of each of 8 rows.
+template <int C>
+__device__ __forceinline__ int value_swizzle(int row) {
+  return C >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+}
+
+// Maximum and sum over the lanes l and l + 32.
+__device__ __forceinline__ float pair_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// A word's two 16-bit elements with zeros in the place of infinities and NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
+}
+// The queries of a sequence.
+struct Queries {
+  int seq, q0, nq, len;  // its row of the table, its first query, their number, its tokens
+};
+
+__device__ __forceinline__ Queries queries_of(const vib3_gqa_chunk& a, int s) {
+  Queries q{s, 0, 0, 0};
+  if (s < a.cache.num_seqs) {
+    q.q0 = min(max(a.cu_q[s], 0), a.q_tokens);
+    q.nq = max(min(a.cu_q[s + 1], a.q_tokens) - q.q0, 0);
+    q.len = gqa_len(a.cache, a.lens[s]);
+  }
+  return q;
+}
+
+// What block b (of `size` rows) of a sequence sees, in tiles: `skip` tiles from the first token on (those with sinks), then from tile
+// `first` on.
+struct Block {
+  Queries q;
+  int row0, rows;        // its first row in the sequence, the sequence's rows
+  int low, high;         // the positions of its first and its last query
+  int skip, first, tiles;
+  __device__ __forceinline__ int token(int t) const { return (t < skip ? t : first + t - skip) * kTile; }
+};
+
+__device__ __forceinline__ Block block_of(const vib3_gqa_chunk& a, const Queries& q, int b, int size, int group) {
+  Block k;
+  k.q = q;
+  k.row0 = b * size;
+  k.rows = q.nq * group;
+  k.low = q.len - q.nq + k.row0 / group;
+  k.high = q.len - q.nq + (min(k.row0 + size, k.rows) - 1) / group;
+  const int start = window_start(max(k.low, 0), a.window);
+  k.first = start / kTile;
+  k.skip = min((min(a.sinks, start) + kTile - 1) / kTile, k.first);
+  k.tiles = k.high < 0 ? 0 : k.high / kTile + 1 - k.first + k.skip;
+  return k;
+}
+
+// Blocks of all sequences are numbered in order, a sequence's last block first (it sees the most tokens). Each wave finds block b
+// by itself, 64 sequences at a time; false: there is no block b.
+__device__ bool find_block(const vib3_gqa_chunk& a, int b, int size, int group, Block* out) {
+  const int lane = lane_id();
+  for (int s0 = 0; s0 < a.cache.num_seqs; s0 += 64) {
+    const Queries q = queries_of(a, s0 + lane);
+    int upto = (int)(((int64_t)q.nq * group + size - 1) / size);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const uint64_t hit = __ballot(b < upto);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const Queries mine{s0 + l, __builtin_amdgcn_readlane(q.q0, l), __builtin_amdgcn_readlane(q.nq, l),
+                         __builtin_amdgcn_readlane(q.len, l)};
+      *out = block_of(a, mine, __builtin_amdgcn_readlane(upto, l) - 1 - b, size, group);
+      return true;
+    }
+    b -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Workspace of a launch in runs. Slot w of the parts holds that of the block that run w starts with (where it does not cover all
+// of it), slot kRuns + w that of the block it ends in, if that is another one.
+struct ChunkWs {
+  int64_t* head;     // [3]: the blocks of a key/value head, their extent, the length of a run
+  int64_t* begin;    // [kMaxBlocks + 1] where the blocks begin
+  int32_t *seq, *in; // [kMaxBlocks] their sequences and numbers in them
+  float2* stat;      // [2 kRuns][rows] reference value (of unscaled scores) and sum
+  float* part;       // [2 kRuns][rows][dim] unnormalised sums, as the lanes hold them
+};
+
+inline size_t chunk_ws(int size, int dim, ChunkWs* w, void* base) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return (uint8_t*)base + p;
+  };
+  ChunkWs r;
+  r.head = (int64_t*)take(24);
+  r.begin = (int64_t*)take(8 * (kMaxBlocks + 1));
+  r.seq = (int32_t*)take(4 * kMaxBlocks);
+  r.in = (int32_t*)take(4 * kMaxBlocks);
+  r.stat = (float2*)take((size_t)8 * 2 * kRuns * size);
+  r.part = (float*)take((size_t)4 * 2 * kRuns * size * dim);
+  if (w) *w = r;
+  return at;
+}
+
+struct ChunkArgs {
+  vib3_gqa_chunk a;
+  ChunkWs w;
+  int group;
+};
+
+// The plan of a launch in runs, in LDS: each workgroup forms it for itself.
+struct Plan {
+  int64_t begin[kMaxBlocks + 1], sums[8];
+  int upto[kMaxBlocks];  // blocks of the sequences up to each
+  int16_t seq[kMaxBlocks], in[kMaxBlocks];
+  int blocks;
+};
+
+// An int64 that all lanes hold, as a value that is known to be uniform.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Sum of v over the threads before this one (THREADS of them); *all: over all of them. A barrier on the way in and out.
+template <int THREADS>
+__device__ int64_t scan_block(int64_t v, int64_t* sums, int64_t* all) {
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  int64_t sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t up = __shfl_up(sum, d);
+    if (lane >= d) sum += up;
+  }
+  __syncthreads();
+  if (lane == 63) sums[tid >> 6] = sum;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) {
+    if (i < tid >> 6) before += sums[i];
+    total += sums[i];
+  }
+  *all = total;
+  return before + sum - v;
+}
+
+template <int THREADS>
+__device__ void make_plan(const ChunkArgs& d, int size, Plan& p) {
+  const vib3_gqa_chunk& a = d.a;
+  const int tid = (int)threadIdx.x;
+  int blocks = 0;  // (no more than kMaxBlocks, unless the offsets decrease somewhere)
+  for (int s0 = 0; s0 < a.cache.num_seqs; s0 += THREADS) {
+    const int s = s0 + tid;
+    const int n = s < a.cache.num_seqs ? (int)(((int64_t)queries_of(a, s).nq * d.group + size - 1) / size) : 0;
+    int64_t all;
+    const int64_t before = scan_block<THREADS>(n, p.sums, &all);
+    if (s < a.cache.num_seqs) p.upto[s] = (int)min(blocks + before + n, (int64_t)kMaxBlocks);
+    blocks = (int)min(blocks + all, (int64_t)kMaxBlocks);
+  }
+  __syncthreads();
+  int64_t at = 0;
+  for (int b0 = 0; b0 < blocks; b0 += THREADS) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < blocks) {
+      int lo = 0, hi = a.cache.num_seqs - 1;  // the first sequence with upto > b
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (p.upto[mid] > b) hi = mid;
+        else lo = mid + 1;
+      }
+      const int in = b - (lo ? p.upto[lo - 1] : 0);
+      p.seq[b] = (int16_t)lo;
+      p.in[b] = (int16_t)in;
+      n = block_of(a, queries_of(a, lo), in, size, d.group).tiles;
+      n = n > 0 ? n + kBlockCost : 0;
+    }
+    int64_t all;
+    const int64_t before = scan_block<THREADS>(n, p.sums, &all);
+    if (b < blocks) p.begin[b] = at + before;
+    at += all;
+  }
+  if (tid == 0) {
+    p.begin[blocks] = at;
+    p.blocks = blocks;
+  }
+  __syncthreads();
+}
+
+template <int DT, int D, int WAVES, int NB, bool RUNS>
+__global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
+  constexpr int C = D / 8;                    // 16-byte chunks of a row
+  constexpr int KS = D / 16;                  // k steps of the scores
+  constexpr int VB = D / 32;                  // 32-column blocks of the sums
+  constexpr int kRows = WAVES * 32 * NB;      // of a block
+  constexpr int kPer = 64 / C;                // tokens of one load instruction of a wave
+  constexpr int kLoads = kTile / kPer / WAVES;  // load instructions of a wave for a tile's keys
+  // Scores a tile ahead of their softmax, and keys two ahead; a head of 256 has no registers for that.
+  constexpr bool kAhead = D < 256;
+  __shared__ __align__(1024) uint8_t ktile[2][kTile * D * 2];
+  __shared__ __align__(1024) uint8_t vtile[2][kTile * D * 2];
+  __shared__ int odd_values;                  // whether values were cleared
+  __shared__ std::conditional_t<RUNS, Plan, int> plan;
+
+  const vib3_gqa_chunk& a = d.a;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const float scale = exponent_scale(a.scale);
+  const uint32_t flip = sign_flip(a.scale);
+  const uint64_t zero = (uint64_t)zero_token;
+  if (tid == 0) odd_values = 0;  // (before the first block's first barrier)
+
+  // One block's tiles t0..t1 - 1 of key/value head g: its sums go to the output, or as a part to a slot of the workspace.
+  auto attend = [&](const Block& bl, int g, int t0, int t1, int slot) {
+    const int group = d.group;
+    // this lane's rows: their positions (-1: none) and the first tokens of their windows
+    int pos[NB], start[NB];
+    int64_t q_at[NB], o_at[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int r = bl.row0 + (wave * NB + n) * 32 + col, rr = min(r, bl.rows - 1), qi = rr / group;
+      const int64_t t = bl.q.q0 + qi, h = g * group + rr - qi * group;
+      q_at[n] = t * a.q_token_stride + h * a.q_head_stride;
+      o_at[n] = t * a.out_token_stride + h * a.out_head_stride;
+      pos[n] = r < bl.rows ? max(bl.q.len - bl.q.nq + qi, -1) : -1;
+      start[n] = pos[n] >= 0 ? window_start(pos[n], a.window) : 0;
+    }
+    // the wave's first and last position (of its rows that there are): tiles that all of them see whole, or none sees
+    const int w_row = bl.row0 + wave * NB * 32;
+    const bool any_rows = w_row < bl.rows;
+    const int w_low = bl.q.len - bl.q.nq + w_row / group;
+    const int w_high = any_rows ? bl.q.len - bl.q.nq + (min(w_row + NB * 32, bl.rows) - 1) / group : -1;
+    const int low_start = window_start(max(w_low, 0), a.window), high_start = window_start(max(w_high, 0), a.window);
+    const int block_start = window_start(max(bl.high, 0), a.window);
+
+    // queries: the B operand, this lane's row at k = 16 s + 8 half
+    s16x8 q[NB][KS];
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        uint4 v = *(const uint4*)((const uint16_t*)a.q + q_at[n] + 16 * s + 8 * half);
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        q[n][s] = __builtin_bit_cast(s16x8, v);
+      }
+    VIB3_WAIT_VM(0);  // here, once: a wait inside the loop would drain the tiles' loads
+
+    // Page numbers of a tile's tokens, a token a lane, then their places as offsets from the pools' start in bytes (-1: not seen).
+    // (With selects, not branches: registers are short here, and the compiler has put a copy that it needed for that at the end
+    // of a divergent branch in front of the instruction that brings the other lanes back, which lost their values.)
+    const int32_t* table = a.cache.block_table + (size_t)bl.q.seq * a.cache.max_pages;
+    const int64_t head_at = (int64_t)g * a.cache.head_stride;
+    int page_no = -1, in_page = -1;
+    auto ask = [&](int t) {
+      const int j = bl.token(min(t, t1 - 1)) + lane;
+      const bool ok = (t < t1) & (j < bl.q.len);
+      const int token = ok ? j : 0, page = token / a.cache.page_size;
+      in_page = ok ? token - page * a.cache.page_size : -1;
+      page_no = table[page];  // (a block with tiles has a first token, and its page an entry)
+    };
+    uint32_t from_lo[kLoads], from_hi[kLoads];  // of this lane's tokens of the tile that keys were loaded of last
+    auto place = [&]() -> uint64_t {
+      const bool ok = (in_page >= 0) & ((unsigned)page_no < (unsigned)a.cache.num_pages);
+      const int64_t at = 2 * ((int64_t)page_no * a.cache.page_stride + (int64_t)in_page * a.cache.token_stride + head_at);
+      const uint32_t none = ok ? 0 : ~0u, lo = (uint32_t)at | none, hi = (uint32_t)((uint64_t)at >> 32) | none;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int from = 4 * ((i * WAVES + wave) * kPer + lane / C);
+        from_lo[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)lo);
+        from_hi[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)hi);
+      }
+      return __ballot(ok);
+    };
+    auto load = [&](const void* pool, uint8_t* dst, auto swizzle) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int run = i * WAVES + wave, row = run * kPer + lane / C;
+        const uint64_t at = (uint64_t)from_hi[i] << 32 | from_lo[i];
+        const uint64_t p = (int32_t)from_hi[i] < 0 ? zero : (uint64_t)pool + at;
+        load_to_lds16((const void*)(p + (((lane % C) ^ swizzle(row)) * 16)), (lds_u8*)dst + run * 1024);
+      }
+    };
+    auto load_keys = [&](int t) { load(a.cache.keys, ktile[t & 1], [](int r) { return key_swizzle<C>(r); }); };
+    auto load_values = [&](int t) { load(a.cache.values, vtile[t & 1], [](int r) { return value_swizzle<C>(r); }); };
+    // A masked place has probability 0, and 0 times an infinity or a NaN is NaN: in tiles with masked places the values that
+    // this wave has loaded are cleared of those, and whether there were any is noted.
+    auto is_masked = [&](int base) { return !(base + kTile - 1 <= bl.low && (base >= block_start || base + kTile <= a.sinks)); };
+    auto clear_values = [&](int t) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        uint4* at = (uint4*)(vtile[t & 1] + (i * WAVES + wave) * 1024 + lane * 16);
+        const uint4 v = *at, w = make_uint4(finite_only<DT>(v.x), finite_only<DT>(v.y), finite_only<DT>(v.z), finite_only<DT>(v.w));
+        if (v.x != w.x || v.y != w.y || v.z != w.z || v.w != w.w) {
+          *at = w;
+          odd = true;
+        }
+      }
+      if (__any(odd) && lane == 0) odd_values = 1;
+    };
+
+    // S^T of a tile: two blocks of 32 tokens
+    auto form_scores = [&](int t, f32x16 (*s)[NB]) {
+      const lds_u8* k = (lds_u8*)ktile[t & 1] + col * D * 2;
+      const int k0 = fresh((half ^ key_swizzle<C>(col)) * 16);
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int n = 0; n < NB; n++) s[b][n] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const s16x8 key = lds_read16(k + b * 32 * D * 2 + (k0 ^ 32 * i));
+#pragma unroll
+          for (int n = 0; n < NB; n++) s[b][n] = mma_wide<DT>(key, q[n][i], s[b][n]);
+        }
+    };
+
+    f32x16 o[NB][VB] = {};
+    float m[NB], l[NB];  // running maximum (of unscaled scores) and this lane's part of the sum
+#pragma unroll
+    for (int n = 0; n < NB; n++) m[n] = -__builtin_huge_valf(), l[n] = 0.0f;
+    f32x16 s[2][NB];
+    uint64_t seen = 0, seen1 = 0;  // the tokens of this tile and the next that are there
+    if (t0 < t1) {
+      ask(t0);
+      seen = place();
+      load_keys(t0);
+      if constexpr (kAhead) {
+        ask(t0 + 1);
+        wait_lds_loads();
+        __syncthreads();
+        load_values(t0);
+        seen1 = place();
+        load_keys(t0 + 1);
+        ask(t0 + 2);
+        form_scores(t0, s);
+      } else {
+        load_values(t0);
+        ask(t0 + 1);
+      }
+    }
+    // this lane's place in a transposing read: row 4 half + (lane % 16) / 4, columns 16 ((lane / 16) % 2) + 4 (lane % 4)
+    const int vrow = 4 * half + ((lane & 15) >> 2);
+    const int vchunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    for (int t = t0; t < t1; t++) {
+      wait_lds_loads();
+      page_no = fresh(page_no);  // has landed too: no wait for it after the loads below
+      const int base = bl.token(t);
+      if (is_masked(base)) clear_values(t);
+      __syncthreads();  // values t and keys t (or t + 1) are in LDS; everyone is done with those before
+      // (loads past the last tile are of zeros)
+      const uint64_t mine = seen;
+      f32x16 s_next[2][NB];
+      if constexpr (kAhead) {
+        load_values(t + 1);
+        seen = seen1;
+        seen1 = place();
+        load_keys(t + 2);
+        ask(t + 3);
+        form_scores(t + 1, s_next);  // past the last tile: of whatever lies there, and not used
+      } else {
+        seen = place();
+        load_keys(t + 1);
+        load_values(t + 1);
+        ask(t + 2);
+        form_scores(t, s);
+      }
+      auto next = [&] {
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int n = 0; n < NB; n++) s[b][n] = s_next[b][n];
+        }
+      };
+      if (base > w_high || (base + kTile <= low_start && base >= a.sinks)) {  // no row of the wave sees any of it
+        next();
+        continue;
+      }
+      if (!(base + kTile - 1 <= w_low && (base >= high_start || base + kTile <= a.sinks) && mine == ~0ull)) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const uint32_t there = (uint32_t)(mine >> (32 * b)) >> (4 * half);
+          const int j0 = base + 32 * b + 4 * fresh(half);
+#pragma unroll
+          for (int n = 0; n < NB; n++) {
+            const int last = pos[n] - j0, from = start[n] - j0, sinks = a.sinks - j0;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int k = 8 * (i >> 2) + (i & 3);
+              const bool hidden = ((there >> k & 1) == 0) | (k > last) | ((k < from) & (k >= sinks));
+              s[b][n][i] = hidden ? -__builtin_huge_valf() : s[b][n][i];
+            }
+          }
+        }
+      }
+
+      uint32_t p[NB][16];
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        float top = s[0][n][0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[0][n][i]);
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, s[1][n][i]);
+        top = pair_max(top);
+        // The reference value of a row's exponentials follows its maximum only where that grew by more than kLag. (Each row by
+        // itself: what others of the wave see does not change its result.)
+        const bool grown = (top - m[n]) * scale > kLag<DT> || (m[n] == -__builtin_huge_valf() && top > m[n]);
+        if (__any(grown)) {
+          const float f = grown ? __builtin_amdgcn_exp2f((m[n] - top) * scale) : 1.0f;
+          m[n] = grown ? top : m[n];
+          l[n] *= f;
+#pragma unroll
+          for (int c = 0; c < VB; c++) o[n][c] *= f;
+        }
+        float ref = m[n] == -__builtin_huge_valf() ? 0.0f : m[n] * scale;
+        const bool far = __builtin_fabsf(ref) > kFarExponent;
+        if (__any(far)) {
+          const float off = far ? m[n] : 0.0f;
+          ref = far ? 0.0f : ref;
+#pragma unroll
+          for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[b][n][i] -= off;
+        }
+        ref -= kProbShift<DT>;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][i], scale, -ref));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][i + 1], scale, -ref));
+            l[n] += e0 + e1;
+            // rounded for the matrix cores; the sum l takes them unrounded
+            p[n][8 * b + (i >> 1)] = pack2<DT>(e0, e1);
+          }
+      }
+      lds_u8* const v = (lds_u8*)vtile[t & 1] + vrow * D * 2 + 8 * (lane & 1);
+      const int v0 = fresh((vchunk ^ value_swizzle<C>(vrow)) * 16);  // 16 and 8 rows further the swizzle is the same
+      // V^T for 32 columns and 16 tokens
+      auto values = [&](int k, int c) {
+        return join(lds_read_tr(v + 16 * k * D * 2 + (v0 ^ 64 * c)), lds_read_tr(v + (16 * k + 8) * D * 2 + (v0 ^ 64 * c)));
+      };
+      auto probs = [&](int n, int k) {
+        return __builtin_bit_cast(s16x8, make_uint4(p[n][4 * k], p[n][4 * k + 1], p[n][4 * k + 2], p[n][4 * k + 3]));
+      };
+#pragma unroll
+      for (int k = 0; k < kTile / 16; k++)
+#pragma unroll
+        for (int c = 0; c < VB; c++) {
+          const s16x8 x = values(k, c);
+#pragma unroll
+          for (int n = 0; n < NB; n++) o[n][c] = mma_wide<DT>(x, probs(n, k), o[n][c]);
+        }
+      next();
+    }
+    wait_lds_loads();  // those past the last tile: not into LDS that the next block's go to
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(odd_values)) {
+      // What was cleared, for the queries that do see it: infinities times a probability of 0 are NaN, as in other tiles.
+      // (Values, scores and probabilities come from memory again, so that the ordinary path holds nothing for this one.)
+#pragma unroll 1
+      for (int t = t0; t < t1; t++) {
+        if (!is_masked(bl.token(t))) continue;
+#pragma unroll 1
+        for (int j = bl.token(t); j < min(bl.token(t) + kTile, bl.q.len); j++) {
+          const int64_t at = gqa_token(a.cache, bl.q.seq, j);
+          if (at < 0) continue;
+          const uint16_t* key = (const uint16_t*)a.cache.keys + at + head_at;
+          const uint16_t* value = (const uint16_t*)a.cache.values + at + head_at;
+#pragma unroll
+          for (int n = 0; n < NB; n++) {
+            float score = 0.0f;
+#pragma unroll 1
+            for (int c = half; c < C; c += 2) {  // the other chunks are the pair's other lane's
+              float x[8], y[8];
+              unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + q_at[n] + 8 * c), x);
+              unpack8<DT>(*(const uint4*)(key + 8 * c), y);
+#pragma unroll
+              for (int i = 0; i < 8; i++) score = __builtin_fmaf(x[i], y[i], score);
+            }
+            score = a.scale < 0.0f ? -pair_sum(score) : pair_sum(score);
+            const float e = __builtin_amdgcn_exp2f((score - (m[n] == -__builtin_huge_valf() ? 0.0f : m[n])) * scale);
+            if (j > pos[n] || (j < start[n] && j >= a.sinks)) continue;
+#pragma unroll
+            for (int c = 0; c < VB; c++)
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const uint16_t y = value[32 * c + 8 * (i >> 2) + 4 * half + (i & 3)];
+                if (finite_only<DT>(y) != y) o[n][c][i] += e != 0.0f ? to_f32<DT>(y) : __builtin_nanf("");
+              }
+          }
+        }
+      }
+      __syncthreads();
+      if (tid == 0) odd_values = 0;
+    }
+
+    if (slot >= 0) {
+      float* part = d.w.part + (size_t)slot * kRows * D;
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const int row = (wave * NB + n) * 32 + col;
+        const float sum = pair_sum(l[n]);
+        if (half == 0) d.w.stat[(size_t)slot * kRows + row] = make_float2(m[n], sum);
+#pragma unroll
+        for (int c = 0; c < VB; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            *(float4*)(part + ((((wave * NB + n) * VB + c) * 4 + i) * 64 + lane) * 4) =
+                make_float4(o[n][c][4 * i], o[n][c][4 * i + 1], o[n][c][4 * i + 2], o[n][c][4 * i + 3]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const float sum = pair_sum(l[n]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool there = bl.row0 + (wave * NB + n) * 32 + col < bl.rows;
+      uint16_t* out = (uint16_t*)a.out + o_at[n];
+#pragma unroll
+      for (int c = 0; c < VB; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+          // columns 8 (i / 4) + 4 half + 0..3 and 8 further: the pair of lanes trades halves, so that each has 8 neighbouring ones
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(o[n][c][i + 2 * j] * inv, o[n][c][i + 2 * j + 1] * inv),
+                                                            pack2<DT>(o[n][c][i + 4 + 2 * j] * inv, o[n][c][i + 5 + 2 * j] * inv), false, false);
+            w[j] = x[0];
+            w[2 + j] = x[1];
+          }
+          if (there) *(uint4*)(out + 32 * c + 2 * i + 8 * half) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+  };
+
+  if constexpr (!RUNS) {
+    const int g = (int)(blockIdx.x % (unsigned)a.cache.kv_heads);
+    Block bl;
+    if (!find_block(a, (int)(blockIdx.x / (unsigned)a.cache.kv_heads), kRows, d.group, &bl)) return;
+    attend(bl, g, 0, bl.tiles, -1);
+  } else {
+    make_plan<WAVES * 64>(d, kRows, plan);
+    const int blocks = __builtin_amdgcn_readfirstlane(plan.blocks);
+    const int64_t extent = uniform64(plan.begin[blocks]), all = extent * a.cache.kv_heads;
+    const int64_t per = max((int64_t)1, (all + kRuns - 1) / kRuns);
+    // workgroups go to the XCDs in turn: an XCD's runs lie next to one another, mostly of one key/value head
+    const int run = (int)(blockIdx.x % 8) * (kRuns / 8) + (int)blockIdx.x / 8;
+    if (blockIdx.x == 0) {  // for the joining
+      for (int b = tid; b <= blocks; b += WAVES * 64) {
+        d.w.begin[b] = plan.begin[b];
+        if (b < blocks) d.w.seq[b] = plan.seq[b], d.w.in[b] = plan.in[b];
+      }
+      if (tid == 0) d.w.head[0] = blocks, d.w.head[1] = extent, d.w.head[2] = per;
+    }
+    const int64_t from = run * per, to = min(from + per, all);
+    if (from >= to) return;
+    int g = (int)(from / extent), b = 0;
+    int64_t at = from - g * extent, left = to - from;
+    for (int hi = blocks - 1; b < hi;) {  // the last block that begins at or before `at`
+      const int mid = (b + hi + 1) / 2;
+      if (uniform64(plan.begin[mid]) <= at) b = mid;
+      else hi = mid - 1;
+    }
+    for (bool first = true; left > 0; first = false) {
+      const int64_t begin = uniform64(plan.begin[b]), end = uniform64(plan.begin[b + 1]), upto = min(end, at + left);
+      if (end > begin) {
+        const Block bl = block_of(a, queries_of(a, __builtin_amdgcn_readfirstlane((int)plan.seq[b])),
+                                  __builtin_amdgcn_readfirstlane((int)plan.in[b]), kRows, d.group);
+        const int t0 = (int)max(at - begin - kBlockCost, (int64_t)0), t1 = (int)(upto - begin - kBlockCost);
+        if (t1 > t0) attend(bl, g, t0, t1, t0 == 0 && t1 == bl.tiles ? -1 : run + (first ? 0 : kRuns));
+      }
+      left -= upto - at;
+      at = upto;
+      if (++b == blocks) b = 0, g++, at = 0;
+    }
   }
 }
 
+// Joins the parts of 32 rows of a block: a wave for each 32 columns. Blocks that see nothing become zero.
+template <int DT, int D>
+__global__ __launch_bounds__(D * 2) void k_gqa_join_tiles(ChunkArgs d, int size) {
+  constexpr int VB = D / 32;
+  const vib3_gqa_chunk& a = d.a;
+  const int lane = (int)threadIdx.x & 63, c = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int subs = size / 32, sub = (int)blockIdx.x % subs, item = (int)blockIdx.x / subs;
+  const int blocks = (int)d.w.head[0];
+  const int64_t extent = d.w.head[1], per = d.w.head[2];
+  const int g = item / max(blocks, 1), b = item - g * blocks;
+  if (blocks == 0 || g >= a.cache.kv_heads) return;
+  const Queries q = queries_of(a, d.w.seq[b]);
+  const int row0 = d.w.in[b] * size + sub * 32, rows = q.nq * d.group;
+  if (row0 >= rows) return;
+  const int64_t lo = g * extent + d.w.begin[b], hi = g * extent + d.w.begin[b + 1];
+  const int w0 = (int)((lo + kBlockCost) / per), parts = hi > lo ? (int)((hi - 1) / per) - w0 + 1 : 0;
+  if (parts == 1) return;
+  const bool late = w0 * per < lo;
+  auto slot = [&](int j) { return (size_t)(w0 + j + (j == 0 && late ? kRuns : 0)); };
+  const float scale = exponent_scale(a.scale);
+  float m = -__builtin_huge_valf(), l = 0.0f;
+  for (int j = 0; j < parts; j++) m = fmaxf(m, d.w.stat[slot(j) * size + sub * 32 + col].x);
+  const float ref = m == -__builtin_huge_valf() ? 0.0f : m;
+  float o[16] = {};
+  for (int j = 0; j < parts; j++) {
+    const float2 st = d.w.stat[slot(j) * size + sub * 32 + col];
+    const float f = __builtin_amdgcn_exp2f((st.x - ref) * scale);
+    const float4* p = (const float4*)(d.w.part + slot(j) * size * D) + ((sub * VB + c) * 4) * 64 + lane;
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = p[i * 64];
+    l += f * st.y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      o[4 * i] += f * v[i].x;
+      o[4 * i + 1] += f * v[i].y;
+      o[4 * i + 2] += f * v[i].z;
+      o[4 * i + 3] += f * v[i].w;
+    }
+  }
+  const int r = row0 + col;
+  if (r >= rows) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int qi = r / d.group;
+  uint16_t* out = (uint16_t*)a.out + (int64_t)(q.q0 + qi) * a.out_token_stride + (int64_t)(g * d.group + r - qi * d.group) * a.out_head_stride;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    *(uint2*)(out + 32 * c + 8 * i + 4 * half) =
+        make_uint2(pack2<DT>(o[4 * i] * inv, o[4 * i + 1] * inv), pack2<DT>(o[4 * i + 2] * inv, o[4 * i + 3] * inv));
+}
+
+// Waves and row blocks of a wave: as their registers leave room for.
+template <int D>
+struct Shape {
+  static constexpr int waves = D == 256 ? 4 : 8, blocks = 1, rows = waves * 32 * blocks;
+};
+
+inline int block_rows(int dim) { return dim == 64 ? Shape<64>::rows : dim == 128 ? Shape<128>::rows : Shape<256>::rows; }
+
+template <int DT, int D>
+int launch_chunk(const ChunkArgs& d, hipStream_t st) {
+  using S = Shape<D>;
+  const vib3_gqa_chunk& a = d.a;
+  // Sequences' blocks number at most this many (each ends in one that is not full, and has a query)
+  const int64_t seqs = a.cache.num_seqs < a.q_tokens ? a.cache.num_seqs : a.q_tokens;
+  const int64_t blocks = ((int64_t)a.q_tokens * d.group + (S::rows - 1) * seqs) / S::rows, items = blocks * a.cache.kv_heads;
+  if (items > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
+  if (items >= 4 * kRuns || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false>), dim3((unsigned)items), dim3(S::waves * 64), 0, st, d);
+  } else {
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true>), dim3(kRuns), dim3(S::waves * 64), 0, st, d);
+    hipLaunchKernelGGL((k_gqa_join_tiles<DT, D>), dim3((unsigned)(items * (S::rows / 32))), dim3(D * 2), 0, st, d, S::rows);
+  }
+  VIB3_RETURN_LAUNCH();
+}
+
 template <int DT>
-void launch_chunk(const vib3_gqa_chunk& a, hipStream_t st) {
-  auto kernel = a.cache.dim == 64 ? k_gqa_chunk<DT, 64> : a.cache.dim == 128 ? k_gqa_chunk<DT, 128> : k_gqa_chunk<DT, 256>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.q_tokens * a.heads + 3) / 4)), dim3(256), 0, st, a);
+int launch_chunk_dt(const ChunkArgs& d, hipStream_t st) {
+  const int dim = d.a.cache.dim;
+  return dim == 64 ? launch_chunk<DT, 64>(d, st) : dim == 128 ? launch_chunk<DT, 128>(d, st) : launch_chunk<DT, 256>(d, st);
 }
 
 }  // namespace
@@ -32,7 +735,7 @@ using namespace vib3;
 
 extern "C" size_t vib3_gqa_chunk_workspace_bytes(const vib3_gqa_chunk* args) {
   if (!args || check_gqa_cache(args->cache) || args->q_tokens < 0 || !gqa_heads(args->heads, args->cache.kv_heads)) return 0;
-  return 256;
+  return chunk_ws(block_rows(args->cache.dim), args->cache.dim, nullptr, nullptr);
 }
 
 extern "C" int vib3_launch_gqa_chunk(const vib3_gqa_chunk* args, void* stream) {
@@ -46,8 +749,10 @@ extern "C" int vib3_launch_gqa_chunk(const vib3_gqa_chunk* args, void* stream) {
   if (!a.cu_q || !a.lens || !mla_aligned(a.q) || !mla_aligned(a.out) || !mla_stride(a.q_token_stride) || !mla_stride(a.q_head_stride) ||
       !mla_stride(a.out_token_stride) || !mla_stride(a.out_head_stride) || !a.workspace || ((uintptr_t)a.workspace & 255))
     return VIB3_ERR_BAD_POINTER;
-  if (a.workspace_bytes < vib3_gqa_chunk_workspace_bytes(&a)) return VIB3_ERR_WORKSPACE;
-  if (a.cache.dtype == VIB3_DT_F16) launch_chunk<VIB3_DT_F16>(a, (hipStream_t)stream);
-  else launch_chunk<VIB3_DT_BF16>(a, (hipStream_t)stream);
-  VIB3_RETURN_LAUNCH();
+  ChunkArgs d;
+  d.a = a;
+  d.group = a.heads / a.cache.kv_heads;
+  if (a.workspace_bytes < chunk_ws(block_rows(a.cache.dim), a.cache.dim, &d.w, a.workspace)) return VIB3_ERR_WORKSPACE;
+  return a.cache.dtype == VIB3_DT_F16 ? launch_chunk_dt<VIB3_DT_F16>(d, (hipStream_t)stream)
+                                      : launch_chunk_dt<VIB3_DT_BF16>(d, (hipStream_t)stream);
 }

@@ -429,7 +429,11 @@ __global__ __launch_bounds__(1024) void k_gqa_join(DecodeArgs d, int team) {
           const float* p = d.w.part + s * D + lane * E;
 #pragma unroll
           for (int e = 0; e < E; e++) v[k][e] = p[e];
-          if (j0 + k * team >= parts) st[k] = make_float2(-__builtin_huge_valf(), 0.0f);
+          if (j0 + k * team >= parts) {
+            st[k] = make_float2(-__builtin_huge_valf(), 0.0f);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[k][e] = 0.0f;
+          }
         }
         float top = m;
 #pragma unroll
@@ -443,7 +447,6 @@ __global__ __launch_bounds__(1024) void k_gqa_join(DecodeArgs d, int team) {
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
           const float w = __builtin_amdgcn_exp2f((st[k].x - ref) * scale);
-          if (w == 0.0f) continue;  // (a weight of 0 says nothing about what lies there)
           l += w * st[k].y;
 #pragma unroll
           for (int e = 0; e < E; e++) o[e] += w * v[k][e];
@@ -466,7 +469,6 @@ __global__ __launch_bounds__(1024) void k_gqa_join(DecodeArgs d, int team) {
       for (int e = 0; e < E; e++) o[e] = 0.0f;
       for (int w = 0; w < team; w++) {
         const float f = __builtin_amdgcn_exp2f((tops[wave + w] - ref) * scale);
-        if (f == 0.0f) continue;
         l += f * totals[wave + w];
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] += f * sums[wave + w][lane * E + e];
