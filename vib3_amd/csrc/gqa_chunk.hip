@@ -33,6 +33,13 @@ constexpr int kRuns = 256;
 // What tokens that are not seen are read from.
 __device__ const uint4 zero_token[256 / 8] = {};
 
+// 16 bytes a lane from global memory, at a wave-uniform address and a lane's offset, to LDS at base + 16 * lane (see mla.h's load_to_lds16).
+__device__ __forceinline__ void load_group_to_lds16(const void* g, uint32_t off, lds_u8* base) {
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
+  // (five wait states, should the address come straight from a vector instruction)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(g) : "memory", "m0");
+}
+
 // Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
 // column l % 32, element i in row 8 (i / 4) + 4 (l / 32) + i % 4.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -251,7 +258,7 @@ __device__ void make_plan(const ChunkArgs& d, int size, Plan& p) {
   __syncthreads();
 }
 
-template <int DT, int D, int WAVES, int NB, bool RUNS>
+template <int DT, int D, int WAVES, int NB, bool RUNS, bool WHOLE>
 __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
   constexpr int C = D / 8;                    // 16-byte chunks of a row
   constexpr int KS = D / 16;                  // k steps of the scores
@@ -309,43 +316,82 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
       }
     VIB3_WAIT_VM(0);  // here, once: a wait inside the loop would drain the tiles' loads
 
-    // Page numbers of a tile's tokens, a token a lane, then their places as offsets from the pools' start in bytes (-1: not seen).
+    // Page numbers of a tile's tokens, a token a lane, or with whole groups of kPer tokens on a page a group a lane; then their places as
+    // offsets from the pools' start in bytes (-1: not there).
     // (With selects, not branches: registers are short here, and the compiler has put a copy that it needed for that at the end
     // of a divergent branch in front of the instruction that brings the other lanes back, which lost their values.)
+    constexpr int kStep = WHOLE ? kPer : 1, kGroups = kTile / kStep;
     const int32_t* table = a.cache.block_table + (size_t)bl.q.seq * a.cache.max_pages;
     const int64_t head_at = (int64_t)g * a.cache.head_stride;
-    int page_no = -1, in_page = -1;
-    auto ask = [&](int t) {
-      const int j = bl.token(min(t, t1 - 1)) + lane;
-      const bool ok = (t < t1) & (j < bl.q.len);
-      const int token = ok ? j : 0, page = token / a.cache.page_size;
-      in_page = ok ? token - page * a.cache.page_size : -1;
-      page_no = table[page];  // (a block with tiles has a first token, and its page an entry)
+    const int first_token = lane % kGroups * kStep;
+    const int turn_page = kTile / a.cache.page_size, turn_rest = kTile - turn_page * a.cache.page_size;
+    int page = 0, rest = 0, page_no = -1, in_page = -1;  // page and rest: of tile `asked`
+    auto find = [&](int t) {  // by division, where a stretch of tiles begins
+      const int j = bl.token(t) + first_token;
+      page = j / a.cache.page_size;
+      rest = j - page * a.cache.page_size;
     };
-    uint32_t from_lo[kLoads], from_hi[kLoads];  // of this lane's tokens of the tile that keys were loaded of last
-    auto place = [&]() -> uint64_t {
+    auto ask = [&](int t) {
+      const bool ok = (t < t1) & (bl.token(t) + first_token < bl.q.len);
+      in_page = ok ? rest : -1;
+      page_no = table[ok ? page : 0];  // (a block with tiles has a first token, and its page an entry)
+      // the next tile's
+      if (t + 1 == bl.skip) {
+        find(t + 1);
+      } else {
+        rest += turn_rest;
+        page += turn_page;
+        const bool over = rest >= a.cache.page_size;
+        rest -= over ? a.cache.page_size : 0;
+        page += over ? 1 : 0;
+      }
+    };
+    struct Place {
+      uint32_t lo, hi;
+    };
+    auto place = [&]() -> Place {
       const bool ok = (in_page >= 0) & ((unsigned)page_no < (unsigned)a.cache.num_pages);
       const int64_t at = 2 * ((int64_t)page_no * a.cache.page_stride + (int64_t)in_page * a.cache.token_stride + head_at);
-      const uint32_t none = ok ? 0 : ~0u, lo = (uint32_t)at | none, hi = (uint32_t)((uint64_t)at >> 32) | none;
-#pragma unroll
-      for (int i = 0; i < kLoads; i++) {
-        const int from = 4 * ((i * WAVES + wave) * kPer + lane / C);
-        from_lo[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)lo);
-        from_hi[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)hi);
-      }
-      return __ballot(ok);
+      const uint32_t none = ok ? 0 : ~0u;
+      return Place{(uint32_t)at | none, (uint32_t)((uint64_t)at >> 32) | none};
     };
-    auto load = [&](const void* pool, uint8_t* dst, auto swizzle) {
+    // The tokens of a tile that are there.
+    auto seen_of = [&](int t, const Place& p) -> uint64_t {
+      if constexpr (!WHOLE) return __ballot((int)p.hi >= 0);
+      const uint64_t groups = __ballot((int)p.hi >= 0);
+      if (groups == ~0ull && bl.token(t) + kTile <= bl.q.len) return ~0ull;
+      return __ballot((groups >> (lane / kStep) & 1) != 0 && bl.token(t) + lane < bl.q.len);
+    };
+    // Chunk `lane % C ^ swizzle(row)` of this lane's token of each of the wave's load instructions. Of a whole group the first token's address is
+    // the same for all lanes, and what a lane adds to it the same for all groups (of every second one, for the keys of a head of 256).
+    auto load = [&](const void* pool, uint8_t* dst, const Place& at, const uint32_t (&lane_at)[2], auto swizzle) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const int run = i * WAVES + wave, row = run * kPer + lane / C;
-        const uint64_t at = (uint64_t)from_hi[i] << 32 | from_lo[i];
-        const uint64_t p = (int32_t)from_hi[i] < 0 ? zero : (uint64_t)pool + at;
-        load_to_lds16((const void*)(p + (((lane % C) ^ swizzle(row)) * 16)), (lds_u8*)dst + run * 1024);
+        if constexpr (WHOLE) {
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at.lo, run), hi = (uint32_t)__builtin_amdgcn_readlane((int)at.hi, run);
+          const bool none = (int32_t)hi < 0;
+          const uint64_t p = none ? zero : (uint64_t)pool + ((uint64_t)hi << 32 | lo);
+          load_group_to_lds16((const void*)p, none ? (uint32_t)(lane % C) * 16 : lane_at[D == 256 ? i & 1 : 0], (lds_u8*)dst + run * 1024);
+        } else {
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)at.lo), hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)at.hi);
+          const uint64_t p = (int32_t)hi < 0 ? zero : (uint64_t)pool + ((uint64_t)hi << 32 | lo);
+          load_to_lds16((const void*)(p + (((lane % C) ^ swizzle(row)) * 16)), (lds_u8*)dst + run * 1024);
+        }
       }
     };
-    auto load_keys = [&](int t) { load(a.cache.keys, ktile[t & 1], [](int r) { return key_swizzle<C>(r); }); };
-    auto load_values = [&](int t) { load(a.cache.values, vtile[t & 1], [](int r) { return value_swizzle<C>(r); }); };
+    auto key_of = [](int r) { return key_swizzle<C>(r); };
+    auto value_of = [](int r) { return value_swizzle<C>(r); };
+    uint32_t key_at[2], value_at[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int row = (i * WAVES + wave) * kPer + lane / C;
+      const uint32_t token = (uint32_t)(lane / C) * (uint32_t)a.cache.token_stride * 2;
+      key_at[i] = token + ((lane % C) ^ key_of(row)) * 16;
+      value_at[i] = token + ((lane % C) ^ value_of(row)) * 16;
+    }
+    auto load_keys = [&](int t, const Place& p) { load(a.cache.keys, ktile[t & 1], p, key_at, key_of); };
+    auto load_values = [&](int t, const Place& p) { load(a.cache.values, vtile[t & 1], p, value_at, value_of); };
     // A masked place has probability 0, and 0 times an infinity or a NaN is NaN: in tiles with masked places the values that
     // this wave has loaded are cleared of those, and whether there were any is noted.
     auto is_masked = [&](int base) { return !(base + kTile - 1 <= bl.low && (base >= block_start || base + kTile <= a.sinks)); };
@@ -354,6 +400,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         uint4* at = (uint4*)(vtile[t & 1] + (i * WAVES + wave) * 1024 + lane * 16);
+        // (of a whole group the tokens past the last one are what lies in its page)
+        if (WHOLE && bl.token(t) + (i * WAVES + wave) * kPer + lane / C >= bl.q.len) *at = make_uint4(0, 0, 0, 0);
         const uint4 v = *at, w = make_uint4(finite_only<DT>(v.x), finite_only<DT>(v.y), finite_only<DT>(v.z), finite_only<DT>(v.w));
         if (v.x != w.x || v.y != w.y || v.z != w.z || v.w != w.w) {
           *at = w;
@@ -387,28 +435,32 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
     for (int n = 0; n < NB; n++) m[n] = -__builtin_huge_valf(), l[n] = 0.0f;
     f32x16 s[2][NB];
     uint64_t seen = 0, seen1 = 0;  // the tokens of this tile and the next that are there
+    Place p1{};                    // of the next tile
     if (t0 < t1) {
+      find(t0);
       ask(t0);
-      seen = place();
-      load_keys(t0);
+      Place p0 = place();
+      seen = seen_of(t0, p0);
+      load_keys(t0, p0);
+      ask(t0 + 1);
       if constexpr (kAhead) {
-        ask(t0 + 1);
         wait_lds_loads();
         __syncthreads();
-        load_values(t0);
-        seen1 = place();
-        load_keys(t0 + 1);
+        load_values(t0, p0);
+        p1 = place();
+        seen1 = seen_of(t0 + 1, p1);
+        load_keys(t0 + 1, p1);
         ask(t0 + 2);
         form_scores(t0, s);
       } else {
-        load_values(t0);
-        ask(t0 + 1);
+        load_values(t0, p0);
       }
     }
     // this lane's place in a transposing read: row 4 half + (lane % 16) / 4, columns 16 ((lane / 16) % 2) + 4 (lane % 4)
     const int vrow = 4 * half + ((lane & 15) >> 2);
     const int vchunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-    for (int t = t0; t < t1; t++) {
+    // One tile: its scores in s, the next one's into s_next.
+    auto step = [&](int t, f32x16 (*s)[NB], f32x16 (*s_next)[NB]) {
       wait_lds_loads();
       page_no = fresh(page_no);  // has landed too: no wait for it after the loads below
       const int base = bl.token(t);
@@ -416,33 +468,23 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
       __syncthreads();  // values t and keys t (or t + 1) are in LDS; everyone is done with those before
       // (loads past the last tile are of zeros)
       const uint64_t mine = seen;
-      f32x16 s_next[2][NB];
       if constexpr (kAhead) {
-        load_values(t + 1);
+        load_values(t + 1, p1);
         seen = seen1;
-        seen1 = place();
-        load_keys(t + 2);
+        p1 = place();
+        seen1 = seen_of(t + 2, p1);
+        load_keys(t + 2, p1);
         ask(t + 3);
         form_scores(t + 1, s_next);  // past the last tile: of whatever lies there, and not used
       } else {
-        seen = place();
-        load_keys(t + 1);
-        load_values(t + 1);
+        p1 = place();
+        seen = seen_of(t + 1, p1);
+        load_keys(t + 1, p1);
+        load_values(t + 1, p1);
         ask(t + 2);
         form_scores(t, s);
       }
-      auto next = [&] {
-        if constexpr (kAhead) {
-#pragma unroll
-          for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int n = 0; n < NB; n++) s[b][n] = s_next[b][n];
-        }
-      };
-      if (base > w_high || (base + kTile <= low_start && base >= a.sinks)) {  // no row of the wave sees any of it
-        next();
-        continue;
-      }
+      if (base > w_high || (base + kTile <= low_start && base >= a.sinks)) return;  // no row of the wave sees any of it
       if (!(base + kTile - 1 <= w_low && (base >= high_start || base + kTile <= a.sinks) && mine == ~0ull)) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -519,7 +561,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
 #pragma unroll
           for (int n = 0; n < NB; n++) o[n][c] = mma_wide<DT>(x, probs(n, k), o[n][c]);
         }
-      next();
+    };
+    if constexpr (kAhead) {  // the two sets of scores in turns
+      f32x16 other[2][NB];
+      for (int t = t0; t < t1; t += 2) {
+        step(t, s, other);
+        if (t + 1 < t1) step(t + 1, other, s);
+      }
+    } else {
+      for (int t = t0; t < t1; t++) step(t, s, s);
     }
     wait_lds_loads();  // those past the last tile: not into LDS that the next block's go to
     __syncthreads();
@@ -705,7 +755,7 @@ struct Shape {
 
 inline int block_rows(int dim) { return dim == 64 ? Shape<64>::rows : dim == 128 ? Shape<128>::rows : Shape<256>::rows; }
 
-template <int DT, int D>
+template <int DT, int D, bool WHOLE>
 int launch_chunk(const ChunkArgs& d, hipStream_t st) {
   using S = Shape<D>;
   const vib3_gqa_chunk& a = d.a;
@@ -714,9 +764,9 @@ int launch_chunk(const ChunkArgs& d, hipStream_t st) {
   const int64_t blocks = ((int64_t)a.q_tokens * d.group + (S::rows - 1) * seqs) / S::rows, items = blocks * a.cache.kv_heads;
   if (items > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
   if (items >= 4 * kRuns || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
-    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false>), dim3((unsigned)items), dim3(S::waves * 64), 0, st, d);
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false, WHOLE>), dim3((unsigned)items), dim3(S::waves * 64), 0, st, d);
   } else {
-    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true>), dim3(kRuns), dim3(S::waves * 64), 0, st, d);
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true, WHOLE>), dim3(kRuns), dim3(S::waves * 64), 0, st, d);
     hipLaunchKernelGGL((k_gqa_join_tiles<DT, D>), dim3((unsigned)(items * (S::rows / 32))), dim3(D * 2), 0, st, d, S::rows);
   }
   VIB3_RETURN_LAUNCH();
@@ -724,8 +774,11 @@ int launch_chunk(const ChunkArgs& d, hipStream_t st) {
 
 template <int DT>
 int launch_chunk_dt(const ChunkArgs& d, hipStream_t st) {
-  const int dim = d.a.cache.dim;
-  return dim == 64 ? launch_chunk<DT, 64>(d, st) : dim == 128 ? launch_chunk<DT, 128>(d, st) : launch_chunk<DT, 256>(d, st);
+  const vib3_gqa_cache& c = d.a.cache;
+  // whole groups of tokens on a page, and their distance in 32 bits
+  if (c.page_size % 8 == 0 && c.token_stride < (1 << 27))
+    return c.dim == 64 ? launch_chunk<DT, 64, true>(d, st) : c.dim == 128 ? launch_chunk<DT, 128, true>(d, st) : launch_chunk<DT, 256, true>(d, st);
+  return c.dim == 64 ? launch_chunk<DT, 64, false>(d, st) : c.dim == 128 ? launch_chunk<DT, 128, false>(d, st) : launch_chunk<DT, 256, false>(d, st);
 }
 
 }  // namespace
