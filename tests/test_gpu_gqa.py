@@ -430,6 +430,18 @@ def test_chunk_sequence_counts(seqs):
     check_chunk(c, *chunk(c, 4, nq), nq)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,nq,nk", [
+    (32, 8, 128, BF16, [70] + [5] * 40, [9000] + [9] * 40), (8, 1, 256, F16, [1] * 300 + [20] + [1] * 300, [3] * 300 + [6000] + [130] * 300),
+    (6, 2, 64, F16, [300, 2, 300] + [2] * 500, [301, 7000, 5000] + [2] * 500), (4, 1, 128, F16, [1] * 20, [64 * i + 1 for i in range(20)]),
+    (16, 16, 64, BF16, [0, 3, 0, 400, 0], [0, 20000, 5, 400, 64]), (8, 1, 128, BF16, [2] * 1024, [70] * 1024),
+])
+def test_chunk_long_sequences_beside_short_ones(heads, kv_heads, dim, dtype, nq, nk):
+    """Blocks that are cut into pieces beside whole ones, and counts of them around those that one launch plans for."""
+    c = Paged(nk, kv_heads, dim, dtype, 64)
+    check_chunk(c, *chunk(c, heads, nq), nq)
+    check_chunk(c, *chunk(c, heads, nq, window=900, sinks=70), nq, window=900, sinks=70)
+
+
 def test_chunk_missing_pages_are_not_seen():
     c = Paged([500, 70], 2, 128, BF16, 16, seed=24)
     c.table[0, 3:7], c.table[1, 0] = -1, 1000

@@ -14,10 +14,10 @@
 // lane, three tiles ahead, and hands the addresses to the lanes that load. 16-byte chunk c of an LDS row lies at c ^ a function of
 // the row, which spreads the reads over the banks.
 //
-// Many blocks: a workgroup each, the longest of a sequence first. Few blocks: their tiles in order, with kBlockCost tiles' time in front of
-// each block, are cut into equal runs, one for each workgroup that fits the card, which a causal mask's unequal blocks and long caches
-// under few queries need alike; what a run has of a block goes to the workspace as it lies in registers, and a second launch
-// joins the parts. The runs follow from the lengths alone, which every workgroup reads for itself, so a captured launch follows them.
+// Many blocks: a workgroup each, the longest of a sequence first. Few blocks: long ones are cut along the tokens into pieces, which a
+// causal mask's unequal blocks and long caches under few queries need alike; a piece's sums go to the workspace as they lie in
+// registers, and a second launch joins them. How long a piece is follows from the lengths alone, which every workgroup reads for
+// itself, so a captured launch follows them.
 #include <type_traits>
 
 #include "gqa.h"
@@ -26,9 +26,13 @@ namespace vib3 {
 namespace {
 
 constexpr int kTile = 64;         // tokens of one step
-constexpr int kMaxBlocks = 1024;  // of a launch in runs, and its most sequences
-constexpr int kBlockCost = 2;     // a block's fixed time, in tiles
-constexpr int kRuns = 256;
+constexpr int kMaxBlocks = 1024;  // of a launch that may cut them, and its most sequences
+// What a piece takes besides its tiles, and what the parts of as many pieces as there are workgroups on the card take on their way through
+// memory and with the second launch, in tiles' time. (32 heads over 8: 2048 tokens cut 82 us, whole 78; 512 after 32768 tokens 301 and 950.)
+constexpr int kPieceCost = 2, kPartsCost = 8, kJoinCost = 2;
+
+// Workgroups on the card at a time.
+__host__ __device__ constexpr int card_groups(int dim) { return dim == 64 ? 512 : 256; }
 
 // What tokens that are not seen are read from.
 __device__ const uint4 zero_token[256 / 8] = {};
@@ -36,8 +40,8 @@ __device__ const uint4 zero_token[256 / 8] = {};
 // 16 bytes a lane from global memory, at a wave-uniform address and a lane's offset, to LDS at base + 16 * lane (see mla.h's load_to_lds16).
 __device__ __forceinline__ void load_group_to_lds16(const void* g, uint32_t off, lds_u8* base) {
   const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base);
-  // (five wait states, should the address come straight from a vector instruction)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(g) : "memory", "m0");
+  // (the address is a scalar select: a vector instruction that wrote it would need wait states that nobody sees here)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(g) : "memory", "m0");
 }
 
 // Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
@@ -143,14 +147,18 @@ __device__ bool find_block(const vib3_gqa_chunk& a, int b, int size, int group, 
   return false;
 }
 
-// Workspace of a launch in runs. Slot w of the parts holds that of the block that run w starts with (where it does not cover all
-// of it), slot kRuns + w that of the block it ends in, if that is another one.
+// A block that was cut, for the joining: its first query's token, the rows of its sequence, its first row there, its pieces, and their
+// first slot (of key/value head 0).
+struct JoinBlock {
+  int q0, rows, row0, pieces, slot, pad[3];
+};
+
+// Workspace of a launch that may cut blocks: fewer than 2 pieces for each workgroup on the card are of cut blocks.
 struct ChunkWs {
-  int64_t* head;     // [3]: the blocks of a key/value head, their extent, the length of a run
-  int64_t* begin;    // [kMaxBlocks + 1] where the blocks begin
-  int32_t *seq, *in; // [kMaxBlocks] their sequences and numbers in them
-  float2* stat;      // [2 kRuns][rows] reference value (of unscaled scores) and sum
-  float* part;       // [2 kRuns][rows][dim] unnormalised sums, as the lanes hold them
+  int32_t* head;     // [2]: cut blocks of a key/value head, their slots
+  JoinBlock* join;   // [groups]
+  float2* stat;      // [slots][rows] reference value (of unscaled scores) and sum
+  float* part;       // [slots][rows][dim] unnormalised sums, as the lanes hold them
 };
 
 inline size_t chunk_ws(int size, int dim, ChunkWs* w, void* base) {
@@ -161,12 +169,11 @@ inline size_t chunk_ws(int size, int dim, ChunkWs* w, void* base) {
     return (uint8_t*)base + p;
   };
   ChunkWs r;
-  r.head = (int64_t*)take(24);
-  r.begin = (int64_t*)take(8 * (kMaxBlocks + 1));
-  r.seq = (int32_t*)take(4 * kMaxBlocks);
-  r.in = (int32_t*)take(4 * kMaxBlocks);
-  r.stat = (float2*)take((size_t)8 * 2 * kRuns * size);
-  r.part = (float*)take((size_t)4 * 2 * kRuns * size * dim);
+  r.head = (int32_t*)take(8);
+  r.join = (JoinBlock*)take(sizeof(JoinBlock) * card_groups(dim));
+  const size_t slots = 2 * (size_t)card_groups(dim);
+  r.stat = (float2*)take(8 * slots * size);
+  r.part = (float*)take(4 * slots * size * dim);
   if (w) *w = r;
   return at;
 }
@@ -177,101 +184,173 @@ struct ChunkArgs {
   int group;
 };
 
-// The plan of a launch in runs, in LDS: each workgroup forms it for itself.
+// The plan of a launch that may cut blocks, in LDS: each workgroup forms it for itself, which is why it takes few steps.
 struct Plan {
-  int64_t begin[kMaxBlocks + 1], sums[8];
-  int upto[kMaxBlocks];  // blocks of the sequences up to each
+  int wave_sums[2][8], wave_counts[8][6], wave_rows[8];
+  float wave_tiles[8];
+  int wave_longest[8];
+  int upto[kMaxBlocks];                    // blocks of the sequences up to each
+  int q0[kMaxBlocks], nq[kMaxBlocks], len[kMaxBlocks];
+  int tiles[kMaxBlocks];
+  int16_t begin[kMaxBlocks + 1];           // pieces of the blocks before each
   int16_t seq[kMaxBlocks], in[kMaxBlocks];
-  int blocks;
+  int16_t slot[kMaxBlocks + 1];            // pieces of cut blocks before each
+  int16_t cuts[kMaxBlocks + 1];            // cut blocks before each
 };
 
-// An int64 that all lanes hold, as a value that is known to be uniform.
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
+// v of lane l combined with those of the lanes below, by `f`; `none` does nothing there. Lane 63 has all.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T v, T none, F f) {
+  const int o = __builtin_bit_cast(int, none);
+  auto step = [&](int moved) { v = f(v, __builtin_bit_cast(T, moved)); };
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x111, 0xf, 0xf, false));  // from the lane below in a row of 16
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x112, 0xf, 0xf, false));  // 2 below
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x114, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x118, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false));  // lane 15's to the second row, 47's to the last
+  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false));  // lane 31's to the upper half
+  return v;
+}
+__device__ __forceinline__ int add_up(int v) {
+  return wave_scan(v, 0, [](int a, int b) { return a + b; });
 }
 
-// Sum of v over the threads before this one (THREADS of them); *all: over all of them. A barrier on the way in and out.
+// Sum of v over the threads before this one (THREADS of them); *all: over all of them. A barrier; calls take turns with `sums`.
 template <int THREADS>
-__device__ int64_t scan_block(int64_t v, int64_t* sums, int64_t* all) {
-  const int tid = (int)threadIdx.x, lane = tid & 63;
-  int64_t sum = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t up = __shfl_up(sum, d);
-    if (lane >= d) sum += up;
-  }
+__device__ int scan_block(int v, int* sums, int* all) {
+  const int tid = (int)threadIdx.x, upto = add_up(v);
+  if ((tid & 63) == 63) sums[tid >> 6] = upto;
   __syncthreads();
-  if (lane == 63) sums[tid >> 6] = sum;
-  __syncthreads();
-  int64_t before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < THREADS / 64; i++) {
-    if (i < tid >> 6) before += sums[i];
-    total += sums[i];
+    const int s = sums[i];
+    before += i < tid >> 6 ? s : 0;
+    total += s;
   }
   *all = total;
-  return before + sum - v;
+  return before + upto - v;
 }
 
 template <int THREADS>
-__device__ void make_plan(const ChunkArgs& d, int size, Plan& p) {
+__device__ int make_plan(const ChunkArgs& d, int size, int groups, Plan& p) {
+  constexpr int kWaves = THREADS / 64;
   const vib3_gqa_chunk& a = d.a;
-  const int tid = (int)threadIdx.x;
-  int blocks = 0;  // (no more than kMaxBlocks, unless the offsets decrease somewhere)
+  const int tid = (int)threadIdx.x, wave = tid >> 6;
+  const bool last = (tid & 63) == 63;
+  int turn = 0, blocks = 0;  // (no more than kMaxBlocks, unless the offsets decrease somewhere)
   for (int s0 = 0; s0 < a.cache.num_seqs; s0 += THREADS) {
     const int s = s0 + tid;
-    const int n = s < a.cache.num_seqs ? (int)(((int64_t)queries_of(a, s).nq * d.group + size - 1) / size) : 0;
-    int64_t all;
-    const int64_t before = scan_block<THREADS>(n, p.sums, &all);
-    if (s < a.cache.num_seqs) p.upto[s] = (int)min(blocks + before + n, (int64_t)kMaxBlocks);
-    blocks = (int)min(blocks + all, (int64_t)kMaxBlocks);
+    const Queries q = queries_of(a, s);  // (without queries past the last sequence)
+    const int n = min((int)(((int64_t)q.nq * d.group + size - 1) / size), kMaxBlocks);
+    int all;
+    const int before = scan_block<THREADS>(n, p.wave_sums[turn ^= 1], &all);
+    if (s < a.cache.num_seqs) {
+      p.upto[s] = min(blocks + before + n, kMaxBlocks);
+      p.q0[s] = q.q0, p.nq[s] = q.nq, p.len[s] = q.len;
+    }
+    blocks = min(blocks + all, kMaxBlocks);
   }
   __syncthreads();
-  int64_t at = 0;
+  float tiles = 0.0f;
+  int rows = 0, longest = 0;
+  for (int b = tid; b < blocks; b += THREADS) {
+    int lo = 0, hi = a.cache.num_seqs - 1;  // the first sequence with upto > b
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (p.upto[mid] > b) hi = mid;
+      else lo = mid + 1;
+    }
+    const int in = b - (lo ? p.upto[lo - 1] : 0);
+    p.seq[b] = (int16_t)lo;
+    p.in[b] = (int16_t)in;
+    const Block bl = block_of(a, Queries{lo, p.q0[lo], p.nq[lo], p.len[lo]}, in, size, d.group);
+    p.tiles[b] = bl.tiles;
+    tiles += (float)bl.tiles;
+    longest = max(longest, bl.tiles);
+    rows += min(size, bl.rows - bl.row0);
+  }
+  tiles = wave_scan(tiles, 0.0f, [](float x, float y) { return x + y; });
+  rows = add_up(rows);
+  longest = wave_scan(longest, 0, [](int x, int y) { return max(x, y); });
+  if (last) p.wave_tiles[wave] = tiles, p.wave_rows[wave] = rows, p.wave_longest[wave] = longest;
+  __syncthreads();
+  float all_tiles = 0.0f, all_rows = 0.0f;
+  longest = 1;
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) {
+    all_tiles += p.wave_tiles[i];
+    all_rows += (float)p.wave_rows[i];
+    longest = max(longest, p.wave_longest[i]);
+  }
+  all_tiles *= (float)a.cache.kv_heads;
+  // The length of a piece: whole blocks, or an even share of the tiles, or more by a third or by half where the even share's pieces do not fit
+  // the card at a time: whichever takes least, of the longest piece, or of rounds of pieces over the card, and of the parts' time.
+  // (An even share is rounded up, above what the sum of tiles lacks: the pieces of cut blocks are fewer than twice the workgroups.)
+  const float even = all_tiles / (float)groups * 1.0001f;
+  const int length[3] = {(int)fminf(even, 1e9f) + 1, (int)fminf(even * 1.34f, 1e9f) + 1, (int)fminf(even * 2.0f, 1e9f) + 1};
+  int count[6] = {};  // pieces, and those of cut blocks
+  for (int b = tid; b < blocks; b += THREADS)
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const int n = max((p.tiles[b] + length[k] - 1) / length[k], 1);
+      count[k] += n;
+      count[3 + k] += n > 1 ? n : 0;
+    }
+#pragma unroll
+  for (int k = 0; k < 6; k++) {
+    count[k] = add_up(count[k]);
+    if (last) p.wave_counts[wave][k] = count[k];
+  }
+  __syncthreads();
+  auto cost = [&](int len, float pieces) {
+    return fmaxf((float)(len + kPieceCost), ceilf(pieces / (float)groups) * (all_tiles / pieces + kPieceCost));
+  };
+  const float filled = all_rows / ((float)max(blocks, 1) * (float)size);
+  int piece = longest;
+  float best = cost(piece, fmaxf((float)blocks * (float)a.cache.kv_heads, 1.0f));
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    int pieces = 0, slots = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) pieces += p.wave_counts[i][k], slots += p.wave_counts[i][3 + k];
+    const float c = cost(length[k], fmaxf((float)pieces * (float)a.cache.kv_heads, 1.0f)) + kJoinCost +
+                    kPartsCost * filled * (float)slots * (float)a.cache.kv_heads / (float)groups;
+    if (slots > 0 && c < best) best = c, piece = length[k];
+  }
+  uint32_t at = 0;  // pieces (of a key/value head fewer than 2^11), above them those of cut blocks (as many), and the cut blocks
   for (int b0 = 0; b0 < blocks; b0 += THREADS) {
     const int b = b0 + tid;
-    int n = 0;
+    uint32_t n = 0;
     if (b < blocks) {
-      int lo = 0, hi = a.cache.num_seqs - 1;  // the first sequence with upto > b
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (p.upto[mid] > b) hi = mid;
-        else lo = mid + 1;
-      }
-      const int in = b - (lo ? p.upto[lo - 1] : 0);
-      p.seq[b] = (int16_t)lo;
-      p.in[b] = (int16_t)in;
-      n = block_of(a, queries_of(a, lo), in, size, d.group).tiles;
-      n = n > 0 ? n + kBlockCost : 0;
+      n = (uint32_t)max((p.tiles[b] + piece - 1) / piece, 1);
+      if (n > 1) n += n << 11 | 1u << 22;
     }
-    int64_t all;
-    const int64_t before = scan_block<THREADS>(n, p.sums, &all);
-    if (b < blocks) p.begin[b] = at + before;
-    at += all;
+    int all;
+    const uint32_t before = at + (uint32_t)scan_block<THREADS>((int)n, p.wave_sums[turn ^= 1], &all);
+    if (b < blocks) p.begin[b] = (int16_t)(before & 2047), p.slot[b] = (int16_t)(before >> 11 & 2047), p.cuts[b] = (int16_t)(before >> 22);
+    at += (uint32_t)all;
   }
-  if (tid == 0) {
-    p.begin[blocks] = at;
-    p.blocks = blocks;
-  }
+  if (tid == 0) p.begin[blocks] = (int16_t)(at & 2047), p.slot[blocks] = (int16_t)(at >> 11 & 2047), p.cuts[blocks] = (int16_t)(at >> 22);
   __syncthreads();
+  return blocks;
 }
 
-template <int DT, int D, int WAVES, int NB, bool RUNS, bool WHOLE>
-__global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
+template <int DT, int D, int WAVES, int NB, bool CUT, bool WHOLE>
+__global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(ChunkArgs d) {
   constexpr int C = D / 8;                    // 16-byte chunks of a row
   constexpr int KS = D / 16;                  // k steps of the scores
   constexpr int VB = D / 32;                  // 32-column blocks of the sums
   constexpr int kRows = WAVES * 32 * NB;      // of a block
   constexpr int kPer = 64 / C;                // tokens of one load instruction of a wave
   constexpr int kLoads = kTile / kPer / WAVES;  // load instructions of a wave for a tile's keys
-  // Scores a tile ahead of their softmax, and keys two ahead; a head of 256 has no registers for that.
-  constexpr bool kAhead = D < 256;
+  // Scores a tile ahead of their softmax, and keys two ahead. A head of 256 has no registers for that; one of 64 does without, and four
+  // waves fit on a SIMD instead of two (12288 tokens of 64 heads over 8: 1.78 -> 1.49 ms).
+  constexpr bool kAhead = D == 128;
   __shared__ __align__(1024) uint8_t ktile[2][kTile * D * 2];
   __shared__ __align__(1024) uint8_t vtile[2][kTile * D * 2];
   __shared__ int odd_values;                  // whether values were cleared
-  __shared__ std::conditional_t<RUNS, Plan, int> plan;
+  __shared__ std::conditional_t<CUT, Plan, int> plan;
 
   const vib3_gqa_chunk& a = d.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -617,6 +696,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
       float* part = d.w.part + (size_t)slot * kRows * D;
 #pragma unroll
       for (int n = 0; n < NB; n++) {
+        if (w_row + n * 32 >= bl.rows) continue;  // no rows: nobody joins them
         const int row = (wave * NB + n) * 32 + col;
         const float sum = pair_sum(l[n]);
         if (half == 0) d.w.stat[(size_t)slot * kRows + row] = make_float2(m[n], sum);
@@ -652,50 +732,41 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_tiles(ChunkArgs d) {
     }
   };
 
-  if constexpr (!RUNS) {
+  if constexpr (!CUT) {
     const int g = (int)(blockIdx.x % (unsigned)a.cache.kv_heads);
     Block bl;
     if (!find_block(a, (int)(blockIdx.x / (unsigned)a.cache.kv_heads), kRows, d.group, &bl)) return;
     attend(bl, g, 0, bl.tiles, -1);
   } else {
-    make_plan<WAVES * 64>(d, kRows, plan);
-    const int blocks = __builtin_amdgcn_readfirstlane(plan.blocks);
-    const int64_t extent = uniform64(plan.begin[blocks]), all = extent * a.cache.kv_heads;
-    const int64_t per = max((int64_t)1, (all + kRuns - 1) / kRuns);
-    // workgroups go to the XCDs in turn: an XCD's runs lie next to one another, mostly of one key/value head
-    const int run = (int)(blockIdx.x % 8) * (kRuns / 8) + (int)blockIdx.x / 8;
-    if (blockIdx.x == 0) {  // for the joining
-      for (int b = tid; b <= blocks; b += WAVES * 64) {
-        d.w.begin[b] = plan.begin[b];
-        if (b < blocks) d.w.seq[b] = plan.seq[b], d.w.in[b] = plan.in[b];
+    const int blocks = __builtin_amdgcn_readfirstlane(make_plan<WAVES * 64>(d, kRows, card_groups(D), plan));
+    const int slots = __builtin_amdgcn_readfirstlane((int)plan.slot[blocks]);
+    if (blockIdx.x == 0) {
+      if (tid == 0) d.w.head[0] = plan.cuts[blocks], d.w.head[1] = slots;
+      for (int b = tid; b < blocks; b += WAVES * 64) {
+        const int s = plan.seq[b], pieces = plan.slot[b + 1] - plan.slot[b];
+        if (pieces > 0) d.w.join[plan.cuts[b]] = JoinBlock{plan.q0[s], plan.nq[s] * d.group, plan.in[b] * kRows, pieces, plan.slot[b], {}};
       }
-      if (tid == 0) d.w.head[0] = blocks, d.w.head[1] = extent, d.w.head[2] = per;
     }
-    const int64_t from = run * per, to = min(from + per, all);
-    if (from >= to) return;
-    int g = (int)(from / extent), b = 0;
-    int64_t at = from - g * extent, left = to - from;
-    for (int hi = blocks - 1; b < hi;) {  // the last block that begins at or before `at`
+    // the last pieces first: those of a sequence's last queries
+    const int g = (int)(blockIdx.x % (unsigned)a.cache.kv_heads);
+    const int at = __builtin_amdgcn_readfirstlane((int)plan.begin[blocks]) - 1 - (int)(blockIdx.x / (unsigned)a.cache.kv_heads);
+    if (at < 0) return;
+    int b = 0;
+    for (int hi = blocks - 1; b < hi;) {  // the last block that begins at or before `at` (each has a piece)
       const int mid = (b + hi + 1) / 2;
-      if (uniform64(plan.begin[mid]) <= at) b = mid;
+      if (__builtin_amdgcn_readfirstlane((int)plan.begin[mid]) <= at) b = mid;
       else hi = mid - 1;
     }
-    for (bool first = true; left > 0; first = false) {
-      const int64_t begin = uniform64(plan.begin[b]), end = uniform64(plan.begin[b + 1]), upto = min(end, at + left);
-      if (end > begin) {
-        const Block bl = block_of(a, queries_of(a, __builtin_amdgcn_readfirstlane((int)plan.seq[b])),
-                                  __builtin_amdgcn_readfirstlane((int)plan.in[b]), kRows, d.group);
-        const int t0 = (int)max(at - begin - kBlockCost, (int64_t)0), t1 = (int)(upto - begin - kBlockCost);
-        if (t1 > t0) attend(bl, g, t0, t1, t0 == 0 && t1 == bl.tiles ? -1 : run + (first ? 0 : kRuns));
-      }
-      left -= upto - at;
-      at = upto;
-      if (++b == blocks) b = 0, g++, at = 0;
-    }
+    const int begin = __builtin_amdgcn_readfirstlane((int)plan.begin[b]), n = __builtin_amdgcn_readfirstlane((int)plan.begin[b + 1]) - begin, i = at - begin;
+    const int s = __builtin_amdgcn_readfirstlane((int)plan.seq[b]);
+    const Queries q{s, __builtin_amdgcn_readfirstlane(plan.q0[s]), __builtin_amdgcn_readfirstlane(plan.nq[s]), __builtin_amdgcn_readfirstlane(plan.len[s])};
+    const Block bl = block_of(a, q, __builtin_amdgcn_readfirstlane((int)plan.in[b]), kRows, d.group);
+    attend(bl, g, (int)((int64_t)bl.tiles * i / n), (int)((int64_t)bl.tiles * (i + 1) / n),
+           n == 1 ? -1 : g * slots + __builtin_amdgcn_readfirstlane((int)plan.slot[b]) + i);
   }
 }
 
-// Joins the parts of 32 rows of a block: a wave for each 32 columns. Blocks that see nothing become zero.
+// Joins the parts of 32 rows of a block that was cut: a wave for each 32 columns.
 template <int DT, int D>
 __global__ __launch_bounds__(D * 2) void k_gqa_join_tiles(ChunkArgs d, int size) {
   constexpr int VB = D / 32;
@@ -703,27 +774,21 @@ __global__ __launch_bounds__(D * 2) void k_gqa_join_tiles(ChunkArgs d, int size)
   const int lane = (int)threadIdx.x & 63, c = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int subs = size / 32, sub = (int)blockIdx.x % subs, item = (int)blockIdx.x / subs;
-  const int blocks = (int)d.w.head[0];
-  const int64_t extent = d.w.head[1], per = d.w.head[2];
-  const int g = item / max(blocks, 1), b = item - g * blocks;
-  if (blocks == 0 || g >= a.cache.kv_heads) return;
-  const Queries q = queries_of(a, d.w.seq[b]);
-  const int row0 = d.w.in[b] * size + sub * 32, rows = q.nq * d.group;
-  if (row0 >= rows) return;
-  const int64_t lo = g * extent + d.w.begin[b], hi = g * extent + d.w.begin[b + 1];
-  const int w0 = (int)((lo + kBlockCost) / per), parts = hi > lo ? (int)((hi - 1) / per) - w0 + 1 : 0;
-  if (parts == 1) return;
-  const bool late = w0 * per < lo;
-  auto slot = [&](int j) { return (size_t)(w0 + j + (j == 0 && late ? kRuns : 0)); };
+  const int b = item / a.cache.kv_heads, g = item - b * a.cache.kv_heads;  // (b is less than the workgroups on the card)
+  const JoinBlock k = d.w.join[b];
+  const int row0 = k.row0 + sub * 32;
+  if (b >= d.w.head[0] || row0 >= k.rows) return;
+  const size_t first = (size_t)g * d.w.head[1] + k.slot;
   const float scale = exponent_scale(a.scale);
   float m = -__builtin_huge_valf(), l = 0.0f;
-  for (int j = 0; j < parts; j++) m = fmaxf(m, d.w.stat[slot(j) * size + sub * 32 + col].x);
+  for (int j = 0; j < k.pieces; j++) m = fmaxf(m, d.w.stat[(first + j) * size + sub * 32 + col].x);
   const float ref = m == -__builtin_huge_valf() ? 0.0f : m;
   float o[16] = {};
-  for (int j = 0; j < parts; j++) {
-    const float2 st = d.w.stat[slot(j) * size + sub * 32 + col];
+#pragma unroll 2
+  for (int j = 0; j < k.pieces; j++) {
+    const float2 st = d.w.stat[(first + j) * size + sub * 32 + col];
     const float f = __builtin_amdgcn_exp2f((st.x - ref) * scale);
-    const float4* p = (const float4*)(d.w.part + slot(j) * size * D) + ((sub * VB + c) * 4) * 64 + lane;
+    const float4* p = (const float4*)(d.w.part + (first + j) * size * D) + ((sub * VB + c) * 4) * 64 + lane;
     float4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = p[i * 64];
@@ -737,10 +802,10 @@ __global__ __launch_bounds__(D * 2) void k_gqa_join_tiles(ChunkArgs d, int size)
     }
   }
   const int r = row0 + col;
-  if (r >= rows) return;
+  if (r >= k.rows) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int qi = r / d.group;
-  uint16_t* out = (uint16_t*)a.out + (int64_t)(q.q0 + qi) * a.out_token_stride + (int64_t)(g * d.group + r - qi * d.group) * a.out_head_stride;
+  uint16_t* out = (uint16_t*)a.out + (int64_t)(k.q0 + qi) * a.out_token_stride + (int64_t)(g * d.group + r - qi * d.group) * a.out_head_stride;
 #pragma unroll
   for (int i = 0; i < 4; i++)
     *(uint2*)(out + 32 * c + 8 * i + 4 * half) =
@@ -763,11 +828,16 @@ int launch_chunk(const ChunkArgs& d, hipStream_t st) {
   const int64_t seqs = a.cache.num_seqs < a.q_tokens ? a.cache.num_seqs : a.q_tokens;
   const int64_t blocks = ((int64_t)a.q_tokens * d.group + (S::rows - 1) * seqs) / S::rows, items = blocks * a.cache.kv_heads;
   if (items > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
-  if (items >= 4 * kRuns || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
+  constexpr int kGroups = card_groups(D);
+  // Whole blocks where they fill the card some times over, or twice if none can be long: planning and the second launch cost 8 us (4096
+  // tokens of 32 heads over 8: 171 us, without 163), but one long block beside 500 short ones would have the card wait for it.
+  int64_t longest = (int64_t)a.cache.max_pages * a.cache.page_size;
+  if (a.window > 0 && (int64_t)a.window + a.sinks + S::rows / d.group < longest) longest = (int64_t)a.window + a.sinks + S::rows / d.group;
+  if (items >= (longest <= 96 * kTile ? 2 : 4) * kGroups || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
     hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false, WHOLE>), dim3((unsigned)items), dim3(S::waves * 64), 0, st, d);
-  } else {
-    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true, WHOLE>), dim3(kRuns), dim3(S::waves * 64), 0, st, d);
-    hipLaunchKernelGGL((k_gqa_join_tiles<DT, D>), dim3((unsigned)(items * (S::rows / 32))), dim3(D * 2), 0, st, d, S::rows);
+  } else {  // (pieces of at least an even share: no more than blocks and shares)
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true, WHOLE>), dim3((unsigned)items + kGroups), dim3(S::waves * 64), 0, st, d);
+    hipLaunchKernelGGL((k_gqa_join_tiles<DT, D>), dim3((unsigned)(items < kGroups ? items : kGroups) * (S::rows / 32)), dim3(D * 2), 0, st, d, S::rows);
   }
   VIB3_RETURN_LAUNCH();
 }
