@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "gqa.h"
+#include "scan.h"
 
 namespace vib3 {
 namespace {
@@ -197,23 +198,6 @@ struct Plan {
   int16_t slot[kMaxBlocks + 1];            // pieces of cut blocks before each
   int16_t cuts[kMaxBlocks + 1];            // cut blocks before each
 };
-
-// v of lane l combined with those of the lanes below, by `f`; `none` does nothing there. Lane 63 has all.
-template <typename T, typename F>
-__device__ __forceinline__ T wave_scan(T v, T none, F f) {
-  const int o = __builtin_bit_cast(int, none);
-  auto step = [&](int moved) { v = f(v, __builtin_bit_cast(T, moved)); };
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x111, 0xf, 0xf, false));  // from the lane below in a row of 16
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x112, 0xf, 0xf, false));  // 2 below
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x114, 0xf, 0xf, false));
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x118, 0xf, 0xf, false));
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false));  // lane 15's to the second row, 47's to the last
-  step(__builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false));  // lane 31's to the upper half
-  return v;
-}
-__device__ __forceinline__ int add_up(int v) {
-  return wave_scan(v, 0, [](int a, int b) { return a + b; });
-}
 
 // Sum of v over the threads before this one (THREADS of them); *all: over all of them. A barrier; calls take turns with `sums`.
 template <int THREADS>
@@ -761,7 +745,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
     const int s = __builtin_amdgcn_readfirstlane((int)plan.seq[b]);
     const Queries q{s, __builtin_amdgcn_readfirstlane(plan.q0[s]), __builtin_amdgcn_readfirstlane(plan.nq[s]), __builtin_amdgcn_readfirstlane(plan.len[s])};
     const Block bl = block_of(a, q, __builtin_amdgcn_readfirstlane((int)plan.in[b]), kRows, d.group);
-    attend(bl, g, (int)((int64_t)bl.tiles * i / n), (int)((int64_t)bl.tiles * (i + 1) / n),
+    const int each = bl.tiles / n, over = bl.tiles - each * n;
+    attend(bl, g, each * i + min(i, over), each * (i + 1) + min(i + 1, over),
            n == 1 ? -1 : g * slots + __builtin_amdgcn_readfirstlane((int)plan.slot[b]) + i);
   }
 }

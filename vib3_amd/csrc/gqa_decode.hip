@@ -5,29 +5,32 @@
 //   k_gqa_attend   the attention, over equal shares of all rows' visible tokens
 //   k_gqa_join     rows that several shares were needed for
 //
-// The shares: tokens are taken 32 at a time (a unit). All units of all rows in order, with kRowCost units' time in front of each row
+// The shares: tokens are taken 32 at a time, 64 for heads of 64 (a unit). All units of all rows in order, with kRowCost units' time in front of each row
 // for taking it up and storing its sums, are cut into equal runs, whatever the rows' lengths. A run is walked by one wave per
 // key/value head (and per 16 heads of its group), all by themselves: there is no barrier after the plan, which every workgroup
 // forms anew from the lengths (a scan of an int a row). Nothing on the host depends on the lengths, so a captured launch follows
 // them.
 //
 // A wave holds the keys of a unit as it gets them from memory, as the matrix cores' A operand (S^T = K . Q^T, the group's heads are
-// the columns), so that a lane has the scores of 8 tokens and one head; packed in pairs of 16 bits they are, as they stand, the B
+// the columns), so that a lane has the scores of 8 of 32 tokens and one head; packed in pairs of 16 bits they are, as they stand, the B
 // operand of O^T = V^T . P^T (the tokens' order along k is free as long as V^T is read in the same one). Values pass through the
-// wave's own 32 rows of LDS, from where transposing reads take V^T. The next unit's keys and values are on their way
+// wave's own rows of LDS, from where transposing reads take V^T. The next unit's keys and values are on their way
 // meanwhile, and the page numbers of the one after that.
+#include <type_traits>
+
 #include "gqa.h"
+#include "scan.h"
 
 namespace vib3 {
 namespace {  // the names below are this file's: other files have a decode_ws or a launch_decode_dt of their own
 
 constexpr int kGqaMaxRows = 65536;
-constexpr int kUnit = 32;     // tokens of one step
 constexpr int kRowCost = 2;   // a row's fixed time, in units
 constexpr int kWorkgroups = 256;
 
-// Waves of a workgroup: as many as their registers leave room for.
-__host__ __device__ constexpr int attend_waves(int dim) { return dim == 64 ? 16 : dim == 128 ? 8 : 4; }
+// Tokens of one step, and waves of a workgroup: as many as their registers leave room for.
+__host__ __device__ constexpr int unit_tokens(int dim) { return dim == 64 ? 64 : 32; }
+__host__ __device__ constexpr int attend_waves(int dim) { return dim == 256 ? 4 : 8; }
 
 // What a wave takes of the heads: 16 of a group at most.
 struct Heads {
@@ -79,41 +82,43 @@ struct DecodeArgs {
   vib3_gqa_decode a;
   DecodeWs w;
   Heads h;
+  Divisor page;
   int runs;
 };
 
+// a / b (exact below 2^42 where it is below 2^11: the quotient's distance from the next integer is more than its rounding).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
+
 // What the query of a row sees, in units: `skip` units from the first token on (those with sinks), then from unit `first` to the end.
+template <int UNIT>
 struct Seen {
   int seq, len, start;        // visible are the tokens from start and the first sinks, to len
   int skip, first, units;
-  __device__ __forceinline__ int token(int u) const { return (u < skip ? u : first + u - skip) * kUnit; }
+  __device__ __forceinline__ int token(int u) const { return (u < skip ? u : first + u - skip) * UNIT; }
 };
 
-__device__ __forceinline__ Seen row_seen(const vib3_gqa_decode& a, int r) {
-  Seen s;
+template <int UNIT>
+__device__ __forceinline__ Seen<UNIT> row_seen(const vib3_gqa_decode& a, int r) {
+  Seen<UNIT> s;
   s.seq = a.seqs ? a.seqs[r] : r;
   s.len = (unsigned)s.seq < (unsigned)a.cache.num_seqs ? gqa_len(a.cache, a.lens[r]) : 0;
   s.start = s.len > 0 ? window_start(s.len - 1, a.window) : 0;
-  s.first = s.start / kUnit;
-  s.skip = min((min(a.sinks, s.start) + kUnit - 1) / kUnit, s.first);
-  s.units = (s.len + kUnit - 1) / kUnit - s.first + s.skip;
+  s.first = s.start / UNIT;
+  s.skip = min((min(a.sinks, s.start) + UNIT - 1) / UNIT, s.first);
+  s.units = (s.len + UNIT - 1) / UNIT - s.first + s.skip;
   return s;
 }
 
 // A row's extent in the order of all: a row that sees nothing has none.
+template <int UNIT>
 __device__ __forceinline__ int64_t row_extent(const vib3_gqa_decode& a, int r) {
-  const int n = r < a.rows ? row_seen(a, r).units : 0;
+  const int n = r < a.rows ? row_seen<UNIT>(a, r).units : 0;
   return n > 0 ? n + kRowCost : 0;
 }
 
-// Sum over the lanes up to this one.
+// Sum over the lanes up to this one (of values from 0 to 2^40).
 __device__ __forceinline__ int64_t scan64(int64_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t up = __shfl_up(v, d);
-    if (lane_id() >= d) v += up;
-  }
-  return v;
+  return ((int64_t)add_up((int)(v >> 16)) << 16) + add_up((int)(v & 0xffff));
 }
 
 // v of lane i (the same in all lanes), as a value that is known to be uniform.
@@ -149,7 +154,8 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
   constexpr int WAVES = attend_waves(D);
   constexpr int KS = D / 32;  // k steps of the scores
   constexpr int VB = D / 16;  // 16-row blocks of the sums
-  __shared__ __align__(1024) uint8_t vtile[WAVES][kUnit * D * 2];
+  constexpr int UNIT = unit_tokens(D), TB = UNIT / 16;  // 16-token blocks of a step
+  __shared__ __align__(1024) uint8_t vtile[WAVES][UNIT * D * 2];
   __shared__ int64_t group_sum[kGqaMaxRows / 64];
   const vib3_gqa_decode& a = d.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
   // the plan: extents of 64 rows at a time, then their sum and where this wave's run begins
   const int row_groups = (a.rows + 63) / 64;
   for (int k = wave; k < row_groups; k += WAVES) {
-    const int64_t n = scan64(row_extent(a, 64 * k + lane));
+    const int64_t n = scan64(row_extent<UNIT>(a, 64 * k + lane));
     if (lane == 63) group_sum[k] = n;
   }
   __syncthreads();
@@ -168,12 +174,12 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
     if (planner)
       for (int i = wave; i < 64 && k + i < row_groups; i += WAVES) {
         const int r = 64 * (k + i) + lane;
-        const int64_t x = row_extent(a, r), at = uniform64(upto - n, i) + scan64(x) - x;
+        const int64_t x = row_extent<UNIT>(a, r), at = uniform64(upto - n, i) + scan64(x) - x;
         if (r < a.rows) d.w.begin[r] = at;
       }
     all = uniform64(upto, 63);
   }
-  const int64_t per = max((int64_t)1, (all + d.runs - 1) / d.runs);
+  const int64_t per = max((int64_t)1, quotient(all + d.runs - 1, d.runs));
   if (planner) {
     if (tid == 0) {
       d.w.begin[a.rows] = all;
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
     if (hit) {
       const int i = __ffsll((unsigned long long)hit) - 1;
       begin = uniform64(upto - n, i);
-      const int64_t x = row_extent(a, 64 * (k + i) + lane), end = scan64(x) + begin;
+      const int64_t x = row_extent<UNIT>(a, 64 * (k + i) + lane), end = scan64(x) + begin;
       const int j = __ffsll((unsigned long long)__ballot(from < end)) - 1;
       begin = uniform64(end - x, j);
       row = 64 * (k + i) + j;
@@ -212,12 +218,12 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
   const uint64_t zbase = (uint64_t)zero_token + 16 * g;
 
   // The stream of units, two steps ahead of the products: page numbers, then addresses and loads.
-  Seen ahead = row_seen(a, row);  // the row of the unit that page numbers are asked for next
+  Seen<UNIT> ahead = row_seen<UNIT>(a, row);  // the row of the unit that page numbers are asked for next
   int ahead_row = row;
   int64_t ahead_begin = begin;
   int ahead_u = (int)max((int64_t)0, from - begin - kRowCost);
   int ahead_end = (int)min((int64_t)ahead.units, to - begin - kRowCost);
-  int page_no[2], place[2];  // of this lane's two tokens; place -1: not seen
+  int page_no[TB], place[TB];  // of this lane's tokens; place -1: not seen
   bool more = true;          // whether the unit that was asked for is one of the run
   auto ask = [&] {
     while (ahead_u >= ahead_end) {  // the next row
@@ -225,32 +231,34 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
       ahead_row++;
       if (ahead_begin + kRowCost >= to) {
         more = false;
-        place[0] = place[1] = -1;
+#pragma unroll
+        for (int b = 0; b < TB; b++) place[b] = -1;
         return;
       }
-      ahead = row_seen(a, ahead_row);
+      ahead = row_seen<UNIT>(a, ahead_row);
       ahead_u = 0;
       ahead_end = (int)min((int64_t)ahead.units, to - ahead_begin - kRowCost);
     }
     const int t0 = ahead.token(ahead_u) + col;
     const int32_t* table = a.cache.block_table + (size_t)ahead.seq * a.cache.max_pages;
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < TB; b++) {
       const int t = t0 + 16 * b;
       const bool ok = t < ahead.len && (t >= ahead.start || t < a.sinks);
-      const int page = ok ? t / a.cache.page_size : 0;
+      const int page = ok ? d.page.of(t) : 0;
       place[b] = ok ? t - page * a.cache.page_size : -1;
       page_no[b] = ld_global4(table + page);
     }
     ahead_u++;
   };
+  using Mask = std::conditional_t<TB == 4, uint64_t, uint32_t>;
   // Loads of the unit that was asked for: this lane's chunks g + 4 c of its two tokens. Returns the mask of the tokens that are seen.
-  auto load = [&](s16x8 (*k)[KS], s16x8 (*v)[KS]) -> uint32_t {
-    uint32_t mask = 0;
+  auto load = [&](s16x8 (*k)[KS], s16x8 (*v)[KS]) -> Mask {
+    Mask mask = 0;
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < TB; b++) {
       const bool ok = place[b] >= 0 && (unsigned)page_no[b] < (unsigned)a.cache.num_pages;
-      mask |= ((uint32_t)__ballot(ok) & 0xffff) << (16 * b);
+      mask |= (Mask)(__ballot(ok) & 0xffff) << (16 * b);
       const uint64_t at = 2 * ((int64_t)page_no[b] * a.cache.page_stride + (int64_t)place[b] * a.cache.token_stride);
       const uint64_t ka = ok ? kbase + at : zbase, va = ok ? vbase + at : zbase;
 #pragma unroll
@@ -270,12 +278,12 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
   lds_u8* const get = tile + vrow * D * 2 + 8 * (col & 1);
   const int get0 = (((col & 3) >> 1) ^ swizzle(vrow)) * 16;
 
-  Seen at = ahead;
+  Seen<UNIT> at = ahead;
   int u = ahead_u, end = ahead_end;
   ask();
   if (!more) return;
-  s16x8 k[2][2][KS], v[2][2][KS];
-  uint32_t mask[2];
+  s16x8 k[2][TB][KS], v[2][TB][KS];
+  Mask mask[2];
   mask[0] = load(k[0], v[0]);
   ask();
   bool first_row = true;
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
       row++;
       first_row = false;
       if (begin + kRowCost >= to) return;
-      at = row_seen(a, row);
+      at = row_seen<UNIT>(a, row);
       u = 0;
       end = (int)min((int64_t)at.units, to - begin - kRowCost);
     }
@@ -303,28 +311,30 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
     }
     f32x4 o[VB] = {};
     float m = -__builtin_huge_valf(), l = 0.0f;  // of this lane's head (unscaled scores); l over this lane's own tokens
-    auto step = [&](s16x8 (*kc)[KS], s16x8 (*vc)[KS], uint32_t seen, s16x8 (*kn)[KS], s16x8 (*vn)[KS], uint32_t* next) {
+    auto step = [&](s16x8 (*kc)[KS], s16x8 (*vc)[KS], Mask seen, s16x8 (*kn)[KS], s16x8 (*vn)[KS], Mask* next) {
       if (more) {
         *next = load(kn, vn);
         ask();
       }
-      f32x4 s[2] = {};
+      f32x4 s[TB] = {};
 #pragma unroll
       for (int c = 0; c < KS; c++)
 #pragma unroll
-        for (int b = 0; b < 2; b++) s[b] = mma32<DT>(kc[b][c], q[c], s[b]);
+        for (int b = 0; b < TB; b++) s[b] = mma32<DT>(kc[b][c], q[c], s[b]);
 #pragma unroll
-      for (int b = 0; b < 2; b++)
+      for (int b = 0; b < TB; b++)
 #pragma unroll
         for (int c = 0; c < KS; c++) *(__attribute__((address_space(3))) s16x8*)(put + 16 * b * D * 2 + (put0 ^ 64 * c)) = vc[b][c];
-      if (seen != 0xffffffffu) {
+      if (seen != (Mask)~(Mask)0) {
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int b = 0; b < TB; b++)
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (!(seen >> (16 * b + 4 * g + i) & 1)) s[b][i] = -__builtin_huge_valf();
       }
-      float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      float top = s[0][0];
+#pragma unroll
+      for (int b = 0; b < TB; b++) top = fmaxf(top, fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
       top = max_over_rows(top);
       // The reference value of a head's exponentials follows its maximum only where that grew by more than kLag.
       const bool grown = (top - m) * scale > kLag<DT> || (m == -__builtin_huge_valf() && top > m);
@@ -341,12 +351,12 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
         const float off = far ? m : 0.0f;
         base = far ? 0.0f : base;
 #pragma unroll
-        for (int b = 0; b < 2; b++) s[b] -= off;
+        for (int b = 0; b < TB; b++) s[b] -= off;
       }
       base -= kProbShift<DT>;
-      uint32_t p[4];
+      uint32_t p[2 * TB];
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
+      for (int b = 0; b < TB; b++) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -base));
@@ -355,15 +365,19 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
         p[2 * b] = pack2<DT>(e[0], e[1]);
         p[2 * b + 1] = pack2<DT>(e[2], e[3]);
       }
-      const s16x8 prob = __builtin_bit_cast(s16x8, make_uint4(p[0], p[1], p[2], p[3]));
 #pragma unroll
-      for (int b = 0; b < VB; b++)
-        o[b] = mma32<DT>(join(lds_read_tr(get + (get0 ^ 32 * b)), lds_read_tr(get + 16 * D * 2 + (get0 ^ 32 * b))), prob, o[b]);
+      for (int t = 0; t < TB; t += 2) {
+        const s16x8 prob = __builtin_bit_cast(s16x8, make_uint4(p[2 * t], p[2 * t + 1], p[2 * t + 2], p[2 * t + 3]));
+        lds_u8* const x = get + 16 * t * D * 2;
+#pragma unroll
+        for (int b = 0; b < VB; b++)
+          o[b] = mma32<DT>(join(lds_read_tr(x + (get0 ^ 32 * b)), lds_read_tr(x + 16 * D * 2 + (get0 ^ 32 * b))), prob, o[b]);
+      }
     };
     for (; u < end; u++) {
       step(k[0], v[0], mask[0], k[1], v[1], &mask[1]);
 #pragma unroll
-      for (int b = 0; b < 2; b++)
+      for (int b = 0; b < TB; b++)
 #pragma unroll
         for (int c = 0; c < KS; c++) {
           k[0][b][c] = k[1][b][c];
@@ -392,24 +406,24 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
 
 // ------------------------------------------------------------------------- joined rows
 
-// `team` waves (1, 2, 4, 8 or 16) of a workgroup of 16 join the parts of one (row, head); rows that see nothing become zero.
-template <int DT, int D>
-__global__ __launch_bounds__(1024) void k_gqa_join(DecodeArgs d, int team) {
+// `team` waves (1, 2, 4, 8 or 16) of a workgroup of WAVES join the parts of one (row, head); rows that see nothing become zero.
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team) {
   constexpr int E = D / 64;  // columns of a lane
   constexpr int kAhead = 4;  // parts in flight
-  __shared__ float sums[16][D];
-  __shared__ float tops[16], totals[16];
+  __shared__ float sums[WAVES][D];
+  __shared__ float tops[WAVES], totals[WAVES];
   const vib3_gqa_decode& a = d.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t x = (int64_t)blockIdx.x * (16 / team) + wave / team;
+  const int x = (int)blockIdx.x * (WAVES / team) + wave / team;
   const int mate = wave % team;
-  const int r = (int)(x / a.heads), h = (int)(x - (int64_t)r * a.heads);
+  const int r = x / a.heads, h = x - r * a.heads;
   int parts = 1;
   float m = -__builtin_huge_valf(), l = 0.0f, o[E] = {};
   if (r < a.rows) {
     const int64_t per = *d.w.head, lo = d.w.begin[r], hi = d.w.begin[r + 1];
-    const int w0 = (int)((lo + kRowCost) / per);
-    parts = hi > lo ? (int)((hi - 1) / per) - w0 + 1 : 0;
+    const int w0 = (int)quotient(lo + kRowCost, per);
+    parts = hi > lo ? (int)quotient(hi - 1, per) - w0 + 1 : 0;
     if (parts > 1) {
       const int kv_head = h / d.h.group, in_group = h - kv_head * d.h.group;
       const int hu = kv_head * d.h.parts + in_group / 16, col = in_group % 16;
@@ -490,7 +504,8 @@ int launch_decode(const DecodeArgs& d, hipStream_t st) {
   const int64_t items = (int64_t)d.a.rows * d.a.heads;
   int team = 16;
   while (team > 1 && items * team > 8192) team /= 2;  // 16 waves a CU twice over
-  hipLaunchKernelGGL((k_gqa_join<DT, D>), dim3((unsigned)((items * team + 15) / 16)), dim3(1024), 0, st, d, team);
+  if (team > 4) hipLaunchKernelGGL((k_gqa_join<DT, D, 16>), dim3((unsigned)((items * team + 15) / 16)), dim3(1024), 0, st, d, team);
+  else hipLaunchKernelGGL((k_gqa_join<DT, D, 4>), dim3((unsigned)((items * team + 3) / 4)), dim3(256), 0, st, d, team);
   VIB3_RETURN_LAUNCH();
 }
 
@@ -527,6 +542,7 @@ extern "C" int vib3_launch_gqa_decode(const vib3_gqa_decode* args, void* stream)
   d.a = a;
   if (a.workspace_bytes < decode_ws(a, &d.w, a.workspace)) return VIB3_ERR_WORKSPACE;
   d.h = split_heads(a.heads, a.cache.kv_heads);
+  d.page = divisor(a.cache.page_size);
   d.runs = run_count(d.h, a.cache.dim);
   return a.cache.dtype == VIB3_DT_F16 ? launch_decode_dt<VIB3_DT_F16>(d, (hipStream_t)stream)
                                       : launch_decode_dt<VIB3_DT_BF16>(d, (hipStream_t)stream);
