@@ -2,7 +2,11 @@
 //
 // A workgroup takes one token: its rows are the heads of q, k and v, one after the other, and D / 16 lanes share a row, 16 elements
 // each, which are 8 pairs of the rotation. The cosines and sines are formed once a token (the angle and its reduction in 64 bits:
-// positions reach 10^6 radians, where f32 angles are off by 0.03) while the first rows are on their way.
+// positions reach 10^6 radians, where f32 angles are off by 0.03) while the first rows are on their way; a row's successor is loaded before
+// the row is stored.
+//
+// Bound by HBM for prompts (6007 tokens of 40 + 8 + 8 heads of 128 from f32: 258 MB in 57 us, 4.5 TB/s; a copy of 2 GB 5.0), by the launch and
+// its chain of reads (sequence, page number, row) for single tokens (5 us).
 #include "gqa.h"
 
 namespace vib3 {

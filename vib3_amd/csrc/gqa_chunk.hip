@@ -18,6 +18,11 @@
 // causal mask's unequal blocks and long caches under few queries need alike; a piece's sums go to the workspace as they lie in
 // registers, and a second launch joins them. How long a piece is follows from the lengths alone, which every workgroup reads for
 // itself, so a captured launch follows them.
+//
+// Measured: 12288 tokens of 32 heads over 8 of 128: 1.24 ms, 994 TFLOP/s (a library product of 8192^3: 1223, held down by the card's power),
+// 64 heads of 64 1.51 ms, 16 over 2 of 256 1.78 ms. The matrix cores are busy for 39 % of the cycles and the vector units for 55 %, and
+// the two add up: products and softmax of one wave interleaved by hand, sums a tile late, and 64 rows a wave were no faster (1.34 to 1.38
+// and, with spilled registers, 2.7 ms). 16 sequences' 4 drafted tokens of 16 heads over 2 of 256 after 317 to 5642: 36 us and 9 to join.
 #include <type_traits>
 
 #include "gqa.h"

@@ -16,6 +16,11 @@
 // operand of O^T = V^T . P^T (the tokens' order along k is free as long as V^T is read in the same one). Values pass through the
 // wave's own rows of LDS, from where transposing reads take V^T. The next unit's keys and values are on their way
 // meanwhile, and the page numbers of the one after that.
+//
+// Measured (attention + joining): 61 rows of 300 to 50000 tokens, 32 heads over 8 of 128: 430 + 7 us, 5.8 TB/s (a kernel that only reads gets
+// 6.0); one row of 901 tokens 9 + 5, launches and dependent reads (length, page number, tokens; place, parts). 97 rows of 64 heads over 8 of 64
+// with a window of 4096: 55 + 6; with 32 tokens a step and 16 waves 59 + 6, which spilled registers. Equal shares against a workgroup
+// per row and head: 440 us against 56 ms for the 61 rows.
 #include <type_traits>
 
 #include "gqa.h"
