@@ -273,7 +273,7 @@ __device__ int make_plan(const ChunkArgs& d, int size, int groups, Plan& p) {
     longest = max(longest, p.wave_longest[i]);
   }
   all_tiles *= (float)a.cache.kv_heads;
-  // The length of a piece: whole blocks, or an even share of the tiles, or more by a third or by half where the even share's pieces do not fit
+  // The length of a piece: whole blocks, an even share of the tiles, or a third more or twice that, where the even share's pieces do not fit
   // the card at a time: whichever takes least, of the longest piece, or of rounds of pieces over the card, and of the parts' time.
   // (An even share is rounded up, above what the sum of tiles lacks: the pieces of cut blocks are fewer than twice the workgroups.)
   const float even = all_tiles / (float)groups * 1.0001f;

@@ -366,7 +366,8 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
 #pragma unroll
         for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -base));
         l += (e[0] + e[1]) + (e[2] + e[3]);
-        // rounded for the matrix cores; the sum l takes them unrounded
+        // rounded for the matrix cores (bf16: 0.0023 relative to 64 bits instead of 0.0017); the sum l takes them unrounded. (Remainders as
+        // a second operand would mend that, but are 0 or negative too, and times an infinity that is seen NaN.)
         p[2 * b] = pack2<DT>(e[0], e[1]);
         p[2 * b + 1] = pack2<DT>(e[2], e[3]);
       }
