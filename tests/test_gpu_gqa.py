@@ -592,6 +592,48 @@ def test_chunk_repeats_bit_for_bit_and_alone():
 # ------------------------------------------------------------------------------- together
 
 
+@pytest.mark.parametrize("ps", [2, 3, 1000, 4097, 65535, 65536])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_page_sizes(ps, dim):
+    lens = [min(3 * ps // 2, 3000 + ps) + 7, 5, 2 * ps if ps > 1000 else 0]
+    c = Paged(lens, 2, dim, F16, ps, spare=1)
+    rows = [(s, n) for s in range(3) for n in (lens[s], lens[s] - 1, min(lens[s], ps), min(lens[s], ps + 1))]
+    check_decode(c, *decode(c, 6, rows), rows)
+    check_decode(c, *decode(c, 6, rows, window=100, sinks=3), rows, window=100, sinks=3)
+    nq = [min(n, 9) for n in lens]
+    check_chunk(c, *chunk(c, 6, nq), nq)
+
+
+def test_longest_sequence():
+    """2^31 - 2^12 tokens, the most that count: a table whose entries all name page 0, but for the last one. Keys are 0 but for token 777
+    of page 0 (score 24) and the last token (score 50), whose values are the only ones that are not 0: what the others have in the sums is
+    below 2^16 e^-24 and 2^31 e^-26, less than half a step."""
+    from vib3_amd import gqa
+    ps, most = 65536, 2 ** 31 - 2 ** 12
+    k, v = (torch.zeros(2, ps, 1, 64, dtype=F16, device="cuda") for _ in range(2))
+    last = (most - 1) % ps
+    k[0, 777], k[1, last] = 24 / 64, 50 / 64
+    v[0, 777], v[1, last] = rnd(1, 64, dtype=F16, seed=1), rnd(1, 64, dtype=F16, seed=2)
+    first, second = v[0, 777, 0].float(), v[1, last, 0].float()
+    c = gqa.GqaCache(k, v)
+    table = ints([[0] * 32767 + [1]])
+    q = torch.ones(6, 2, 64, dtype=F16, device="cuda")
+    zero = torch.zeros_like(first)
+
+    def check(got, want):
+        assert bool(((got.float() - torch.stack(want)[:, None]).abs() <= 2 * R.half_step(F16) * torch.stack(want)[:, None].abs()).all())
+    op = gqa.GqaDecode(c, 2, 6)
+    lens = ints([2 ** 31 - 1, most, most - 1, 3 * ps + 778, 3 * ps, 777])
+    check(op.launch(q, table, lens, 1.0, seqs=ints([0] * 6)), [second, second, first, first, first, zero])
+    for sinks, low in ((0, zero), (778, first), (777, zero)):
+        check(op.launch(q, table, lens, 1.0, seqs=ints([0] * 6), window=4096, sinks=sinks),
+              [second, second, low, first, zero if sinks < 778 else first, zero])
+    op = gqa.GqaChunk(c, 2, 6, 1)
+    check(op.launch(q[:3], table, ints([0, 3]), ints([most]), 1.0), [first, first, second])
+    check(op.launch(q[:3], table, ints([0, 3]), ints([2 ** 31 - 1]), 1.0, window=4096, sinks=0), [zero, zero, second])
+    check(op.launch(q[:3], table, ints([0, 3]), ints([most - 1]), 1.0, window=4096, sinks=778), [first, first, first])
+
+
 def test_host_refusals():
     from vib3_amd import gqa
     k = torch.zeros(4, 16, 2, 128, dtype=BF16, device="cuda")

@@ -182,6 +182,22 @@ def test_compact_many_pages():
                                        torch.zeros(n + 1, 1, 1, 64, dtype=torch.half, device="cuda"))])
 
 
+@pytest.mark.parametrize("ps", [65535, 65536])
+@pytest.mark.parametrize("kinds", [["heads"], ["wide", "mla"]])
+def test_largest_pages(kinds, ps):
+    from vib3_amd import pages as P
+    caches, pools = make_caches(kinds, 6, ps, seed=ps)
+    table, lens = [[5, 2, -1], [-1, -1, -1], [4, -1, -1]], [ps + 12345, 0, ps]
+    dev, want = ints(table), bits(pools)
+    fork_host(table, lens, [0], [1], [3], want, ps, 3)
+    P.fork_pages(caches, dev, ints(lens), ints([0]), ints([1]), ints([3]))
+    lens[1] = lens[0]
+    assert dev.tolist() == table and all(same(a, b) for a, b in zip(pools, want))
+    live, moved = compact_host(table, lens, want, ps, 6)
+    assert P.PageCompaction(caches).launch(dev, ints(lens)).tolist() == [live] and dev.tolist() == moved
+    assert all(same(a, b) for a, b in zip(pools, want))
+
+
 def test_host_refusals():
     from vib3_amd import pages as P
     (a,), _ = make_caches(["tokens"], 4, 16)
