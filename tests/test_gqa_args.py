@@ -1,6 +1,8 @@
 """Refusals of the grouped-query attention and page launchers: every one returns its code before anything is launched, so they run
 without a GPU, on addresses that are never read."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 
@@ -192,3 +194,18 @@ def test_host_functions_refuse_cpu_tensors():
         pages.fork_pages([torch.zeros(2)], None, None, None, None, None)
     with pytest.raises(ValueError):
         pages.PageCompaction([])
+
+
+def test_descriptions_lie_as_the_header_says(tmp_path):
+    """Sizes and offsets of the ctypes descriptions against a C compiler's."""
+    pairs = {"vib3_gqa_cache": _lib.GqaCacheDesc, "vib3_gqa_append": _lib.GqaAppendDesc, "vib3_gqa_decode": _lib.GqaDecodeDesc,
+             "vib3_gqa_chunk": _lib.GqaChunkDesc, "vib3_page_pool": _lib.PagePoolDesc, "vib3_fork_pages": _lib.ForkPagesDesc,
+             "vib3_compact_pages": _lib.CompactPagesDesc}
+    lines = [f'printf("%zu %zu\\n", sizeof({name}), offsetof({name}, {f[0]}));' for name, d in pairs.items() for f in d._fields_]
+    source = tmp_path / "lay.c"
+    source.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"vib3_hip.h\"\nint main(void) {\n" + "\n".join(lines) + "\nreturn 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, "-o", str(tmp_path / "lay"), str(source)], check=True, capture_output=True)
+    out = subprocess.run([str(tmp_path / "lay")], check=True, capture_output=True, text=True).stdout.split("\n")
+    want = [f"{C.sizeof(d)} {getattr(d, f[0]).offset}" for d in pairs.values() for f in d._fields_]
+    assert out[:-1] == want

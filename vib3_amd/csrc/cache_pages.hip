@@ -24,6 +24,7 @@ struct Pool {
 struct Pools {
   Pool pool[kPools];
 };
+static_assert(sizeof(Pools) <= 3584, "4 KB of arguments a launch, with what else it takes");
 
 __host__ __device__ inline int64_t page_chunks(const vib3_page_pool& p, int page_size) {
   return (int64_t)p.runs * page_size * (p.token_bytes / 16);
