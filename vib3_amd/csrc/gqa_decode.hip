@@ -87,7 +87,6 @@ struct DecodeArgs {
   vib3_gqa_decode a;
   DecodeWs w;
   Heads h;
-  Divisor page;
   int runs;
 };
 
@@ -250,7 +249,7 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
     for (int b = 0; b < TB; b++) {
       const int t = t0 + 16 * b;
       const bool ok = t < ahead.len && (t >= ahead.start || t < a.sinks);
-      const int page = ok ? d.page.of(t) : 0;
+      const int page = ok ? t / a.cache.page_size : 0;  // (by multiplication heads of 64 and 128 gain 0.5 %, those of 256 lose 5)
       place[b] = ok ? t - page * a.cache.page_size : -1;
       page_no[b] = ld_global4(table + page);
     }
@@ -548,7 +547,6 @@ extern "C" int vib3_launch_gqa_decode(const vib3_gqa_decode* args, void* stream)
   d.a = a;
   if (a.workspace_bytes < decode_ws(a, &d.w, a.workspace)) return VIB3_ERR_WORKSPACE;
   d.h = split_heads(a.heads, a.cache.kv_heads);
-  d.page = divisor(a.cache.page_size);
   d.runs = run_count(d.h, a.cache.dim);
   return a.cache.dtype == VIB3_DT_F16 ? launch_decode_dt<VIB3_DT_F16>(d, (hipStream_t)stream)
                                       : launch_decode_dt<VIB3_DT_BF16>(d, (hipStream_t)stream);
