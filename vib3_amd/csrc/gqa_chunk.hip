@@ -347,7 +347,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
   const float scale = exponent_scale(a.scale);
   const uint32_t flip = sign_flip(a.scale);
   const uint64_t zero = (uint64_t)zero_token;
-  if (tid == 0) odd_values = 0;  // (before the first block's first barrier)
+  if (tid == 0) odd_values = 0;
+  __syncthreads();  // any wave may set it, in the first tile already
 
   // One block's tiles t0..t1 - 1 of key/value head g: its sums go to the output, or as a part to a slot of the workspace.
   auto attend = [&](const Block& bl, int g, int t0, int t1, int slot) {
