@@ -25,6 +25,13 @@ __device__ __forceinline__ int gqa_len(const vib3_gqa_cache& c, int n) {
 // The first token of the window of position p.
 __device__ __forceinline__ int window_start(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
 
+// A word's two 16-bit elements with zeros in the place of infinities and NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
+}
+
 // Host checks shared by the launchers.
 inline int check_gqa_cache(const vib3_gqa_cache& c) {
   if (!mla_dtype(c.dtype) || (c.dim != 64 && c.dim != 128 && c.dim != 256)) return VIB3_ERR_UNSUPPORTED;

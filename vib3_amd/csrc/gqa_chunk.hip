@@ -83,12 +83,6 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// A word's two 16-bit elements with zeros in the place of infinities and NaN.
-template <int DT>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
-}
 // The queries of a sequence.
 struct Queries {
   int seq, q0, nq, len;  // its row of the table, its first query, their number, its tokens
@@ -640,46 +634,84 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
     } else {
       for (int t = t0; t < t1; t++) step(t, s, s);
     }
-    wait_lds_loads();  // those past the last tile: not into LDS that the next block's go to
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(odd_values)) {
-      // What was cleared, for the queries that do see it: infinities times a probability of 0 are NaN, as in other tiles.
-      // (Values, scores and probabilities come from memory again, so that the ordinary path holds nothing for this one.)
+    wait_lds_loads();  // those past the last tile too: they must not land after the workgroup has ended
+    __syncthreads();   // odd_values is whole
+    // What is not finite, for the queries that see it: a value that was cleared is missing, and one whose probability is 0 in the
+    // 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. Such values are looked for in memory,
+    // and count by their probability in f32, in masked tiles and others alike. (Scores are formed again from memory too, so that
+    // the ordinary path holds nothing for this one.)
+    float odd_sum[8] = {};  // NaN where a sum of this lane is not finite
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int c = 0; c < VB; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) odd_sum[i % 8] = __builtin_fmaf(o[n][c][i], 0.0f, odd_sum[i % 8]);
+#pragma unroll
+    for (int i = 1; i < 8; i++) odd_sum[0] += odd_sum[i];
+    if (__builtin_amdgcn_readfirstlane(odd_values) || __any(odd_sum[0] != odd_sum[0])) {
+      const int lane_now = fresh(lane), half_now = lane_now >> 5;  // (the loop above has its own)
+      constexpr uint16_t kFraction = DT == VIB3_DT_F16 ? 0x3ff : 0x7f;
+      // a bit for each of the lane's sums: what an infinity of either sign and what a NaN is added to
+      uint32_t above[NB][(VB + 1) / 2] = {}, below[NB][(VB + 1) / 2] = {}, none[NB][(VB + 1) / 2] = {};
 #pragma unroll 1
       for (int t = t0; t < t1; t++) {
-        if (!is_masked(bl.token(t))) continue;
+        const int base = bl.token(t);
+        if (base > w_high || (base + kTile <= low_start && base >= a.sinks)) continue;
 #pragma unroll 1
-        for (int j = bl.token(t); j < min(bl.token(t) + kTile, bl.q.len); j++) {
-          const int64_t at = gqa_token(a.cache, bl.q.seq, j);
-          if (at < 0) continue;
-          const uint16_t* key = (const uint16_t*)a.cache.keys + at + head_at;
-          const uint16_t* value = (const uint16_t*)a.cache.values + at + head_at;
+        for (int j0 = base; j0 < base + kTile; j0 += kPer) {
+          const int jl = j0 + lane_now / C;
+          const int64_t at = jl < bl.q.len ? gqa_token(a.cache, bl.q.seq, jl) : -1;
+          const uint4 w = *(const uint4*)(at < 0 ? (const uint16_t*)zero : (const uint16_t*)a.cache.values + at + head_at + lane_now % C * 8);
+          uint64_t hits = __ballot(finite_only<DT>(w.x) != w.x || finite_only<DT>(w.y) != w.y || finite_only<DT>(w.z) != w.z ||
+                                   finite_only<DT>(w.w) != w.w);
+          while (hits) {
+            const int in = (__ffsll((unsigned long long)hits) - 1) / C, j = j0 + in;
+            hits &= ~(((1ull << C) - 1) << (in * C));
+            const int64_t token = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)((uint64_t)at >> 32), in * C) << 32 |
+                                            (uint32_t)__builtin_amdgcn_readlane((int)at, in * C));
+            const uint16_t* key = (const uint16_t*)a.cache.keys + token + head_at;
+            const uint16_t* value = (const uint16_t*)a.cache.values + token + head_at;
 #pragma unroll
-          for (int n = 0; n < NB; n++) {
-            float score = 0.0f;
+            for (int n = 0; n < NB; n++) {
+              float score = 0.0f;
 #pragma unroll 1
-            for (int c = half; c < C; c += 2) {  // the other chunks are the pair's other lane's
-              float x[8], y[8];
-              unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + q_at[n] + 8 * c), x);
-              unpack8<DT>(*(const uint4*)(key + 8 * c), y);
+              for (int c = half_now; c < C; c += 2) {  // the other chunks are the pair's other lane's
+                float x[8], y[8];
+                unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + q_at[n] + 8 * c), x);
+                unpack8<DT>(*(const uint4*)(key + 8 * c), y);
 #pragma unroll
-              for (int i = 0; i < 8; i++) score = __builtin_fmaf(x[i], y[i], score);
-            }
-            score = a.scale < 0.0f ? -pair_sum(score) : pair_sum(score);
-            const float e = __builtin_amdgcn_exp2f((score - (m[n] == -__builtin_huge_valf() ? 0.0f : m[n])) * scale);
-            if (j > pos[n] || (j < start[n] && j >= a.sinks)) continue;
-#pragma unroll
-            for (int c = 0; c < VB; c++)
-#pragma unroll
-              for (int i = 0; i < 16; i++) {
-                const uint16_t y = value[32 * c + 8 * (i >> 2) + 4 * half + (i & 3)];
-                if (finite_only<DT>(y) != y) o[n][c][i] += e != 0.0f ? to_f32<DT>(y) : __builtin_nanf("");
+                for (int i = 0; i < 8; i++) score = __builtin_fmaf(x[i], y[i], score);
               }
+              score = a.scale < 0.0f ? -pair_sum(score) : pair_sum(score);
+              const float e = __builtin_amdgcn_exp2f((score - (m[n] == -__builtin_huge_valf() ? 0.0f : m[n])) * scale);
+              const bool sees = (j <= pos[n]) & ((j >= start[n]) | (j < a.sinks));
+#pragma unroll
+              for (int c = 0; c < VB; c++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                  const uint16_t y = value[32 * c + 8 * (i >> 2) + 4 * half_now + (i & 3)];
+                  const bool odd = sees & (finite_only<DT>(y) != y), nan = (e == 0.0f) | ((y & kFraction) != 0), minus = (y & 0x8000) != 0;
+                  const uint32_t bit = 1u << (c % 2 * 16 + i);
+                  none[n][c / 2] |= odd & nan ? bit : 0;
+                  above[n][c / 2] |= odd & !nan & !minus ? bit : 0;
+                  below[n][c / 2] |= odd & !nan & minus ? bit : 0;
+                }
+            }
           }
         }
       }
-      __syncthreads();
-      if (tid == 0) odd_values = 0;
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int c = 0; c < VB; c++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const uint32_t bit = 1u << (c % 2 * 16 + i);
+            const bool up = above[n][c / 2] & bit, down = below[n][c / 2] & bit, nan = (none[n][c / 2] & bit) || (up && down);
+            const float odd = nan ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf();
+            o[n][c][i] = nan | up | down ? odd : o[n][c][i];
+          }
     }
 
     if (slot >= 0) {

@@ -3,7 +3,7 @@
 // Bound by the bytes of the cache: a key and a value of dim 16-bit elements serve heads / kv_heads queries, 4 flops a byte and query.
 // Two launches:
 //   k_gqa_attend   the attention, over equal shares of all rows' visible tokens
-//   k_gqa_join     rows that several shares were needed for
+//   k_gqa_join     rows that several shares were needed for, and those in which something is not finite once more
 //
 // The shares: tokens are taken 32 at a time, 64 for heads of 64 (a unit). All units of all rows in order, with kRowCost units' time in front of each row
 // for taking it up and storing its sums, are cut into equal runs, whatever the rows' lengths. A run is walked by one wave per
@@ -411,7 +411,94 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
 
 // ------------------------------------------------------------------------- joined rows
 
-// `team` waves (1, 2, 4, 8 or 16) of a workgroup of WAVES join the parts of one (row, head); rows that see nothing become zero.
+// Result y (E columns a lane) of a row and head in which something is not finite, as the formula gives it in f32: an infinite value whose
+// probability is 0 in the 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. By one wave, from
+// memory, kPer tokens at a time and D / 8 lanes a token: the largest score, then the values that are not finite, with their probabilities.
+template <int DT, int D>
+__device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r, int h, int64_t head_at, float (&y)[D / 64]) {
+  constexpr int C = D / 8, kPer = 64 / C, E = D / 64, kAhead = 4;
+  const int lane = lane_id();
+  const Seen<1> row = row_seen<1>(a, r);
+  const int sinks = min(a.sinks, row.start);
+  const int tokens = sinks + row.len - row.start;  // that the row sees
+  const auto place = [&](int i) -> int64_t {
+    return i < tokens ? gqa_token(a.cache, row.seq, i < sinks ? i : row.start + i - sinks) : -1;
+  };
+  const auto chunk = [&](const void* pool, int64_t at) {
+    return *(const uint4*)(at < 0 ? (const uint16_t*)zero_token : (const uint16_t*)pool + at + head_at + lane % C * 8);
+  };
+  float q[8];
+  unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + (int64_t)r * a.q_row_stride + (int64_t)h * a.q_head_stride + lane % C * 8), q);
+  const auto score = [&](uint4 key) {
+    float k[8], s = 0.0f;
+    unpack8<DT>(key, k);
+#pragma unroll
+    for (int i = 0; i < 8; i++) s = __builtin_fmaf(q[i], k[i], s);
+#pragma unroll
+    for (int d = 1; d < C; d *= 2) s += __shfl_xor(s, d);
+    return a.scale < 0.0f ? -s : s;
+  };
+  float top = -__builtin_huge_valf();
+  bool none = false;  // whether a score is no number
+#pragma unroll 1
+  for (int i0 = 0; i0 < tokens; i0 += kAhead * kPer) {
+    int64_t at[kAhead];
+    uint4 key[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) at[k] = place(i0 + k * kPer + lane / C);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) key[k] = chunk(a.cache.keys, at[k]);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      const float s = score(key[k]);
+      top = at[k] < 0 ? top : fmaxf(top, s);
+      none |= (at[k] >= 0) & (s != s);
+    }
+  }
+#pragma unroll
+  for (int d = C; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (__any(none) || top == __builtin_huge_valf()) {
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = __builtin_nanf("");
+    return;
+  }
+  const float scale = exponent_scale(a.scale);
+  float odd[E] = {};  // the columns' infinities and NaN
+#pragma unroll 1
+  for (int i0 = 0; i0 < tokens; i0 += kAhead * kPer) {
+    int64_t at[kAhead];
+    uint4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) at[k] = place(i0 + k * kPer + lane / C);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) v[k] = chunk(a.cache.values, at[k]);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      uint64_t hits = __ballot(finite_only<DT>(v[k].x) != v[k].x || finite_only<DT>(v[k].y) != v[k].y || finite_only<DT>(v[k].z) != v[k].z ||
+                               finite_only<DT>(v[k].w) != v[k].w);
+      if (hits == 0) continue;
+      const float s = score(chunk(a.cache.keys, at[k]));
+      while (hits) {
+        const int in = (__ffsll((unsigned long long)hits) - 1) / C;
+        hits &= ~(((1ull << C) - 1) << (in * C));
+        const int64_t token = uniform64(at[k], in * C);
+        const float p = __builtin_amdgcn_exp2f((__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(s), in * C)) - top) * scale);
+        const uint16_t* value = (const uint16_t*)a.cache.values + token + head_at + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const uint16_t x = value[e];
+          const float add = p != 0.0f ? to_f32<DT>(x) : __builtin_nanf("");
+          odd[e] += finite_only<DT>(x) != x ? add : 0.0f;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) y[e] = odd[e] != 0.0f ? odd[e] : y[e];
+}
+
+// `team` waves (1, 2, 4, 8 or 16) of a workgroup of WAVES join the parts of one (row, head); rows that see nothing become zero. Rows of
+// one share, which wrote them, are looked at too: what is not finite is formed again.
 template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team) {
   constexpr int E = D / 64;  // columns of a lane
@@ -494,11 +581,20 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team)
       }
     }
   }
-  if (r >= a.rows || mate || parts == 1) return;
+  if (r >= a.rows || mate) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + lane * E;
+  float y[E], odd = 0.0f;
 #pragma unroll
-  for (int e = 0; e < E; e++) out[e] = from_f32<DT>(o[e] * inv);
+  for (int e = 0; e < E; e++) {
+    y[e] = parts == 1 ? to_f32<DT>(out[e]) : o[e] * inv;
+    odd = __builtin_fmaf(y[e], 0.0f, odd);
+  }
+  const bool again = __any(odd != odd);
+  if (again) count_infinities<DT, D>(a, r, h, h / d.h.group * a.cache.head_stride, y);
+  if (parts == 1 && !again) return;
+#pragma unroll
+  for (int e = 0; e < E; e++) out[e] = from_f32<DT>(y[e]);
 }
 
 template <int DT, int D>
