@@ -67,6 +67,27 @@ def test_decode(dtype, heads, kv_heads, dim, n, at, ps, gap):
     check(c, q, got, torch.tensor(lens, device="cuda") - 1, at, gap, 30, at + 1)
 
 
+@pytest.mark.parametrize("rows", [5, 600])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scores_that_are_all_minus_infinity(dtype, heads, kv_heads, dim, rows):
+    """Nothing has a probability: zeros, also where values are not finite; NaN scores and +infinity give NaN."""
+    n = 300
+    c = Paged([n], kv_heads, dim, dtype, 16, seed=71)
+    c.k[0].zero_()
+    c.k[0][..., 0] = -INF
+    c.v[0][5, :, 0], c.v[0][200, :, 1] = INF, NAN
+    c.store()
+    q = ones(n, heads, dim, dtype)
+    lens = [n - i % n for i in range(rows)]
+    for whole in (True, False):
+        assert bool((run(c, heads, [n], whole, many=MANY if whole else 1, q=q)[1] == 0).all())
+        assert bool(run(c, heads, [n], whole, many=MANY if whole else 1, q=-q)[1].isnan().all())
+    one = q[:1].expand(rows, heads, dim)
+    assert bool((decode(c, heads, [(0, x) for x in lens], q=one)[1] == 0).all())
+    assert bool(decode(c, heads, [(0, x) for x in lens], q=-q[:1].expand(rows, heads, dim))[1].isnan().all())
+
+
 def test_both_infinities_and_small_probabilities_together():
     """A column's infinities of both signs give NaN, also where one of them counts 2^-90 of the other."""
     from vib3_amd import gqa

@@ -702,7 +702,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
         }
       }
 #pragma unroll
-      for (int n = 0; n < NB; n++)
+      for (int n = 0; n < NB; n++) {
+        const bool zero_sum = m[n] == -__builtin_huge_valf() && pair_sum(l[n]) == 0.0f;  // nothing has a probability
 #pragma unroll
         for (int c = 0; c < VB; c++)
 #pragma unroll
@@ -710,8 +711,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
             const uint32_t bit = 1u << (c % 2 * 16 + i);
             const bool up = above[n][c / 2] & bit, down = below[n][c / 2] & bit, nan = (none[n][c / 2] & bit) || (up && down);
             const float odd = nan ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf();
-            o[n][c][i] = nan | up | down ? odd : o[n][c][i];
+            o[n][c][i] = zero_sum ? 0.0f : nan | up | down ? odd : o[n][c][i];
           }
+      }
     }
 
     if (slot >= 0) {

@@ -457,9 +457,11 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
   }
 #pragma unroll
   for (int d = C; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  if (__any(none) || top == __builtin_huge_valf()) {
+  if (__any(none) || top == -__builtin_huge_valf() || top == __builtin_huge_valf()) {
+    // (scores that are all -infinity give nothing a probability)
+    const float all = !__any(none) && top < 0.0f ? 0.0f : __builtin_nanf("");
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = __builtin_nanf("");
+    for (int e = 0; e < E; e++) y[e] = all;
     return;
   }
   const float scale = exponent_scale(a.scale);
