@@ -8,6 +8,7 @@
 // Bound by HBM for prompts (6007 tokens of 40 + 8 + 8 heads of 128 from f32: 258 MB in 57 us, 4.5 TB/s; a copy of 2 GB 5.0), by the launch and
 // its chain of reads (sequence, page number, row) for single tokens (5 us).
 #include "gqa.h"
+#include "scan.h"
 
 namespace vib3 {
 namespace {
@@ -16,7 +17,8 @@ template <int DT, int D>
 __global__ __launch_bounds__(256) void k_gqa_append(vib3_gqa_append a) {
   constexpr int kLanes = D / 16;  // of a row
   __shared__ float2 turns[D / 2];
-  const int tid = (int)threadIdx.x, t = (int)blockIdx.x;
+  const int tid = (int)threadIdx.x, t = (int)wide_block();
+  if ((unsigned)t >= (unsigned)a.tokens) return;
   const int s = a.seqs[t], p = a.positions[t];
   if ((unsigned)s >= (unsigned)a.cache.num_seqs || p < 0) return;
   const int64_t cached = gqa_token(a.cache, s, p);
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(256) void k_gqa_append(vib3_gqa_append a) {
 template <int DT>
 void launch_append(const vib3_gqa_append& a, hipStream_t st) {
   auto kernel = a.cache.dim == 64 ? k_gqa_append<DT, 64> : a.cache.dim == 128 ? k_gqa_append<DT, 128> : k_gqa_append<DT, 256>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.tokens), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(kernel, wide_grid(a.tokens), dim3(256), 0, st, a);
 }
 
 }  // namespace

@@ -757,9 +757,10 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
   };
 
   if constexpr (!CUT) {
-    const int g = (int)(blockIdx.x % (unsigned)a.cache.kv_heads);
+    const unsigned item = wide_block();
+    const int g = (int)(item % (unsigned)a.cache.kv_heads);
     Block bl;
-    if (!find_block(a, (int)(blockIdx.x / (unsigned)a.cache.kv_heads), kRows, d.group, &bl)) return;
+    if (!find_block(a, (int)(item / (unsigned)a.cache.kv_heads), kRows, d.group, &bl)) return;
     attend(bl, g, 0, bl.tiles, -1);
   } else {
     const int blocks = __builtin_amdgcn_readfirstlane(make_plan<WAVES * 64>(d, kRows, card_groups(D), plan));
@@ -859,7 +860,7 @@ int launch_chunk(const ChunkArgs& d, hipStream_t st) {
   int64_t longest = (int64_t)a.cache.max_pages * a.cache.page_size;
   if (a.window > 0 && (int64_t)a.window + a.sinks + S::rows / d.group < longest) longest = (int64_t)a.window + a.sinks + S::rows / d.group;
   if (items >= (longest <= 96 * kTile ? 2 : 4) * kGroups || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
-    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false, WHOLE>), dim3((unsigned)items), dim3(S::waves * 64), 0, st, d);
+    hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, false, WHOLE>), wide_grid(items), dim3(S::waves * 64), 0, st, d);
   } else {  // (pieces of at least an even share: no more than blocks and shares)
     hipLaunchKernelGGL((k_gqa_tiles<DT, D, S::waves, S::blocks, true, WHOLE>), dim3((unsigned)items + kGroups), dim3(S::waves * 64), 0, st, d);
     hipLaunchKernelGGL((k_gqa_join_tiles<DT, D>), dim3((unsigned)(items < kGroups ? items : kGroups) * (S::rows / 32)), dim3(D * 2), 0, st, d, S::rows);

@@ -509,7 +509,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team)
   __shared__ float tops[WAVES], totals[WAVES];
   const vib3_gqa_decode& a = d.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int x = (int)blockIdx.x * (WAVES / team) + wave / team;
+  const int x = (int)wide_block() * (WAVES / team) + wave / team;
   const int mate = wave % team;
   const int r = x / a.heads, h = x - r * a.heads;
   int parts = 1;
@@ -607,8 +607,8 @@ int launch_decode(const DecodeArgs& d, hipStream_t st) {
   const int64_t items = (int64_t)d.a.rows * d.a.heads;
   int team = 16;
   while (team > 1 && items * team > 8192) team /= 2;  // 16 waves a CU twice over
-  if (team > 4) hipLaunchKernelGGL((k_gqa_join<DT, D, 16>), dim3((unsigned)((items * team + 15) / 16)), dim3(1024), 0, st, d, team);
-  else hipLaunchKernelGGL((k_gqa_join<DT, D, 4>), dim3((unsigned)((items * team + 3) / 4)), dim3(256), 0, st, d, team);
+  if (team > 4) hipLaunchKernelGGL((k_gqa_join<DT, D, 16>), wide_grid((items * team + 15) / 16), dim3(1024), 0, st, d, team);
+  else hipLaunchKernelGGL((k_gqa_join<DT, D, 4>), wide_grid((items * team + 3) / 4), dim3(256), 0, st, d, team);
   VIB3_RETURN_LAUNCH();
 }
 

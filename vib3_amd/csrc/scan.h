@@ -1,4 +1,4 @@
-// scan.h — sums over the lanes of a wave, and division by a number that a launch fixes.
+// scan.h — sums over the lanes of a wave, division by a number that a launch fixes, and launches of any number of workgroups.
 #pragma once
 
 #include "common.h"
@@ -37,5 +37,13 @@ inline Divisor divisor(int n) {
   while ((int64_t)1 << shift < n) shift++;
   return Divisor{(uint32_t)((((uint64_t)1 << (31 + shift)) + (uint64_t)n - 1) / (uint64_t)n), shift};
 }
+
+// A grid of at least this many workgroups (up to 2^31). A dimension holds fewer than 2^32 threads, so many workgroups are rows of 2^21;
+// those past the number end at once. wide_block: a workgroup's place in it.
+inline dim3 wide_grid(int64_t blocks) {
+  constexpr int64_t kRow = 1 << 21;
+  return blocks <= kRow ? dim3((unsigned)blocks) : dim3((unsigned)kRow, (unsigned)((blocks + kRow - 1) / kRow));
+}
+__device__ __forceinline__ unsigned wide_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 }  // namespace vib3
