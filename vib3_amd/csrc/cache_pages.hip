@@ -257,7 +257,7 @@ int check_pools(const vib3_page_pool* pools, int num_pools, int num_pages, int p
     if ((num_pages && !p.base) || ((uintptr_t)p.base & 15) || p.token_bytes % 16 || p.page_stride % 16 || p.run_stride % 16 ||
         p.token_stride % 16)
       return VIB3_ERR_BAD_POINTER;
-    if (page_chunks(p, page_size) > 0x7fffffff - kPiece) return VIB3_ERR_BAD_COUNT;
+    if ((int64_t)p.runs * page_size > (0x7fffffff - kPiece) / (p.token_bytes / 16)) return VIB3_ERR_BAD_COUNT;  // page_chunks fits an int
   }
   return 0;
 }
