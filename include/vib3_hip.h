@@ -617,8 +617,8 @@ int vib3_launch_mla_prefill(const vib3_mla_prefill *args, void *stream);
  * no token, or whose scores are all -infinity, gives zeros. What it does not see leaves it as it
  * is, infinities and NaN included; where it sees some, it is what the formula gives in f32 (0
  * times infinity is NaN): an infinite value counts as an infinity where its probability is at least
- * 2^-126 of the largest, as NaN where that is 0 in f32, and between the two as either. (Such rows are
- * formed again, which takes longer.) Statistics and sums are f32; probabilities go to the matrix cores in the
+ * 2^-126 of the largest, and as an infinity or NaN below that. (Sums that are NaN are looked into
+ * again, which takes longer.) Statistics and sums are f32; probabilities go to the matrix cores in the
  * 16-bit type, in f16 with all of its bits down to 2^-25 of the row's largest, and off by at most
  * 2^-36 of that below.
  * ---------------------------------------------------------------------------------------- */

@@ -86,6 +86,27 @@ def test_scores_that_are_all_minus_infinity(dtype, heads, kv_heads, dim, rows):
     one = q[:1].expand(rows, heads, dim)
     assert bool((decode(c, heads, [(0, x) for x in lens], q=one)[1] == 0).all())
     assert bool(decode(c, heads, [(0, x) for x in lens], q=-q[:1].expand(rows, heads, dim))[1].isnan().all())
+    c.v[0].fill_(NAN)
+    c.store()
+    assert bool((decode(c, heads, [(0, x) for x in lens], q=one)[1] == 0).all())
+    assert bool((run(c, heads, [n], True, q=q)[1] == 0).all()) and bool((run(c, heads, [n], False, many=1, q=q)[1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,first", [(300, 299), (300, 150), (9000, 8999), (9000, 4000), (9000, 0)])
+def test_values_that_are_nan_beside_infinities(dtype, n, first):
+    """Tokens from `first` on hold NaN in two columns; an infinity in a third one counts little (40 nats below)."""
+    c = Paged([n], 2, 128, dtype, 16, seed=73)
+    c.k[0].zero_()
+    c.k[0][7, :, 0] = -40.0
+    c.v[0][first:, :, 4:6], c.v[0][7, :, 9] = NAN, INF
+    c.store()
+    q = ones(64, 8, 128, dtype)
+    for got in (decode(c, 8, [(0, n)] * 3, scale=1.0, q=q[:3])[1], run(c, 8, [64], False, many=1, scale=1.0, q=q)[1][-1:],
+                run(c, 8, [64], True, scale=1.0, q=q)[1][-1:]):
+        assert bool(got[..., 4:6].isnan().all()) and bool((got[..., 9] == INF).all())
+        others = [i for i in range(128) if i not in (4, 5, 9)]
+        assert bool(got[..., others].isfinite().all())
 
 
 def test_both_infinities_and_small_probabilities_together():

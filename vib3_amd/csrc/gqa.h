@@ -32,6 +32,13 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
   return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
 }
 
+// Whether one of a word's two 16-bit elements is NaN.
+template <int DT>
+__device__ __forceinline__ bool has_nan(uint32_t w) {
+  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
+  return (w & 0x7fffu) > e || (w >> 16 & 0x7fffu) > e;
+}
+
 // Host checks shared by the launchers.
 inline int check_gqa_cache(const vib3_gqa_cache& c) {
   if (!mla_dtype(c.dtype) || (c.dim != 64 && c.dim != 128 && c.dim != 256)) return VIB3_ERR_UNSUPPORTED;

@@ -637,9 +637,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
     wait_lds_loads();  // those past the last tile too: they must not land after the workgroup has ended
     __syncthreads();   // odd_values is whole
     // What is not finite, for the queries that see it: a value that was cleared is missing, and one whose probability is 0 in the
-    // 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. Such values are looked for in memory,
-    // and count by their probability in f32, in masked tiles and others alike. (Scores are formed again from memory too, so that
-    // the ordinary path holds nothing for this one.)
+    // 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. Such values are looked for in memory, in
+    // masked tiles or, for a sum that is NaN, in all, and count by their probability in f32. (Scores are formed again from memory
+    // too, so that the ordinary path holds nothing for this one.)
     float odd_sum[8] = {};  // NaN where a sum of this lane is not finite
 #pragma unroll
     for (int n = 0; n < NB; n++)
@@ -650,6 +650,18 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
 #pragma unroll
     for (int i = 1; i < 8; i++) odd_sum[0] += odd_sum[i];
     if (__builtin_amdgcn_readfirstlane(odd_values) || __any(odd_sum[0] != odd_sum[0])) {
+      bool open = false, number[NB], zero_sum[NB];  // whether a NaN has to be explained; whether the probabilities' sum is no NaN, and 0
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const float sum = pair_sum(l[n]);
+        number[n] = sum == sum;  // (a sum of probabilities that is NaN makes all of the row NaN)
+        zero_sum[n] = m[n] == -__builtin_huge_valf() && sum == 0.0f;
+#pragma unroll
+        for (int c = 0; c < VB; c++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) open |= number[n] & (o[n][c][i] != o[n][c][i]);
+      }
+      bool search = __any(open);
       const int lane_now = fresh(lane), half_now = lane_now >> 5;  // (the loop above has its own)
       constexpr uint16_t kFraction = DT == VIB3_DT_F16 ? 0x3ff : 0x7f;
       // a bit for each of the lane's sums: what an infinity of either sign and what a NaN is added to
@@ -657,7 +669,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
 #pragma unroll 1
       for (int t = t0; t < t1; t++) {
         const int base = bl.token(t);
-        if (base > w_high || (base + kTile <= low_start && base >= a.sinks)) continue;
+        if (base > w_high || (base + kTile <= low_start && base >= a.sinks) || !(search || is_masked(base))) continue;
+        bool found = false;
 #pragma unroll 1
         for (int j0 = base; j0 < base + kTile; j0 += kPer) {
           const int jl = j0 + lane_now / C;
@@ -665,6 +678,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
           const uint4 w = *(const uint4*)(at < 0 ? (const uint16_t*)zero : (const uint16_t*)a.cache.values + at + head_at + lane_now % C * 8);
           uint64_t hits = __ballot(finite_only<DT>(w.x) != w.x || finite_only<DT>(w.y) != w.y || finite_only<DT>(w.z) != w.z ||
                                    finite_only<DT>(w.w) != w.w);
+          found |= hits != 0;
           while (hits) {
             const int in = (__ffsll((unsigned long long)hits) - 1) / C, j = j0 + in;
             hits &= ~(((1ull << C) - 1) << (in * C));
@@ -675,11 +689,11 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
 #pragma unroll
             for (int n = 0; n < NB; n++) {
               float score = 0.0f;
-#pragma unroll 1
-              for (int c = half_now; c < C; c += 2) {  // the other chunks are the pair's other lane's
+#pragma unroll 4
+              for (int c = 0; c < C; c += 2) {  // the other chunks are the pair's other lane's
                 float x[8], y[8];
-                unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + q_at[n] + 8 * c), x);
-                unpack8<DT>(*(const uint4*)(key + 8 * c), y);
+                unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + q_at[n] + 8 * (c + half_now)), x);
+                unpack8<DT>(*(const uint4*)(key + 8 * (c + half_now)), y);
 #pragma unroll
                 for (int i = 0; i < 8; i++) score = __builtin_fmaf(x[i], y[i], score);
               }
@@ -700,20 +714,29 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
             }
           }
         }
+        if (search && found) {  // until each NaN has its reason
+          open = false;
+#pragma unroll
+          for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int c = 0; c < VB; c++)
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+                open |= number[n] && o[n][c][i] != o[n][c][i] && !((none[n][c / 2] | (above[n][c / 2] & below[n][c / 2])) >> (c % 2 * 16 + i) & 1);
+          search = __any(open);
+        }
       }
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-        const bool zero_sum = m[n] == -__builtin_huge_valf() && pair_sum(l[n]) == 0.0f;  // nothing has a probability
+      for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int c = 0; c < VB; c++)
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const uint32_t bit = 1u << (c % 2 * 16 + i);
             const bool up = above[n][c / 2] & bit, down = below[n][c / 2] & bit, nan = (none[n][c / 2] & bit) || (up && down);
-            const float odd = nan ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf();
-            o[n][c][i] = zero_sum ? 0.0f : nan | up | down ? odd : o[n][c][i];
+            const float odd = nan ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf(), sum = o[n][c][i];
+            o[n][c][i] = zero_sum[n] ? 0.0f : !(nan | up | down) ? sum : sum != sum ? odd : sum + odd;
           }
-      }
     }
 
     if (slot >= 0) {

@@ -3,7 +3,7 @@
 // Bound by the bytes of the cache: a key and a value of dim 16-bit elements serve heads / kv_heads queries, 4 flops a byte and query.
 // Two launches:
 //   k_gqa_attend   the attention, over equal shares of all rows' visible tokens
-//   k_gqa_join     rows that several shares were needed for, and those in which something is not finite once more
+//   k_gqa_join     rows that several shares were needed for, and those in which something is NaN once more
 //
 // The shares: tokens are taken 32 at a time, 64 for heads of 64 (a unit). All units of all rows in order, with kRowCost units' time in front of each row
 // for taking it up and storing its sums, are cut into equal runs, whatever the rows' lengths. A run is walked by one wave per
@@ -411,9 +411,10 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
 
 // ------------------------------------------------------------------------- joined rows
 
-// Result y (E columns a lane) of a row and head in which something is not finite, as the formula gives it in f32: an infinite value whose
+// Result y (E columns a lane) of a row and head in which something is NaN, as the formula gives it in f32: an infinite value whose
 // probability is 0 in the 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. By one wave, from
-// memory, kPer tokens at a time and D / 8 lanes a token: the largest score, then the values that are not finite, with their probabilities.
+// memory, kPer tokens at a time and D / 8 lanes a token: the largest score and values that are NaN, then the other values that are not
+// finite, with their probabilities. It ends where each NaN has a reason.
 template <int DT, int D>
 __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r, int h, int64_t head_at, float (&y)[D / 64]) {
   constexpr int C = D / 8, kPer = 64 / C, E = D / 64, kAhead = 4;
@@ -421,8 +422,16 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
   const Seen<1> row = row_seen<1>(a, r);
   const int sinks = min(a.sinks, row.start);
   const int tokens = sinks + row.len - row.start;  // that the row sees
-  const auto place = [&](int i) -> int64_t {
-    return i < tokens ? gqa_token(a.cache, row.seq, i < sinks ? i : row.start + i - sinks) : -1;
+  const auto place = [&](int i) -> int64_t {  // the newest come first: of a sequence that has become NaN they are
+    const int j = tokens - 1 - i;
+    return j < 0 ? -1 : gqa_token(a.cache, row.seq, j < sinks ? j : row.start + j - sinks);
+  };
+  const auto each = [&](uint64_t hits, auto f) {  // the tokens in whose chunks something was found
+    while (hits) {
+      const int in = (__ffsll((unsigned long long)hits) - 1) / C;
+      hits &= ~(((1ull << C) - 1) << (in * C));
+      f(in);
+    }
   };
   const auto chunk = [&](const void* pool, int64_t at) {
     return *(const uint4*)(at < 0 ? (const uint16_t*)zero_token : (const uint16_t*)pool + at + head_at + lane % C * 8);
@@ -438,21 +447,38 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
     for (int d = 1; d < C; d *= 2) s += __shfl_xor(s, d);
     return a.scale < 0.0f ? -s : s;
   };
+  float odd[E] = {};  // the columns' infinities and NaN
+  bool open = true;   // whether a NaN of this lane still has no reason
+  const auto look = [&] {
+    open = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) open |= y[e] != y[e] && odd[e] == odd[e];
+  };
   float top = -__builtin_huge_valf();
   bool none = false;  // whether a score is no number
 #pragma unroll 1
-  for (int i0 = 0; i0 < tokens; i0 += kAhead * kPer) {
+  for (int i0 = 0; i0 < tokens && !__any(none); i0 += kAhead * kPer) {
     int64_t at[kAhead];
-    uint4 key[kAhead];
+    uint4 key[kAhead], v[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; k++) at[k] = place(i0 + k * kPer + lane / C);
 #pragma unroll
-    for (int k = 0; k < kAhead; k++) key[k] = chunk(a.cache.keys, at[k]);
+    for (int k = 0; k < kAhead; k++) key[k] = chunk(a.cache.keys, at[k]), v[k] = chunk(a.cache.values, at[k]);
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
       const float s = score(key[k]);
       top = at[k] < 0 ? top : fmaxf(top, s);
       none |= (at[k] >= 0) & (s != s);
+      // values that are NaN are so with any probability
+      const uint64_t hits = __ballot(has_nan<DT>(v[k].x) || has_nan<DT>(v[k].y) || has_nan<DT>(v[k].z) || has_nan<DT>(v[k].w));
+      if (hits == 0) continue;
+      each(hits, [&](int in) {
+        const uint16_t* value = (const uint16_t*)a.cache.values + uniform64(at[k], in * C) + head_at + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) odd[e] = has_nan<DT>(value[e]) ? __builtin_nanf("") : odd[e];
+      });
+      look();
+      if (!__any(open) && __any(top > -__builtin_huge_valf())) return;
     }
   }
 #pragma unroll
@@ -465,9 +491,8 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
     return;
   }
   const float scale = exponent_scale(a.scale);
-  float odd[E] = {};  // the columns' infinities and NaN
 #pragma unroll 1
-  for (int i0 = 0; i0 < tokens; i0 += kAhead * kPer) {
+  for (int i0 = 0; i0 < tokens && __any(open); i0 += kAhead * kPer) {
     int64_t at[kAhead];
     uint4 v[kAhead];
 #pragma unroll
@@ -476,31 +501,29 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
     for (int k = 0; k < kAhead; k++) v[k] = chunk(a.cache.values, at[k]);
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
-      uint64_t hits = __ballot(finite_only<DT>(v[k].x) != v[k].x || finite_only<DT>(v[k].y) != v[k].y || finite_only<DT>(v[k].z) != v[k].z ||
-                               finite_only<DT>(v[k].w) != v[k].w);
+      const uint64_t hits = __ballot(finite_only<DT>(v[k].x) != v[k].x || finite_only<DT>(v[k].y) != v[k].y ||
+                                     finite_only<DT>(v[k].z) != v[k].z || finite_only<DT>(v[k].w) != v[k].w);
       if (hits == 0) continue;
       const float s = score(chunk(a.cache.keys, at[k]));
-      while (hits) {
-        const int in = (__ffsll((unsigned long long)hits) - 1) / C;
-        hits &= ~(((1ull << C) - 1) << (in * C));
-        const int64_t token = uniform64(at[k], in * C);
+      each(hits, [&](int in) {
         const float p = __builtin_amdgcn_exp2f((__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(s), in * C)) - top) * scale);
-        const uint16_t* value = (const uint16_t*)a.cache.values + token + head_at + lane * E;
+        const uint16_t* value = (const uint16_t*)a.cache.values + uniform64(at[k], in * C) + head_at + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e++) {
           const uint16_t x = value[e];
           const float add = p != 0.0f ? to_f32<DT>(x) : __builtin_nanf("");
           odd[e] += finite_only<DT>(x) != x ? add : 0.0f;
         }
-      }
+      });
     }
+    look();
   }
 #pragma unroll
-  for (int e = 0; e < E; e++) y[e] = odd[e] != 0.0f ? odd[e] : y[e];
+  for (int e = 0; e < E; e++) y[e] = y[e] != y[e] && odd[e] != 0.0f ? odd[e] : y[e];
 }
 
 // `team` waves (1, 2, 4, 8 or 16) of a workgroup of WAVES join the parts of one (row, head); rows that see nothing become zero. Rows of
-// one share, which wrote them, are looked at too: what is not finite is formed again.
+// one share, which wrote them, are looked at too: what is NaN is formed again.
 template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team) {
   constexpr int E = D / 64;  // columns of a lane
@@ -586,14 +609,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_gqa_join(DecodeArgs d, int team)
   if (r >= a.rows || mate) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + (int64_t)r * a.out_row_stride + (int64_t)h * a.out_head_stride + lane * E;
-  float y[E], odd = 0.0f;
+  float y[E];
+  bool nan = false;
 #pragma unroll
   for (int e = 0; e < E; e++) {
     y[e] = parts == 1 ? to_f32<DT>(out[e]) : o[e] * inv;
-    odd = __builtin_fmaf(y[e], 0.0f, odd);
+    nan |= y[e] != y[e];
   }
-  const bool again = __any(odd != odd);
-  if (again) count_infinities<DT, D>(a, r, h, h / d.h.group * a.cache.head_stride, y);
+  const bool again = __any(nan) && l == l;  // (a sum of probabilities that is NaN makes all of the row NaN)
+  if (__builtin_expect(again, false)) count_infinities<DT, D>(a, r, h, h / d.h.group * a.cache.head_stride, y);
   if (parts == 1 && !again) return;
 #pragma unroll
   for (int e = 0; e < E; e++) out[e] = from_f32<DT>(y[e]);
