@@ -618,9 +618,10 @@ int vib3_launch_mla_prefill(const vib3_mla_prefill *args, void *stream);
  * is, infinities and NaN included; where it sees some, it is what the formula gives in f32 (0
  * times infinity is NaN): an infinite value counts as an infinity where its probability is at least
  * 2^-126 of the largest, and as an infinity or NaN below that. (Sums that are NaN are looked into
- * again, which takes longer.) Statistics and sums are f32; probabilities go to the matrix cores in the
- * 16-bit type, in f16 with all of its bits down to 2^-25 of the row's largest, and off by at most
- * 2^-36 of that below.
+ * again, which takes longer.) Statistics and sums are f32. Probabilities go to the matrix cores in the
+ * 16-bit type: vib3_launch_gqa_chunk's rounded to it, vib3_launch_gqa_decode's in two summands, off by
+ * at most 2^-15 of the number in bf16 and 2^-21 in f16. f16 has all of its bits down to 2^-25 of the
+ * row's largest, and is off by at most 2^-36 of that below.
  * ---------------------------------------------------------------------------------------- */
 typedef struct vib3_gqa_cache {
     void *keys, *values;        /* [num_pages][page_size][kv_heads][dim] each */
