@@ -32,11 +32,9 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
   return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
 }
 
-// Whether one of a word's two 16-bit elements is NaN.
 template <int DT>
-__device__ __forceinline__ bool has_nan(uint32_t w) {
-  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
-  return (w & 0x7fffu) > e || (w >> 16 & 0x7fffu) > e;
+__device__ __forceinline__ bool all_finite(uint4 v) {
+  return finite_only<DT>(v.x) == v.x && finite_only<DT>(v.y) == v.y && finite_only<DT>(v.z) == v.z && finite_only<DT>(v.w) == v.w;
 }
 
 // Host checks shared by the launchers.

@@ -676,8 +676,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
           const int jl = j0 + lane_now / C;
           const int64_t at = jl < bl.q.len ? gqa_token(a.cache, bl.q.seq, jl) : -1;
           const uint4 w = *(const uint4*)(at < 0 ? (const uint16_t*)zero : (const uint16_t*)a.cache.values + at + head_at + lane_now % C * 8);
-          uint64_t hits = __ballot(finite_only<DT>(w.x) != w.x || finite_only<DT>(w.y) != w.y || finite_only<DT>(w.z) != w.z ||
-                                   finite_only<DT>(w.w) != w.w);
+          uint64_t hits = __ballot(!all_finite<DT>(w));
           found |= hits != 0;
           while (hits) {
             const int in = (__ffsll((unsigned long long)hits) - 1) / C, j = j0 + in;

@@ -429,13 +429,51 @@ __global__ __launch_bounds__(attend_waves(D) * 64) void k_gqa_attend(DecodeArgs 
 
 // ------------------------------------------------------------------------- joined rows
 
+// What values hold that is not finite, in the 8 elements of a chunk (packed as they are): `up` and `down` are 0 where there was an
+// infinity of that sign, `nan` is not 0 where there was a NaN. top: what such an element's magnitude begins with.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <int DT>
+struct Odd {
+  static constexpr uint16_t top = DT == VIB3_DT_F16 ? 0x7c00 : 0x7f80;
+  u16x2 up[4], down[4], nan[4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 4; i++) up[i] = down[i] = u16x2{0xffff, 0xffff}, nan[i] = u16x2{0, 0};
+  }
+  // A value whose probability is 0 or not: 0 times an infinity is NaN.
+  __device__ __forceinline__ void add(uint4 v, bool zero) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint16_t most = zero ? top - 1 : top, off = zero ? 0xffff : 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const u16x2 x = __builtin_bit_cast(u16x2, w[i]), size = x & (uint16_t)0x7fff;
+      up[i] = __builtin_elementwise_min(up[i], (x ^ top) | off);
+      down[i] = __builtin_elementwise_min(down[i], (x ^ (uint16_t)(top | 0x8000)) | off);
+      nan[i] = __builtin_elementwise_max(nan[i], __builtin_elementwise_max(size, u16x2{most, most}) - most);
+    }
+  }
+  // Bit i for an infinity above 0 in element i, bit 8 + i for one below, bit 16 + i for a NaN.
+  __device__ __forceinline__ uint32_t bits() const {
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) b |= ((up[i / 2][i % 2] ? 0 : 1u) | (down[i / 2][i % 2] ? 0 : 1u << 8) | (nan[i / 2][i % 2] ? 1u << 16 : 0)) << i;
+    return b;
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+  if constexpr (DT == VIB3_DT_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), c, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+}
+
 // Result y (E columns a lane) of a row and head in which something is NaN, as the formula gives it in f32: an infinite value whose
 // probability is 0 in the 16-bit type only (f16, below 2^-36 of the largest) made a NaN of what is an infinity. By one wave, from
-// memory, kPer tokens at a time and D / 8 lanes a token: the largest score and values that are NaN, then the other values that are not
-// finite, with their probabilities. It ends where each NaN has a reason.
+// memory, kPer tokens at a time and D / 8 lanes a token: the largest score, the smallest one of a token whose value is not finite, and
+// what such values hold; if that one's probability is 0 (in f32), once more, by each one's. It ends early where values are NaN.
 template <int DT, int D>
 __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r, int h, int64_t head_at, float (&y)[D / 64]) {
-  constexpr int C = D / 8, kPer = 64 / C, E = D / 64, kAhead = 4;
+  constexpr int C = D / 8, kPer = 64 / C, E = D / 64, kAhead = 2;
   const int lane = lane_id();
   const Seen<1> row = row_seen<1>(a, r);
   const int sinks = min(a.sinks, row.start);
@@ -444,63 +482,73 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
     const int j = tokens - 1 - i;
     return j < 0 ? -1 : gqa_token(a.cache, row.seq, j < sinks ? j : row.start + j - sinks);
   };
-  const auto each = [&](uint64_t hits, auto f) {  // the tokens in whose chunks something was found
-    while (hits) {
-      const int in = (__ffsll((unsigned long long)hits) - 1) / C;
-      hits &= ~(((1ull << C) - 1) << (in * C));
-      f(in);
-    }
-  };
   const auto chunk = [&](const void* pool, int64_t at) {
     return *(const uint4*)(at < 0 ? (const uint16_t*)zero_token : (const uint16_t*)pool + at + head_at + lane % C * 8);
   };
-  float q[8];
-  unpack8<DT>(*(const uint4*)((const uint16_t*)a.q + (int64_t)r * a.q_row_stride + (int64_t)h * a.q_head_stride + lane % C * 8), q);
+  const uint32_t flip = sign_flip(a.scale);
+  const uint4 q = *(const uint4*)((const uint16_t*)a.q + (int64_t)r * a.q_row_stride + (int64_t)h * a.q_head_stride + lane % C * 8);
   const auto score = [&](uint4 key) {
-    float k[8], s = 0.0f;
-    unpack8<DT>(key, k);
-#pragma unroll
-    for (int i = 0; i < 8; i++) s = __builtin_fmaf(q[i], k[i], s);
-#pragma unroll
-    for (int d = 1; d < C; d *= 2) s += __shfl_xor(s, d);
-    return a.scale < 0.0f ? -s : s;
+    float s = dot2<DT>(q.x ^ flip, key.x, dot2<DT>(q.y ^ flip, key.y, dot2<DT>(q.z ^ flip, key.z, dot2<DT>(q.w ^ flip, key.w, 0.0f))));
+    auto more = [&](int moved) { s += __int_as_float(moved); };  // over the token's lanes
+    more(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0xb1, 0xf, 0xf, false));
+    more(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0x4e, 0xf, 0xf, false));
+    more(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0x141, 0xf, 0xf, false));
+    if (C > 8) more(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0x140, 0xf, 0xf, false));
+    if (C > 16) s += __shfl_xor(s, 16);
+    return s;
   };
-  float odd[E] = {};  // the columns' infinities and NaN
-  bool open = true;   // whether a NaN of this lane still has no reason
-  const auto look = [&] {
-    open = false;
+  // f(whether there is a token, its score, this lane's chunk of its value), until `done` after a group of them
+  const auto walk = [&](auto f, auto done) {
+    int64_t next[kAhead];
 #pragma unroll
-    for (int e = 0; e < E; e++) open |= y[e] != y[e] && odd[e] == odd[e];
-  };
-  float top = -__builtin_huge_valf();
-  bool none = false;  // whether a score is no number
+    for (int k = 0; k < kAhead; k++) next[k] = place(k * kPer + lane / C);
 #pragma unroll 1
-  for (int i0 = 0; i0 < tokens && !__any(none); i0 += kAhead * kPer) {
-    int64_t at[kAhead];
-    uint4 key[kAhead], v[kAhead];
+    for (int i0 = 0; i0 < tokens; i0 += kAhead * kPer) {
+      bool there[kAhead];
+      uint4 key[kAhead], v[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; k++) at[k] = place(i0 + k * kPer + lane / C);
+      for (int k = 0; k < kAhead; k++) there[k] = next[k] >= 0, key[k] = chunk(a.cache.keys, next[k]), v[k] = chunk(a.cache.values, next[k]);
 #pragma unroll
-    for (int k = 0; k < kAhead; k++) key[k] = chunk(a.cache.keys, at[k]), v[k] = chunk(a.cache.values, at[k]);
+      for (int k = 0; k < kAhead; k++) next[k] = place(i0 + (kAhead + k) * kPer + lane / C);
 #pragma unroll
-    for (int k = 0; k < kAhead; k++) {
-      const float s = score(key[k]);
-      top = at[k] < 0 ? top : fmaxf(top, s);
-      none |= (at[k] >= 0) & (s != s);
-      // values that are NaN are so with any probability
-      const uint64_t hits = __ballot(has_nan<DT>(v[k].x) || has_nan<DT>(v[k].y) || has_nan<DT>(v[k].z) || has_nan<DT>(v[k].w));
-      if (hits == 0) continue;
-      each(hits, [&](int in) {
-        const uint16_t* value = (const uint16_t*)a.cache.values + uniform64(at[k], in * C) + head_at + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) odd[e] = has_nan<DT>(value[e]) ? __builtin_nanf("") : odd[e];
-      });
-      look();
-      if (!__any(open) && __any(top > -__builtin_huge_valf())) return;
+      for (int k = 0; k < kAhead; k++) f(there[k], score(key[k]), v[k]);
+      if (done()) return;
     }
-  }
+  };
+  // what the values hold in this lane's E columns (as Odd::bits)
+  Odd<DT> odd;
+  odd.clear();
+  const auto mine = [&] {
+    uint32_t all = odd.bits();
 #pragma unroll
-  for (int d = C; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    for (int d = C; d < 64; d *= 2) all |= (uint32_t)__shfl_xor((int)all, d);
+    return (uint32_t)__shfl((int)all, lane * E / 8) >> (lane * E % 8);
+  };
+  float top = -__builtin_huge_valf(), low = __builtin_huge_valf();
+  bool none = false;  // whether a score is no number
+  bool settled = false;
+  walk(
+      [&](bool there, float s, uint4 v) {
+        top = there ? fmaxf(top, s) : top;
+        none |= there & (s != s);
+        low = all_finite<DT>(v) ? low : fminf(low, s);
+        odd.add(v, false);
+      },
+      [&] {
+        if (__any(none)) return true;
+        bool open = false;  // a value that is NaN is so with any probability
+#pragma unroll
+        for (int i = 0; i < 4; i++) open |= __builtin_bit_cast(uint32_t, odd.nan[i]) != 0;
+        if (!__any(open) || !__any(top > -__builtin_huge_valf())) return false;
+        const uint32_t has = mine();
+        open = false;
+#pragma unroll
+        for (int e = 0; e < E; e++) open |= y[e] != y[e] && !(has >> (16 + e) & 1);
+        return settled = !__any(open);
+      });
+  if (settled) return;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d)), low = fminf(low, __shfl_xor(low, d));
   if (__any(none) || top == -__builtin_huge_valf() || top == __builtin_huge_valf()) {
     // (scores that are all -infinity give nothing a probability)
     const float all = !__any(none) && top < 0.0f ? 0.0f : __builtin_nanf("");
@@ -509,35 +557,17 @@ __device__ __forceinline__ void count_infinities(const vib3_gqa_decode& a, int r
     return;
   }
   const float scale = exponent_scale(a.scale);
-#pragma unroll 1
-  for (int i0 = 0; i0 < tokens && __any(open); i0 += kAhead * kPer) {
-    int64_t at[kAhead];
-    uint4 v[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) at[k] = place(i0 + k * kPer + lane / C);
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) v[k] = chunk(a.cache.values, at[k]);
-#pragma unroll
-    for (int k = 0; k < kAhead; k++) {
-      const uint64_t hits = __ballot(finite_only<DT>(v[k].x) != v[k].x || finite_only<DT>(v[k].y) != v[k].y ||
-                                     finite_only<DT>(v[k].z) != v[k].z || finite_only<DT>(v[k].w) != v[k].w);
-      if (hits == 0) continue;
-      const float s = score(chunk(a.cache.keys, at[k]));
-      each(hits, [&](int in) {
-        const float p = __builtin_amdgcn_exp2f((__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(s), in * C)) - top) * scale);
-        const uint16_t* value = (const uint16_t*)a.cache.values + uniform64(at[k], in * C) + head_at + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const uint16_t x = value[e];
-          const float add = p != 0.0f ? to_f32<DT>(x) : __builtin_nanf("");
-          odd[e] += finite_only<DT>(x) != x ? add : 0.0f;
-        }
-      });
-    }
-    look();
+  if (__builtin_amdgcn_exp2f((low - top) * scale) == 0.0f) {
+    odd.clear();
+    walk([&](bool, float s, uint4 v) { odd.add(v, __builtin_amdgcn_exp2f((s - top) * scale) == 0.0f); }, [] { return false; });
   }
+  const uint32_t has = mine();
 #pragma unroll
-  for (int e = 0; e < E; e++) y[e] = y[e] != y[e] && odd[e] != 0.0f ? odd[e] : y[e];
+  for (int e = 0; e < E; e++) {
+    const bool up = has >> e & 1, down = has >> (8 + e) & 1, nan = (has >> (16 + e) & 1) || (up && down);
+    const float x = nan ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf();
+    y[e] = y[e] != y[e] && (nan | up | down) ? x : y[e];
+  }
 }
 
 // `team` waves (1, 2, 4, 8 or 16) of a workgroup of WAVES join the parts of one (row, head); rows that see nothing become zero. Rows of
