@@ -25,13 +25,7 @@ __device__ __forceinline__ int gqa_len(const vib3_gqa_cache& c, int n) {
 // The first token of the window of position p.
 __device__ __forceinline__ int window_start(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
 
-// A word's two 16-bit elements with zeros in the place of infinities and NaN.
-template <int DT>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
-}
-
+// Whether eight 16-bit elements are all finite.
 template <int DT>
 __device__ __forceinline__ bool all_finite(uint4 v) {
   return finite_only<DT>(v.x) == v.x && finite_only<DT>(v.y) == v.y && finite_only<DT>(v.z) == v.z && finite_only<DT>(v.w) == v.w;

@@ -50,39 +50,6 @@ __device__ __forceinline__ void load_group_to_lds16(const void* g, uint32_t off,
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(g) : "memory", "m0");
 }
 
-// Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
-// column l % 32, element i in row 8 (i / 4) + 4 (l / 32) + i % 4.
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-template <int DT>
-__device__ __forceinline__ f32x16 mma_wide(s16x8 a, s16x8 b, f32x16 c) {
-  if (DT == VIB3_DT_F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Where chunk 0 of a row lies, for rows of C chunks: 16 (or 8) rows in a row-wise read of one chunk fall into different banks.
-template <int C>
-__device__ __forceinline__ int key_swizzle(int row) {
-  return C >= 16 ? row & 15 : (row >> 1) & 7;
-}
-
-// The same for values, of which a transposing read takes 64 bytes of each of 8 rows.
-template <int C>
-__device__ __forceinline__ int value_swizzle(int row) {
-  return C >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
-}
-
-// Maximum and sum over the lanes l and l + 32.
-__device__ __forceinline__ float pair_max(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float pair_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
 // The queries of a sequence.
 struct Queries {
   int seq, q0, nq, len;  // its row of the table, its first query, their number, its tokens

@@ -132,20 +132,6 @@ __device__ __forceinline__ int64_t uniform64(int64_t v, int i) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// Maximum and sum over the four lanes that share lane % 16.
-__device__ __forceinline__ float max_over_rows(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float sum_over_rows(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // 16 bytes of global memory, and an int that is the same in all lanes and not written while the kernel runs.
 __device__ __forceinline__ s16x8 ld_global16(uint64_t p) { return *(const __attribute__((address_space(1))) s16x8*)p; }
 __device__ __forceinline__ int ld_global4(const int32_t* p) { return *(const __attribute__((address_space(1))) int32_t*)(uint64_t)p; }

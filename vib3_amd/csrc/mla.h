@@ -128,6 +128,17 @@ __device__ __forceinline__ f32x4 mma32(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
+// column l % 32, element i in row 8 (i / 4) + 4 (l / 32) + i % 4.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ f32x16 mma_wide(s16x8 a, s16x8 b, f32x16 c) {
+  if (DT == VIB3_DT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 // Two f32 rounded to a pair of 16-bit elements (nearest even).
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -186,6 +197,49 @@ __device__ __forceinline__ s16x4 lds_read_tr(lds_u8* p) {
 
 __device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Where chunk 0 of a row lies, for rows of C chunks: 16 (or 8) rows in a row-wise read of one chunk fall into different banks.
+template <int C>
+__device__ __forceinline__ int key_swizzle(int row) {
+  return C >= 16 ? row & 15 : C == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+// The same for values, of which a transposing read takes 64 bytes of each of 8 rows.
+template <int C>
+__device__ __forceinline__ int value_swizzle(int row) {
+  return C >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+}
+
+// Maximum and sum over the lanes l and l + 32.
+__device__ __forceinline__ float pair_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// A word's two 16-bit elements with zeros in the place of infinities and NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
+}
+
+// Maximum and sum over the four lanes that share lane % 16.
+__device__ __forceinline__ float max_over_rows(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_rows(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // v as a value that the compiler does not know to be the same each time: what is formed from it is formed where it is used,

@@ -26,46 +26,6 @@ constexpr int kKeys = 64;  // keys of one step
 // What rows behind the last key are read from.
 __device__ const uint4 zero_key[128 / 8] = {};
 
-// Operand layouts of the 32x32x16 products: lane l holds row (A) or column (B) l % 32 at k = 8 (l / 32) + 0..7; of the result,
-// column l % 32, element i in row 8 (i / 4) + 4 (l / 32) + i % 4.
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-template <int DT>
-__device__ __forceinline__ f32x16 mma_wide(s16x8 a, s16x8 b, f32x16 c) {
-  if (DT == VIB3_DT_F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Where chunk 0 of a row lies, for rows of C chunks: 16 (or 8) rows in a row-wise read of one chunk fall into different banks.
-template <int C>
-__device__ __forceinline__ int key_swizzle(int row) {
-  return C == 16 ? row & 15 : C == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
-}
-
-// The same for values, of which a transposing read takes 64 bytes of each of 8 rows.
-template <int C>
-__device__ __forceinline__ int value_swizzle(int row) {
-  return C == 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
-}
-
-// Maximum and sum over the lanes l and l + 32.
-__device__ __forceinline__ float pair_max(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float pair_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
-// A word's two 16-bit elements with zeros in the place of infinities and NaN.
-template <int DT>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  constexpr uint32_t e = DT == VIB3_DT_F16 ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
-}
-
 // The queries of a workgroup: sequence, first query in it, and its queries and keys.
 struct Block {
   int q0, nq, k0, nk, first;
