@@ -702,7 +702,7 @@ int vib3_launch_gqa_decode(const vib3_gqa_decode *args, void *stream);
  * table's capacity. Offsets must not decrease (rows may be left out otherwise). */
 typedef struct vib3_gqa_chunk {
     vib3_gqa_cache cache;
-    int heads, q_tokens;               /* heads <= 1024 */
+    int heads, q_tokens;               /* heads <= 1024, q_tokens * heads < 2^31 - 256 */
     const int32_t *cu_q;               /* [num_seqs + 1] */
     const int32_t *lens;               /* [num_seqs] */
     const void *q;                     /* [q_tokens][heads][dim] */

@@ -882,7 +882,7 @@ extern "C" int vib3_launch_gqa_chunk(const vib3_gqa_chunk* args, void* stream) {
   if (const int rc = check_gqa_cache(a.cache)) return rc;
   if (!__builtin_isfinite(a.scale)) return VIB3_ERR_UNSUPPORTED;
   if (!gqa_heads(a.heads, a.cache.kv_heads) || a.q_tokens < 0 || a.window < 0 || a.sinks < 0) return VIB3_ERR_BAD_COUNT;
-  if ((int64_t)a.q_tokens * a.heads > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
+  if ((int64_t)a.q_tokens * a.heads > 0x7fffffff - 256) return VIB3_ERR_BAD_COUNT;  // so that the end of the last block is an int
   if (a.q_tokens == 0 || a.cache.num_seqs == 0) return 0;
   if (!a.cu_q || !a.lens || !mla_aligned(a.q) || !mla_aligned(a.out) || !mla_stride(a.q_token_stride) || !mla_stride(a.q_head_stride) ||
       !mla_stride(a.out_token_stride) || !mla_stride(a.out_head_stride) || !a.workspace || ((uintptr_t)a.workspace & 255))
