@@ -10,8 +10,8 @@
 // same one, which the transposing LDS reads allow). The scores of the next tile are formed next to the softmax of this one, so that
 // the matrix cores and the vector units have work of one wave at a time.
 //
-// Keys and values go straight from memory to LDS, double-buffered. Each wave looks up the pages of a tile's 64 tokens, a token a
-// lane, three tiles ahead, and hands the addresses to the lanes that load. 16-byte chunk c of an LDS row lies at c ^ a function of
+// Keys and values go straight from memory to LDS, double-buffered. Each wave looks up the pages of a tile's 64 tokens, a token (or a
+// group of them on one page) a lane, three tiles ahead for heads of 128, two for others, and hands the addresses to the lanes that load. 16-byte chunk c of an LDS row lies at c ^ a function of
 // the row, which spreads the reads over the banks.
 //
 // Many blocks: a workgroup each, the longest of a sequence first. Few blocks: long ones are cut along the tokens into pieces, which a
