@@ -70,10 +70,10 @@ __device__ __forceinline__ void copy_piece(const Pool& p, int page_size, int tok
 // ------------------------------------------------------------------------- fork
 
 // Workgroups 0..count - 1 write the children's rows of the table (in the first launch of a call), the others copy.
-__global__ __launch_bounds__(256) void k_fork_pages(vib3_fork_pages a, Pools pools, int num_pools, int pieces, int table_blocks) {
-  const int block = (int)wide_block(), b = block - table_blocks;
-  if (block < 0 || (b >= 0 && b / pieces / a.count >= num_pools)) return;
-  const int i = b < 0 ? block : b / pieces % a.count;
+__global__ __launch_bounds__(256) void k_fork_pages(vib3_fork_pages a, Pools pools, int pieces, int table_blocks, unsigned blocks) {
+  const unsigned block = wide_block();
+  if (block >= blocks) return;
+  const int b = (int)block - table_blocks, i = b < 0 ? (int)block : b / pieces % a.count;
   const int p = a.parents[i], c = a.children[i], fresh = a.new_pages[i];
   if ((unsigned)p >= (unsigned)a.num_seqs || (unsigned)c >= (unsigned)a.num_seqs) return;
   const int64_t cap = min((int64_t)a.max_pages * a.page_size, (int64_t)0x7fffffff);
@@ -282,7 +282,7 @@ extern "C" int vib3_launch_fork_pages(const vib3_fork_pages* args, void* stream)
     const int table_blocks = first == 0 ? a.count : 0;
     const int64_t blocks = table_blocks + (int64_t)a.count * n * pieces;
     if (blocks > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
-    hipLaunchKernelGGL(k_fork_pages, wide_grid(blocks), dim3(256), 0, (hipStream_t)stream, a, pools, n, pieces, table_blocks);
+    hipLaunchKernelGGL(k_fork_pages, wide_grid(blocks), dim3(256), 0, (hipStream_t)stream, a, pools, pieces, table_blocks, (unsigned)blocks);
     first += n;
   } while (first < a.num_pools);
   VIB3_RETURN_LAUNCH();
