@@ -20,9 +20,9 @@
 // itself, so a captured launch follows them.
 //
 // Measured: 12288 tokens of 32 heads over 8 of 128: 1.24 ms, 994 TFLOP/s (a library product of 8192^3: 1223, held down by the card's power),
-// 64 heads of 64 1.51 ms, 16 over 2 of 256 1.78 ms. The matrix cores are busy for 39 % of the cycles and the vector units for 55 %, and
+// 64 heads of 64 1.51 ms, 16 over 2 of 256 1.77 ms. The matrix cores are busy for 43 % of the cycles and the vector units for 50 %, and
 // the two add up: products and softmax of one wave interleaved by hand, sums a tile late, and 64 rows a wave were no faster (1.34 to 1.38
-// and, with spilled registers, 2.7 ms). 16 sequences' 4 drafted tokens of 16 heads over 2 of 256 after 317 to 5642: 36 us and 9 to join.
+// and, with spilled registers, 2.7 ms). 16 sequences' 4 drafted tokens of 16 heads over 2 of 256 after 317 to 5642: 37 us and 10 to join.
 #include <type_traits>
 
 #include "gqa.h"
@@ -570,7 +570,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 64 ? 4 : 1) void k_gqa_tiles(Chunk
             const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][i], scale, -ref));
             const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][i + 1], scale, -ref));
             l[n] += e0 + e1;
-            // rounded for the matrix cores; the sum l takes them unrounded
+            // rounded for the matrix cores; the sum l takes them unrounded. (The remainder as a second operand takes 44 % more: 12288 tokens
+            // 1284 -> 1851 us. Without it the result is off by 0.0022 in bf16 and 0.00026 in f16, rounded once by 0.0016 and 0.00021.)
             p[n][8 * b + (i >> 1)] = pack2<DT>(e0, e1);
           }
       }
@@ -844,8 +845,13 @@ int launch_chunk(const ChunkArgs& d, hipStream_t st) {
   const int64_t blocks = ((int64_t)a.q_tokens * d.group + (S::rows - 1) * seqs) / S::rows, items = blocks * a.cache.kv_heads;
   if (items > 0x7fffffff) return VIB3_ERR_BAD_COUNT;
   constexpr int kGroups = card_groups(D);
-  // Whole blocks where they fill the card some times over, or twice if none can be long: planning and the second launch cost 8 us (4096
-  // tokens of 32 heads over 8: 171 us, without 163), but one long block beside 500 short ones would have the card wait for it.
+  // Whole blocks save the plan and the second launch, but the card waits for a long one beside short ones, and the host does not know the
+  // lengths. So: whole from four blocks a place on the card, and from two where none can see more than 96 tiles. Measured with 32 heads
+  // over 8 of 128, us whole / cut:
+  //   one prompt   80 / 88 (2048 tokens, one block a place: cut, for what may lie beside it), 185 / 200 (4096, two), 363 / 377 (6144, three
+  //                of 96 tiles), 463 / 477 (7168, 3.5 of 112 tiles), 590 / 603 (8192, four)
+  //   16 tokens after 6000 (94 tiles) beside prompts of 200   145 / 98 (24 of them, three blocks a place), 156 / 172 (48, six)
+  //   the same after 30000                                    673 / 125 and 675 / 200: the 96 keeps the first of them cut, the last is not
   int64_t longest = (int64_t)a.cache.max_pages * a.cache.page_size;
   if (a.window > 0 && (int64_t)a.window + a.sinks + S::rows / d.group < longest) longest = (int64_t)a.window + a.sinks + S::rows / d.group;
   if (items >= (longest <= 96 * kTile ? 2 : 4) * kGroups || blocks > kMaxBlocks || a.cache.num_seqs > kMaxBlocks) {
