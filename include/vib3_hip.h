@@ -684,7 +684,7 @@ typedef struct vib3_gqa_decode {
     int64_t q_row_stride, q_head_stride;
     float scale;
     int window, sinks;                 /* window 0: none */
-    void *out;                         /* [rows][heads][dim] */
+    void *out;                         /* [rows][heads][dim], no part of q */
     int64_t out_row_stride, out_head_stride;
     void *workspace;                   /* vib3_gqa_decode_workspace_bytes() bytes, 256-byte
                                           aligned; calls that may overlap need one each */
@@ -709,7 +709,7 @@ typedef struct vib3_gqa_chunk {
     int64_t q_token_stride, q_head_stride;
     float scale;
     int window, sinks;                 /* window 0: none */
-    void *out;                         /* [q_tokens][heads][dim] */
+    void *out;                         /* [q_tokens][heads][dim], no part of q */
     int64_t out_token_stride, out_head_stride;
     void *workspace;                   /* vib3_gqa_chunk_workspace_bytes() bytes, 256-byte
                                           aligned; calls that may overlap need one each */
