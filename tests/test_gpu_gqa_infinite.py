@@ -40,9 +40,8 @@ def check(c, q, got, pos, at, gap, window=0, sinks=0):
     close(got[~sees], want[~sees], tol[~sees], "queries that do not see it")
 
 
-@pytest.mark.parametrize("gap", [22.0, 40.0, 84.0, 120.0])
-@pytest.mark.parametrize("whole,at,window,sinks", [(True, 10, 0, 0), (True, 150, 0, 0), (True, 70, 200, 0), (False, 150, 0, 0), (False, 3, 100, 5),
-                                                   (False, 299, 0, 0)])
+@pytest.mark.parametrize("gap", [40.0, 84.0, 120.0])
+@pytest.mark.parametrize("whole,at,window,sinks", [(True, 10, 0, 0), (True, 150, 200, 0), (False, 150, 0, 0), (False, 3, 100, 5)])
 @pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_chunk(dtype, heads, kv_heads, dim, whole, at, window, sinks, gap):
@@ -52,8 +51,8 @@ def test_chunk(dtype, heads, kv_heads, dim, whole, at, window, sinks, gap):
     check(c, q, got, torch.arange(n, device="cuda"), at, gap, window, sinks)
 
 
-@pytest.mark.parametrize("gap", [22.0, 40.0, 84.0, 120.0])
-@pytest.mark.parametrize("n,at,ps", [(40, 7, 16), (400, 399, 7), (3000, 0, 16), (9000, 5000, 64)])
+@pytest.mark.parametrize("gap", [40.0, 84.0, 120.0])
+@pytest.mark.parametrize("n,at,ps", [(40, 7, 16), (400, 399, 7), (9000, 5000, 64)])
 @pytest.mark.parametrize("heads,kv_heads,dim", SHAPES + [(17, 1, 128)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_decode(dtype, heads, kv_heads, dim, n, at, ps, gap):
