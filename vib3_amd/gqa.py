@@ -127,7 +127,7 @@ class GqaDecode(_Attention):
                seqs: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Row r of q [rows, heads, dim] is the newest of the first lens[r] cached tokens of sequence seqs[r] (None: sequence r;
         int32 [rows]) and sees those or, with a window, the newest `window` and the first `sinks` of them. Returns out
-        [rows, heads, dim] (default: the head of self.out)."""
+        [rows, heads, dim] (default: the head of self.out), which is no part of q."""
         c = self.cache
         rows, qs, outs, out = self._to(q, out, self.max_rows)
         desc = c._desc(block_table)
@@ -156,7 +156,8 @@ class GqaChunk(_Attention):
                window: int = 0, sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Sequence s (a row of block_table) has the queries cu_q[s]..cu_q[s + 1] of q [tokens, heads, dim] (int32 [seqs + 1]), the
         newest of its first lens[s] cached tokens (int32 [seqs]). Each sees the tokens up to its own or, with a window, the
-        newest `window` and the first `sinks` of them. Returns out [tokens, heads, dim] (default: the head of self.out)."""
+        newest `window` and the first `sinks` of them. Returns out [tokens, heads, dim] (default: the head of self.out), which is no
+        part of q."""
         c = self.cache
         tokens, qs, outs, out = self._to(q, out, self.max_tokens)
         desc = c._desc(block_table)
